@@ -403,6 +403,162 @@ wm_status wm_server_result(wm_server *s, uint64_t request_id, uint32_t *out_ids,
 /* Forget a request (finished or not); its cache returns to the pool. */
 wm_status wm_server_release(wm_server *s, uint64_t request_id);
 
+/* ---- paged 8-bit KV cache and token scores ---------------------------- */
+
+/* No counterpart in the reference (its KVCache is one buffer per sequence
+ * with a scale per position, src/model/kv_cache.rs:41-54): a cache in pages
+ * that any number of sequences share, for one layer, and the attention that
+ * reads it.  All arithmetic is f32 or wider; the results are those of the
+ * formulas below up to rounding, not tied to a summation order.
+ *
+ * Every pointer in these structs is device memory of the caller, which the
+ * library reads or writes only during the work it enqueues on the context's
+ * stream.  The lengths and the page table are read on the device, so a
+ * captured graph follows them; the host values max_new and max_kv_len bound
+ * them.  Contents the host cannot check never lead outside the buffers:
+ * see each call, and wm_paged_batch_check for a check on host copies. */
+
+/* Element types of activations and logits: GGML type ids (src/gguf/types.rs:14-60). */
+typedef enum wm_dtype {
+    WM_DTYPE_F32 = 0,
+    WM_DTYPE_F16 = 1,
+    WM_DTYPE_BF16 = 30
+} wm_dtype;
+
+/* One layer's page pool.  A page holds page_size positions (16, 32 or 64) of
+ * every kv head; the block of one head in one page is int8 codes and one f32
+ * scale for K and one for V: value = code * scale.  head_dim is 64 or 128.
+ * The code arrays are 16-byte aligned. */
+typedef struct wm_paged_kv {
+    int8_t *k_codes;  /* [n_pages][n_kv_heads][page_size][head_dim] */
+    int8_t *v_codes;  /* [n_pages][n_kv_heads][head_dim][page_size]: positions innermost */
+    float *k_scales;  /* [n_pages][n_kv_heads] */
+    float *v_scales;  /* [n_pages][n_kv_heads] */
+    uint32_t n_pages;
+    uint32_t page_size;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;
+} wm_paged_kv;
+
+/* A step's sequences.  Sequence i has n = cu_tokens[i+1] - cu_tokens[i] of
+ * the step's packed tokens; kv_len[i] counts its positions with these n
+ * included, so its token j is at position kv_len[i] - n + j, which lives in
+ * page page_table[i * table_stride + position / page_size].  Tokens from
+ * cu_tokens[n_seqs] to n_tokens are padding: no output of theirs is written.
+ * A token whose position is negative (kv_len[i] < n) has no place in the
+ * cache: it is not appended, and its attention row is empty. */
+typedef struct wm_paged_batch {
+    const int32_t *cu_tokens;  /* n_seqs + 1, non-decreasing from 0 */
+    const int32_t *kv_len;     /* n_seqs */
+    const int32_t *page_table; /* [n_seqs][table_stride] */
+    uint32_t n_seqs;
+    uint32_t table_stride;     /* table_stride * page_size >= max_kv_len */
+    uint32_t n_tokens;         /* rows of the packed arrays */
+    uint32_t max_new;          /* bounds every n */
+    uint32_t max_kv_len;       /* bounds every kv_len */
+} wm_paged_batch;
+
+/* Rotary positions: the first n_rot dims (a multiple of 8, at most head_dim)
+ * of each head are rotated in pairs by the angle whose cosine and sine are
+ * cos[position * n_rot / 2 + i], sin[...] (any base or scaling of the angles
+ * is in the tables; n_pos >= max_kv_len rows). */
+typedef enum wm_rope_layout {
+    WM_ROPE_HALF = 0,       /* pairs (i, i + n_rot / 2): NEOX (src/model/primitives.rs:326-341) */
+    WM_ROPE_INTERLEAVED = 1 /* pairs (2i, 2i + 1) */
+} wm_rope_layout;
+typedef struct wm_rope {
+    const float *cos; /* [n_pos][n_rot / 2], 16-byte aligned */
+    const float *sin;
+    uint32_t n_pos;
+    uint32_t n_rot;
+    uint32_t layout;  /* wm_rope_layout */
+} wm_rope;
+
+/* Checks host copies of a step's arrays (host-only, no device needed):
+ * cu_tokens non-decreasing from 0 and within n_tokens and max_new, kv_len
+ * within 0 and max_kv_len, every page the step reads or writes within the
+ * pool, and, with `appends` != 0, every page the append writes written by
+ * one sequence only and read by no other.  WM_E_ARG (null pointer, a bound
+ * of the structs themselves), WM_E_SHAPE (lengths), WM_E_BOUNDS (pages); the
+ * device pointers in `kv` and `batch` are not looked at. */
+wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batch,
+                               const int32_t *cu_tokens, const int32_t *kv_len,
+                               const int32_t *page_table, int appends);
+
+/* Append a step's keys and values, rotated on the way, and rotate its
+ * queries.  q [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads]
+ * [head_dim] of `type` (wm_dtype), tokens q_stride, k_stride and v_stride
+ * elements apart (parts of one fused row are fine); q_out like q (may be q
+ * itself).  n_heads = 0: no queries (q and q_out may be null).  rope null: no
+ * rotation.  Pointers are 16-byte aligned and strides a multiple of 16 bytes.
+ *
+ * With r the rotated key (exact products and sum, rounded once to f32) or
+ * the value, a block (page, head) that receives tokens gets
+ *   scale = max(its scale before, if positions before this step's first lie
+ *               in it, else 0;  f32(max |r| over the finite new r / 127)),
+ *   new codes  r / scale rounded half away from zero, within +-127
+ *              (NaN: 0; scale 0: 0),
+ *   and, where the scale grew, its earlier codes c * old scale / scale
+ *   rounded the same way.
+ * The quotients are rounded exactly.  Positions behind the last are left as
+ * they were.  q_out is the rotated query rounded once to its type.
+ * A sequence whose lengths break their bounds is skipped; tokens of a page
+ * outside the pool are not stored.  Two sequences must not append into one
+ * page. */
+wm_status wm_paged_kv_append_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch,
+                                 const wm_rope *rope, int type, const void *d_q, uint64_t q_stride,
+                                 uint32_t n_heads, const void *d_k, uint64_t k_stride, const void *d_v,
+                                 uint64_t v_stride, void *d_q_out, uint64_t q_out_stride);
+
+/* The cache's values at the batch's tokens' positions (the paged form of
+ * KVCache::read_into, src/model/kv_cache.rs:192-219): k_out and v_out
+ * [n_tokens][n_kv_heads][head_dim] of `type`, code * scale in f32, rounded
+ * once.  Either may be null.  Nothing is written for a sequence whose lengths
+ * break their bounds or a token without a position; a page outside the pool
+ * reads as NaN.  Alignment as above. */
+wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
+                               void *d_k_out, uint64_t k_stride, void *d_v_out, uint64_t v_stride);
+
+/* Causal attention of the batch's tokens over the cache, K and V of the
+ * tokens themselves included (append first).  Query head h reads kv head
+ * h / (n_heads / n_kv_heads).  For a token at position p:
+ *   s_j = scale * q . k_j (j <= p),  out = sum_j softmax(s)_j v_j,
+ *   lse = ln sum_j exp(s_j)  (d_lse [n_tokens][n_heads] f32, nullable).
+ * A row without positions gives 0 and lse -inf.  A row that reads a page
+ * outside the pool, or a sequence whose lengths break their bounds, gives NaN.
+ * q and out are of `type`, as in the append; out may be q.
+ * work: wm_paged_attention_workspace bytes, 16-byte aligned, overwritten;
+ * calls that may run at the same time (graphs replayed on two streams) need
+ * one each.  The workspace grows with the batch's host bounds only. */
+size_t wm_paged_attention_workspace(const wm_paged_kv *kv, const wm_paged_batch *batch, uint32_t n_heads);
+wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
+                                 const void *d_q, uint64_t q_stride, uint32_t n_heads, float scale, void *d_out,
+                                 uint64_t out_stride, float *d_lse, void *d_work, size_t work_bytes);
+
+/* Log probabilities of given tokens under rows of logits (of `type`,
+ * row_stride elements apart, any alignment of the element): per row x with
+ * token t
+ *   logprob = x_t - ln sum_j exp(x_j),   entropy = -sum_j p_j ln p_j,
+ *   rank    = how many tokens come before t by (logit descending, id),
+ *   top_ids, top_logprobs [n_rows][top_k]: the first top_k tokens in that
+ *             order (top_k <= 64 and <= vocab).
+ * Each output may be null (top_ids and top_logprobs must be when top_k is 0).
+ * -inf logits count as probability 0; a row of only -inf gives logprob -inf
+ * and entropy 0.  A row that holds NaN or +inf gives NaN for its
+ * log probabilities and entropy (NaN sorts below every number).  A token
+ * outside the vocabulary gives logprob NaN and rank -1; with tokens null,
+ * logprob and rank must be null.
+ * work: wm_token_logprobs_workspace bytes, 16-byte aligned, as above. */
+size_t wm_token_logprobs_workspace(uint32_t n_rows, uint32_t vocab, uint32_t top_k);
+wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uint64_t row_stride, uint32_t n_rows,
+                                uint32_t vocab, const int32_t *d_tokens, uint32_t top_k, float *d_logprob,
+                                float *d_entropy, int32_t *d_rank, int32_t *d_top_ids, float *d_top_logprobs,
+                                void *d_work, size_t work_bytes);
+/* Host-slice form (f32 rows of `vocab` values; copies, runs, copies back). */
+wm_status wm_token_logprobs(wm_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t vocab,
+                            const int32_t *tokens, uint32_t top_k, float *logprob, float *entropy, int32_t *rank,
+                            int32_t *top_ids, float *top_logprobs);
+
 /* ---- GGUF files (src/gguf/reader.rs, src/model/graph.rs) ------------- */
 
 /* GgufFile::parse (src/gguf/reader.rs:120-415): the header, metadata and

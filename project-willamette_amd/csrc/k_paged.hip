@@ -1,0 +1,518 @@
+// The paged 8-bit KV cache: append with the rotation applied, read back.
+//
+// A block is one kv head's positions in one page, with one scale for K and
+// one for V.  One workgroup serves one block of one sequence: it owns the
+// block for the launch (two sequences may not append into one page), so the
+// maximum, the codes and the scale need no exchange between workgroups.
+#include <cstdio>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "wm_paged.h"
+
+namespace {
+
+constexpr int NT = 256;  // threads per workgroup, four waves
+
+// Quotient a / s of two f32 (s > 0) rounded half away from zero, within
+// +-127, exactly: inv = 1 / s in f64 makes |a| * inv good to 2^-51 relative.
+// A quotient that is no tie lies at least 2^-33 away from one (a and (k + .5) s
+// differ by 2^-32 of either at least: both have 32 bits), so adding 2^-40
+// takes the ties up and nothing else.
+__device__ __forceinline__ int quotient_code(float a, double inv) {
+    const double t = fabs((double)a) * inv + (0.5 + 0x1p-40);
+    const int m = t < 127.0 ? (int)t : (t >= 127.0 ? 127 : 0);  // NaN: 0
+    return a < 0.0f ? -m : m;
+}
+__device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {
+    return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | (uint32_t)d << 24;
+}
+__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(w << (24 - 8 * i)) >> 24; }
+// Earlier codes under a grown scale: c * s_old is exact in f32's products
+// only as f64 (7 + 24 bits), so the quotient is rounded the same way.
+__device__ __forceinline__ int rescale_code(int c, double ratio) {
+    const double t = fabs((double)c) * ratio + (0.5 + 0x1p-40);
+    const int m = t < 127.0 ? (int)t : 127;
+    return c < 0 ? -m : m;
+}
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, double ratio) {
+    return pack_codes(rescale_code(byte_of(w, 0), ratio), rescale_code(byte_of(w, 1), ratio),
+                      rescale_code(byte_of(w, 2), ratio), rescale_code(byte_of(w, 3), ratio));
+}
+
+// |v| where v is finite, else 0.
+__device__ __forceinline__ float finite_abs(float v) {
+    const float a = fabsf(v);
+    return a <= 3.402823466e38f ? a : 0.0f;
+}
+__device__ __forceinline__ float finite_abs4(wm_f4 v) {
+    return fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+}
+
+// A head is taken in units of 8 dims, as two runs of 4 that hold whole
+// pairs: unit u < n_rot / 8 of the half layout is (4u.., n_rot / 2 + 4u..),
+// every other unit 8 dims in a row.
+struct unit_dims {
+    int a, b;
+    bool rot;
+};
+__device__ __forceinline__ unit_dims dims_of(int u, int n_rot, bool half) {
+    unit_dims d;
+    d.rot = 8 * u < n_rot;
+    const bool split = d.rot && half;
+    d.a = split ? 4 * u : 8 * u;
+    d.b = split ? n_rot / 2 + 4 * u : 8 * u + 4;
+    return d;
+}
+// The rotation of one unit's four pairs, products and sums exact in f64
+// (48-bit products, one rounding of their sum), rounded to f32.
+__device__ __forceinline__ float rot_lo(float x, float y, float c, float s) {
+    return (float)__builtin_fma((double)x, (double)c, -((double)y * (double)s));
+}
+__device__ __forceinline__ float rot_hi(float x, float y, float c, float s) {
+    return (float)__builtin_fma((double)y, (double)c, (double)x * (double)s);
+}
+__device__ __forceinline__ void rotate_unit(wm_f4 &a, wm_f4 &b, wm_f4 c, wm_f4 s, bool half) {
+    if (half) {
+        wm_f4 x = a, y = b;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            a[i] = rot_lo(x[i], y[i], c[i], s[i]);
+            b[i] = rot_hi(x[i], y[i], c[i], s[i]);
+        }
+    } else {
+        wm_f4 x = a, y = b;
+        a[0] = rot_lo(x[0], x[1], c[0], s[0]);
+        a[1] = rot_hi(x[0], x[1], c[0], s[0]);
+        a[2] = rot_lo(x[2], x[3], c[1], s[1]);
+        a[3] = rot_hi(x[2], x[3], c[1], s[1]);
+        b[0] = rot_lo(y[0], y[1], c[2], s[2]);
+        b[1] = rot_hi(y[0], y[1], c[2], s[2]);
+        b[2] = rot_lo(y[2], y[3], c[3], s[3]);
+        b[3] = rot_hi(y[2], y[3], c[3], s[3]);
+    }
+}
+
+struct append_args {
+    wm_paged_kv kv;
+    wm_paged_batch b;
+    wm_rope rope;  // n_rot 0: none
+    const void *q, *k, *v;
+    void *q_out;
+    uint64_t qs, ks, vs, qos;  // elements between tokens
+    uint32_t group;            // query heads per kv head (0: no queries)
+    uint32_t touch;            // pages a sequence can touch, at most
+};
+
+// One block's place in the step: sequence s, its page lp, kv head h.
+struct block_place {
+    wm_seq q;
+    int lp, h, page;
+    bool live, stored;  // positions of the step lie in it; its page is in the pool
+};
+__device__ __forceinline__ block_place place_block(const wm_paged_kv &kv, const wm_paged_batch &b, uint32_t touch,
+                                                   uint32_t id) {
+    block_place p;
+    p.h = id % kv.n_kv_heads;
+    const uint32_t sm = id / kv.n_kv_heads, s = sm / touch;
+    p.q = wm_load_seq(b, s);
+    p.lp = max(p.q.start, 0) / (int)kv.page_size + (int)(sm % touch);
+    p.live = p.q.ok && p.q.n > 0 && (int64_t)p.lp * kv.page_size < p.q.len;
+    p.page = p.live ? b.page_table[(uint64_t)s * b.table_stride + p.lp] : -1;
+    p.stored = p.page >= 0 && (uint32_t)p.page < kv.n_pages;
+    return p;
+}
+
+// Append.  Bound by the bytes of q, k, v in and q out (the codes are a
+// quarter of f32's), and for a decode step by latency: the chain is lengths,
+// page id, old scale, and the earlier codes of a block are loaded with the
+// scale, before it is known whether they change.  Thread units: K (position,
+// 8 dims), V (4 positions, 4 dims) so that its transposed codes leave as
+// whole dwords.
+template <typename T, int PS, int D>
+__global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
+    constexpr int NK = (PS * D / 8 + NT - 1) / NT;   // K units per thread
+    constexpr int NV = (PS * D / 16 + NT - 1) / NT;  // V units per thread
+    __shared__ float red[2][NT / 64];
+    const block_place p = place_block(a.kv, a.b, a.touch, blockIdx.x);
+    if (!p.live) return;
+    const int tid = threadIdx.x, n_rot = (int)a.rope.n_rot;
+    const bool half = a.rope.layout == WM_ROPE_HALF;
+    const int base = p.lp * PS;  // first position of the page
+    const int lo = max(p.q.start, 0) - base, hi = min(p.q.len - base, PS);  // its new slots: [max(lo, 0), hi)
+    const int first = max(lo, 0);
+    const int64_t tok = (int64_t)p.q.tok0 + base - p.q.start;  // packed token of slot 0
+    const uint64_t blk = (uint64_t)(p.stored ? p.page : 0) * a.kv.n_kv_heads + p.h;
+    int8_t *kc = a.kv.k_codes + blk * (PS * D), *vc = a.kv.v_codes + blk * (PS * D);
+    const T *k = (const T *)a.k + (uint64_t)p.h * D, *v = (const T *)a.v + (uint64_t)p.h * D;
+    float sk_old = 0.0f, sv_old = 0.0f;
+    if (first > 0 && p.stored) sk_old = a.kv.k_scales[blk], sv_old = a.kv.v_scales[blk];
+
+    wm_f4 ka[NK], kb[NK];
+    uint32_t oa[NK], ob[NK];
+    float mk = 0.0f, mv = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+        const int unit = tid + i * NT, slot = unit / (D / 8);
+        const unit_dims d = dims_of(unit % (D / 8), n_rot, half);
+        ka[i] = kb[i] = wm_f4{0, 0, 0, 0};
+        oa[i] = ob[i] = 0;
+        if (unit >= PS * D / 8) continue;
+        if (slot >= first && slot < hi) {
+            const T *row = k + (uint64_t)(tok + slot) * a.ks;
+            ka[i] = wm_ld4(row + d.a);
+            kb[i] = wm_ld4(row + d.b);
+        } else if (slot < first && p.stored) {
+            oa[i] = *(const uint32_t *)(kc + slot * D + d.a);
+            ob[i] = *(const uint32_t *)(kc + slot * D + d.b);
+        }
+    }
+    wm_f4 vv[NV][4];
+    uint32_t ov[NV][4];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; j++) vv[i][j] = wm_f4{0, 0, 0, 0}, ov[i][j] = 0;
+        if (unit >= PS * D / 16 || quad >= hi) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (quad + j >= first && quad + j < hi) vv[i][j] = wm_ld4(v + (uint64_t)(tok + quad + j) * a.vs + dim);
+        if ((quad < first || quad + 4 > hi) && p.stored) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) ov[i][j] = *(const uint32_t *)(vc + (dim + j) * PS + quad);
+        }
+    }
+    if (a.group) {
+        const int n_units = (hi - first) * (int)a.group * (D / 8);
+        for (int w = tid; w < n_units; w += NT) {
+            const int u = w % (D / 8), hg = w / (D / 8), slot = first + hg / (int)a.group;
+            const uint64_t head = (uint64_t)p.h * a.group + hg % a.group;
+            const unit_dims d = dims_of(u, n_rot, half);
+            const T *row = (const T *)a.q + (uint64_t)(tok + slot) * a.qs + head * D;
+            T *out = (T *)a.q_out + (uint64_t)(tok + slot) * a.qos + head * D;
+            wm_f4 x = wm_ld4(row + d.a), y = wm_ld4(row + d.b);
+            if (d.rot) {
+                const uint64_t at = (uint64_t)(base + slot) * (n_rot / 2) + 4 * u;
+                rotate_unit(x, y, *(const wm_f4 *)(a.rope.cos + at), *(const wm_f4 *)(a.rope.sin + at), half);
+            }
+            wm_st4(out + d.a, x);
+            wm_st4(out + d.b, y);
+        }
+    }
+    if (!p.stored) return;
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+        const int unit = tid + i * NT, slot = unit / (D / 8), u = unit % (D / 8);
+        if (unit < PS * D / 8 && slot >= first && slot < hi) {
+            if (8 * u < n_rot) {
+                const uint64_t at = (uint64_t)(base + slot) * (n_rot / 2) + 4 * u;
+                rotate_unit(ka[i], kb[i], *(const wm_f4 *)(a.rope.cos + at), *(const wm_f4 *)(a.rope.sin + at), half);
+            }
+            mk = fmaxf(mk, fmaxf(finite_abs4(ka[i]), finite_abs4(kb[i])));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) mv = fmaxf(mv, finite_abs4(vv[i][j]));
+    mk = wm_wave_max_nonneg(mk);
+    mv = wm_wave_max_nonneg(mv);
+    if ((tid & 63) == 0) red[0][tid >> 6] = mk, red[1][tid >> 6] = mv;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) mk = fmaxf(mk, red[0][w]), mv = fmaxf(mv, red[1][w]);
+    const float sk = fmaxf(sk_old, (float)((double)mk / 127.0)), sv = fmaxf(sv_old, (float)((double)mv / 127.0));
+    const double ik = sk > 0.0f ? 1.0 / (double)sk : 0.0, iv = sv > 0.0f ? 1.0 / (double)sv : 0.0;
+    const bool grew_k = sk > sk_old && first > 0, grew_v = sv > sv_old && first > 0;
+    const double rk = (double)sk_old * ik, rv = (double)sv_old * iv;
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+        const int unit = tid + i * NT, slot = unit / (D / 8);
+        const unit_dims d = dims_of(unit % (D / 8), n_rot, half);
+        if (unit >= PS * D / 8) continue;
+        uint32_t *wa = (uint32_t *)(kc + slot * D + d.a), *wb = (uint32_t *)(kc + slot * D + d.b);
+        if (slot >= first && slot < hi) {
+            *wa = pack_codes(quotient_code(ka[i].x, ik), quotient_code(ka[i].y, ik), quotient_code(ka[i].z, ik),
+                             quotient_code(ka[i].w, ik));
+            *wb = pack_codes(quotient_code(kb[i].x, ik), quotient_code(kb[i].y, ik), quotient_code(kb[i].z, ik),
+                             quotient_code(kb[i].w, ik));
+        } else if (slot < first && grew_k) {
+            *wa = rescale4(oa[i], rk);
+            *wb = rescale4(ob[i], rk);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
+        if (unit >= PS * D / 16 || quad >= hi || (quad + 4 <= first && !grew_v)) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {  // dim + j of four positions
+            const uint32_t old = ov[i][j], kept = grew_v ? rescale4(old, rv) : old;
+            uint32_t w = 0;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const uint32_t mask = 255u << (8 * t);
+                const int slot = quad + t;
+                const uint32_t fresh = (uint32_t)(quotient_code(vv[i][t][j], iv) & 255) << (8 * t);
+                w |= slot < first ? kept & mask : slot < hi ? fresh : old & mask;
+            }
+            *(uint32_t *)(vc + (dim + j) * PS + quad) = w;
+        }
+    }
+    if (tid == 0) a.kv.k_scales[blk] = sk, a.kv.v_scales[blk] = sv;
+}
+
+struct read_args {
+    wm_paged_kv kv;
+    wm_paged_batch b;
+    void *k, *v;
+    uint64_t ks, vs;
+    uint32_t touch;
+};
+
+__device__ __forceinline__ wm_f4 values4(uint32_t w, float s) {
+    return wm_f4{(float)byte_of(w, 0) * s, (float)byte_of(w, 1) * s, (float)byte_of(w, 2) * s, (float)byte_of(w, 3) * s};
+}
+
+// Read back: bound by its output bytes.  A unit is 4 positions x 4 dims: K's
+// rows are a dword each, V's transposed through the unit's 16 bytes.
+template <typename T, int PS, int D>
+__global__ __launch_bounds__(NT) void k_paged_read(read_args a) {
+    const block_place p = place_block(a.kv, a.b, a.touch, blockIdx.x);
+    if (!p.live) return;
+    const int base = p.lp * PS, first = max(max(p.q.start, 0) - base, 0), hi = min(p.q.len - base, PS);
+    const int64_t tok = (int64_t)p.q.tok0 + base - p.q.start;
+    const uint64_t blk = (uint64_t)(p.stored ? p.page : 0) * a.kv.n_kv_heads + p.h;
+    const int8_t *kc = a.kv.k_codes + blk * (PS * D), *vc = a.kv.v_codes + blk * (PS * D);
+    const float nan = __uint_as_float(0x7FC00000u);
+    const float sk = p.stored ? a.kv.k_scales[blk] : nan, sv = p.stored ? a.kv.v_scales[blk] : nan;
+    for (int unit = threadIdx.x; unit < PS * D / 16; unit += NT) {
+        const int quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
+        if (quad + 4 <= first || quad >= hi) continue;
+        uint32_t wk[4], wv[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            wk[j] = *(const uint32_t *)(kc + (quad + j) * D + dim);
+            wv[j] = *(const uint32_t *)(vc + (dim + j) * PS + quad);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int slot = quad + t;
+            if (slot < first || slot >= hi) continue;
+            const uint64_t row = (uint64_t)(tok + slot);
+            if (a.k) wm_st4((T *)a.k + row * a.ks + (uint64_t)p.h * D + dim, values4(wk[t], sk));
+            const uint32_t col = pack_codes(byte_of(wv[0], t), byte_of(wv[1], t), byte_of(wv[2], t), byte_of(wv[3], t));
+            if (a.v) wm_st4((T *)a.v + row * a.vs + (uint64_t)p.h * D + dim, values4(col, sv));
+        }
+    }
+}
+
+// Pages one sequence of the step can touch, at most: its tokens and the
+// positions before its first in the same page.
+uint32_t touched_pages(const wm_paged_kv *kv, const wm_paged_batch *b) {
+    const uint64_t most = b->max_new < b->max_kv_len ? b->max_new : b->max_kv_len;
+    return most ? (uint32_t)((most + 2 * kv->page_size - 2) / kv->page_size) : 0;
+}
+wm_status block_grid(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t *grid) {
+    const uint64_t n = (uint64_t)touched_pages(kv, b) * b->n_seqs * kv->n_kv_heads;
+    if (n > 0x7FFFFFFFull / NT)  // the launch counts threads in 32 bits
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu blocks in one step", who, (unsigned long long)n);
+    *grid = (uint32_t)n;
+    return WM_OK;
+}
+
+template <typename T, int PS, int D> struct launch_append {
+    static void go(const append_args &a, uint32_t grid, hipStream_t s) {
+        k_paged_append<T, PS, D><<<grid, NT, 0, s>>>(a);
+    }
+};
+template <typename T, int PS, int D> struct launch_read {
+    static void go(const read_args &a, uint32_t grid, hipStream_t s) { k_paged_read<T, PS, D><<<grid, NT, 0, s>>>(a); }
+};
+template <template <typename, int, int> class L, typename T, typename A>
+void by_page(uint32_t ps, uint32_t d, const A &a, uint32_t grid, hipStream_t s) {
+    if (d == 64) {
+        if (ps == 16) L<T, 16, 64>::go(a, grid, s);
+        else if (ps == 32) L<T, 32, 64>::go(a, grid, s);
+        else L<T, 64, 64>::go(a, grid, s);
+    } else {
+        if (ps == 16) L<T, 16, 128>::go(a, grid, s);
+        else if (ps == 32) L<T, 32, 128>::go(a, grid, s);
+        else L<T, 64, 128>::go(a, grid, s);
+    }
+}
+template <template <typename, int, int> class L, typename A>
+void by_shape(int type, uint32_t ps, uint32_t d, const A &a, uint32_t grid, hipStream_t s) {
+    if (type == WM_DTYPE_F32) by_page<L, float>(ps, d, a, grid, s);
+    else if (type == WM_DTYPE_F16) by_page<L, _Float16>(ps, d, a, grid, s);
+    else by_page<L, __bf16>(ps, d, a, grid, s);
+}
+
+// The fields that need no device; the message goes to `msg`.
+wm_status check_fields(const wm_paged_kv *kv, const wm_paged_batch *b, char *msg, size_t n) {
+    if (!kv || !b) return snprintf(msg, n, "null descriptor"), WM_E_ARG;
+    if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64)
+        return snprintf(msg, n, "page_size %u is not 16, 32 or 64", kv->page_size), WM_E_SHAPE;
+    if (kv->head_dim != 64 && kv->head_dim != 128)
+        return snprintf(msg, n, "head_dim %u is not 64 or 128", kv->head_dim), WM_E_SHAPE;
+    if (kv->n_kv_heads == 0 || kv->n_kv_heads > 65536)
+        return snprintf(msg, n, "%u kv heads", kv->n_kv_heads), WM_E_SHAPE;
+    if (kv->n_pages == 0 || kv->n_pages > 0x7FFFFFFFu)
+        return snprintf(msg, n, "%u pages", kv->n_pages), WM_E_SHAPE;
+    if (b->n_tokens > 0x7FFFFFFFu || b->n_seqs > 0x7FFFFFFEu || b->max_kv_len > 1u << 30)
+        return snprintf(msg, n, "n_tokens %u, n_seqs %u or max_kv_len %u is too large", b->n_tokens, b->n_seqs,
+                        b->max_kv_len), WM_E_SHAPE;
+    if (b->max_new > b->n_tokens)
+        return snprintf(msg, n, "max_new %u is above n_tokens %u", b->max_new, b->n_tokens), WM_E_SHAPE;
+    if ((uint64_t)b->table_stride * kv->page_size < b->max_kv_len)
+        return snprintf(msg, n, "table_stride %u pages of %u hold fewer than max_kv_len %u positions", b->table_stride,
+                        kv->page_size, b->max_kv_len), WM_E_SHAPE;
+    return WM_OK;
+}
+
+}  // namespace
+
+size_t wm_dtype_size(int type) {
+    return type == WM_DTYPE_F32 ? 4 : type == WM_DTYPE_F16 || type == WM_DTYPE_BF16 ? 2 : 0;
+}
+
+wm_status wm_paged_check(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const wm_paged_batch *b) {
+    char msg[160];
+    if (wm_status st = check_fields(kv, b, msg, sizeof msg)) return wm_set_error(ctx, st, "%s: %s", who, msg);
+    if (!kv->k_codes || !kv->v_codes || !kv->k_scales || !kv->v_scales)
+        return wm_set_error(ctx, WM_E_ARG, "%s: null page pool", who);
+    if (((uintptr_t)kv->k_codes | (uintptr_t)kv->v_codes) % 16 || ((uintptr_t)kv->k_scales | (uintptr_t)kv->v_scales) % 4)
+        return wm_set_error(ctx, WM_E_ARG, "%s: misaligned page pool", who);
+    if (b->n_seqs && (!b->cu_tokens || !b->kv_len || (!b->page_table && b->max_kv_len)))
+        return wm_set_error(ctx, WM_E_ARG, "%s: null lengths or page table", who);
+    if (((uintptr_t)b->cu_tokens | (uintptr_t)b->kv_len | (uintptr_t)b->page_table) % 4)
+        return wm_set_error(ctx, WM_E_ARG, "%s: misaligned lengths or page table", who);
+    return WM_OK;
+}
+
+wm_status wm_paged_check_array(wm_ctx *ctx, const char *who, const char *name, const void *p, uint64_t stride,
+                               uint32_t heads, uint32_t head_dim, size_t elem) {
+    if (!p) return wm_set_error(ctx, WM_E_ARG, "%s: null %s", who, name);
+    if ((uintptr_t)p % 16 || stride * elem % 16)
+        return wm_set_error(ctx, WM_E_ARG, "%s: %s and its rows must be 16-byte aligned", who, name);
+    if (stride < (uint64_t)heads * head_dim || stride > 1ull << 40)
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %s rows of %u x %u values are %llu apart", who, name, heads, head_dim,
+                            (unsigned long long)stride);
+    return WM_OK;
+}
+
+extern "C" {
+
+wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *b, const int32_t *cu_tokens,
+                               const int32_t *kv_len, const int32_t *page_table, int appends) {
+    char msg[160];
+    if (wm_status st = check_fields(kv, b, msg, sizeof msg)) return st;
+    if (b->n_seqs == 0) return WM_OK;
+    if (!cu_tokens || !kv_len || (!page_table && b->max_kv_len)) return WM_E_ARG;
+    if (cu_tokens[0] != 0) return WM_E_SHAPE;
+    for (uint32_t s = 0; s < b->n_seqs; s++) {
+        const int64_t n = (int64_t)cu_tokens[s + 1] - cu_tokens[s];
+        if (n < 0 || n > b->max_new || (uint32_t)cu_tokens[s + 1] > b->n_tokens) return WM_E_SHAPE;
+        if (kv_len[s] < 0 || (uint32_t)kv_len[s] > b->max_kv_len) return WM_E_SHAPE;
+    }
+    // per page: 0 free, 1 read, 2 appended to
+    std::vector<uint8_t> use;
+    try {
+        if (appends) use.assign(kv->n_pages, 0);
+    } catch (const std::bad_alloc &) {
+        return WM_E_OOM;
+    }
+    for (uint32_t s = 0; s < b->n_seqs; s++) {
+        const int64_t n = (int64_t)cu_tokens[s + 1] - cu_tokens[s], len = kv_len[s];
+        if (!n) continue;  // reads and writes nothing
+        const int64_t start = len > n ? len - n : 0;
+        for (int64_t lp = 0; lp * kv->page_size < len; lp++) {
+            const int32_t page = page_table[(uint64_t)s * b->table_stride + lp];
+            if (page < 0 || (uint32_t)page >= kv->n_pages) return WM_E_BOUNDS;
+            if (!appends) continue;
+            const bool write = (lp + 1) * kv->page_size > start;
+            if (write ? use[page] != 0 : use[page] == 2) return WM_E_BOUNDS;
+            use[page] = write ? 2 : 1;
+        }
+    }
+    return WM_OK;
+}
+
+wm_status wm_paged_kv_append_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch,
+                                 const wm_rope *rope, int type, const void *d_q, uint64_t q_stride,
+                                 uint32_t n_heads, const void *d_k, uint64_t k_stride, const void *d_v,
+                                 uint64_t v_stride, void *d_q_out, uint64_t q_out_stride) {
+    static const char who[] = "paged_kv_append";
+    if (!ctx) return WM_E_ARG;
+    wm_status st;
+    if ((st = wm_paged_check(ctx, who, kv, batch))) return st;
+    const size_t elem = wm_dtype_size(type);
+    if (!elem) return wm_set_error(ctx, WM_E_UNSUPPORTED_TYPE, "%s: type %d is not F32, F16 or BF16", who, type);
+    if (n_heads % kv->n_kv_heads || n_heads > 1u << 20)
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %u query heads over %u kv heads", who, n_heads, kv->n_kv_heads);
+    append_args a;
+    memset(&a, 0, sizeof a);
+    if (rope) {
+        a.rope = *rope;
+        if (rope->n_rot % 8 || rope->n_rot > kv->head_dim)
+            return wm_set_error(ctx, WM_E_SHAPE, "%s: n_rot %u is not a multiple of 8 up to head_dim %u", who,
+                                rope->n_rot, kv->head_dim);
+        if (rope->layout != WM_ROPE_HALF && rope->layout != WM_ROPE_INTERLEAVED)
+            return wm_set_error(ctx, WM_E_ARG, "%s: rope layout %u", who, rope->layout);
+        if (rope->n_rot) {
+            if (!rope->cos || !rope->sin || ((uintptr_t)rope->cos | (uintptr_t)rope->sin) % 16)
+                return wm_set_error(ctx, WM_E_ARG, "%s: null or misaligned rope tables", who);
+            if (rope->n_pos < batch->max_kv_len)
+                return wm_set_error(ctx, WM_E_SHAPE, "%s: rope tables of %u positions for max_kv_len %u", who,
+                                    rope->n_pos, batch->max_kv_len);
+        }
+    }
+    if (batch->n_tokens == 0 || batch->n_seqs == 0) return WM_OK;
+    if ((st = wm_paged_check_array(ctx, who, "k", d_k, k_stride, kv->n_kv_heads, kv->head_dim, elem))) return st;
+    if ((st = wm_paged_check_array(ctx, who, "v", d_v, v_stride, kv->n_kv_heads, kv->head_dim, elem))) return st;
+    if (n_heads) {
+        if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
+        if ((st = wm_paged_check_array(ctx, who, "q_out", d_q_out, q_out_stride, n_heads, kv->head_dim, elem))) return st;
+    }
+    a.kv = *kv, a.b = *batch;
+    a.q = d_q, a.k = d_k, a.v = d_v, a.q_out = d_q_out;
+    a.qs = q_stride, a.ks = k_stride, a.vs = v_stride, a.qos = q_out_stride;
+    a.group = n_heads / kv->n_kv_heads;
+    a.touch = touched_pages(kv, batch);
+    uint32_t grid;
+    if ((st = block_grid(ctx, who, kv, batch, &grid))) return st;
+    if (!grid) return WM_OK;
+    wm_device_guard dev(ctx->device);
+    WM_HIP(ctx, dev.err);
+    by_shape<launch_append>(type, kv->page_size, kv->head_dim, a, grid, ctx->stream);
+    WM_HIP(ctx, hipGetLastError());
+    return WM_OK;
+}
+
+wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
+                               void *d_k_out, uint64_t k_stride, void *d_v_out, uint64_t v_stride) {
+    static const char who[] = "paged_kv_read";
+    if (!ctx) return WM_E_ARG;
+    wm_status st;
+    if ((st = wm_paged_check(ctx, who, kv, batch))) return st;
+    const size_t elem = wm_dtype_size(type);
+    if (!elem) return wm_set_error(ctx, WM_E_UNSUPPORTED_TYPE, "%s: type %d is not F32, F16 or BF16", who, type);
+    if (batch->n_tokens == 0 || batch->n_seqs == 0 || (!d_k_out && !d_v_out)) return WM_OK;
+    if (d_k_out && (st = wm_paged_check_array(ctx, who, "k_out", d_k_out, k_stride, kv->n_kv_heads, kv->head_dim, elem)))
+        return st;
+    if (d_v_out && (st = wm_paged_check_array(ctx, who, "v_out", d_v_out, v_stride, kv->n_kv_heads, kv->head_dim, elem)))
+        return st;
+    read_args a{*kv, *batch, d_k_out, d_v_out, k_stride, v_stride, touched_pages(kv, batch)};
+    uint32_t grid;
+    if ((st = block_grid(ctx, who, kv, batch, &grid))) return st;
+    if (!grid) return WM_OK;
+    wm_device_guard dev(ctx->device);
+    WM_HIP(ctx, dev.err);
+    by_shape<launch_read>(type, kv->page_size, kv->head_dim, a, grid, ctx->stream);
+    WM_HIP(ctx, hipGetLastError());
+    return WM_OK;
+}
+
+}  // extern "C"

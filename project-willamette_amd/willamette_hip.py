@@ -100,6 +100,29 @@ class SamplingParams(C.Structure):
                    repetition_penalty is not None)
 
 
+# wm_dtype: element types of the paged cache's activations and of logits
+DTYPES = {"f32": 0, "f16": 1, "bf16": 30}
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+
+
+class PagedKV(C.Structure):
+    """wm_paged_kv: one layer's page pool (device pointers)."""
+    _fields_ = [("k_codes", _vp), ("v_codes", _vp), ("k_scales", _vp), ("v_scales", _vp), ("n_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class PagedBatch(C.Structure):
+    """wm_paged_batch: a step's sequences (device pointers, host bounds)."""
+    _fields_ = [("cu_tokens", _vp), ("kv_len", _vp), ("page_table", _vp), ("n_seqs", C.c_uint32),
+                ("table_stride", C.c_uint32), ("n_tokens", C.c_uint32), ("max_new", C.c_uint32),
+                ("max_kv_len", C.c_uint32)]
+
+
+class Rope(C.Structure):
+    """wm_rope: cosines and sines [n_pos][n_rot / 2] (device pointers)."""
+    _fields_ = [("cos", _vp), ("sin", _vp), ("n_pos", C.c_uint32), ("n_rot", C.c_uint32), ("layout", C.c_uint32)]
+
+
 def _sig(name, restype, *argtypes):
     f = getattr(lib, name)
     f.restype = restype
@@ -186,6 +209,19 @@ EXPORTS = {
     "wm_debug_seq_sum": (C.c_int, _vp, _f32p, C.c_size_t, _f32p),
     "wm_debug_q6k_bounded_logits": (C.c_int, _vp, _vp, _f32p, C.c_size_t, _f32p, _f32p),
     "wm_debug_q6k_bounded_logits_dev": (C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int),
+    "wm_paged_batch_check": (C.c_int, C.POINTER(PagedKV), C.POINTER(PagedBatch), _i32p, _i32p, _i32p, C.c_int),
+    "wm_paged_kv_append_dev": (C.c_int, _vp, C.POINTER(PagedKV), C.POINTER(PagedBatch), C.POINTER(Rope), C.c_int,
+                               _vp, C.c_uint64, C.c_uint32, _vp, C.c_uint64, _vp, C.c_uint64, _vp, C.c_uint64),
+    "wm_paged_kv_read_dev": (C.c_int, _vp, C.POINTER(PagedKV), C.POINTER(PagedBatch), C.c_int, _vp, C.c_uint64,
+                             _vp, C.c_uint64),
+    "wm_paged_attention_workspace": (C.c_size_t, C.POINTER(PagedKV), C.POINTER(PagedBatch), C.c_uint32),
+    "wm_paged_attention_dev": (C.c_int, _vp, C.POINTER(PagedKV), C.POINTER(PagedBatch), C.c_int, _vp, C.c_uint64,
+                               C.c_uint32, C.c_float, _vp, C.c_uint64, _vp, _vp, C.c_size_t),
+    "wm_token_logprobs_workspace": (C.c_size_t, C.c_uint32, C.c_uint32, C.c_uint32),
+    "wm_token_logprobs_dev": (C.c_int, _vp, C.c_int, _vp, C.c_uint64, C.c_uint32, C.c_uint32, _vp, C.c_uint32, _vp,
+                              _vp, _vp, _vp, _vp, _vp, C.c_size_t),
+    "wm_token_logprobs": (C.c_int, _vp, _f32p, C.c_uint32, C.c_uint32, _i32p, C.c_uint32, _f32p, _f32p, _i32p, _i32p,
+                          _f32p),
     "wm_gguf_parse": (C.c_int, _u8p, C.c_size_t, C.POINTER(_vp), C.c_char_p, C.c_size_t),
     "wm_gguf_open": (C.c_int, C.c_char_p, C.POINTER(_vp), C.c_char_p, C.c_size_t),
     "wm_gguf_close": (None, _vp),
@@ -542,6 +578,52 @@ def q6k_bounded_logits(ctx: Context, t: Tensor, hidden: np.ndarray):
     ctx.check(lib.wm_debug_q6k_bounded_logits(ctx.h, t.h, _ptr(hidden, C.c_float), hidden.size,
                                               _ptr(approx, C.c_float), _ptr(bound, C.c_float)))
     return approx, bound
+
+
+# ---------------------------------------------------------------------------
+# paged 8-bit KV cache and token scores
+# ---------------------------------------------------------------------------
+
+def paged_batch_check(kv: PagedKV, batch: PagedBatch, cu_tokens, kv_len, page_table, appends: bool = True) -> None:
+    """wm_paged_batch_check on host copies of the step's arrays (no GPU needed)."""
+    cu, n, t = (np.ascontiguousarray(a, np.int32) for a in (cu_tokens, kv_len, page_table))
+    if cu.size != batch.n_seqs + 1 or n.size != batch.n_seqs or t.size != batch.n_seqs * batch.table_stride:
+        raise ValueError("paged_batch_check: the arrays' sizes are not the batch's")
+    st = lib.wm_paged_batch_check(C.byref(kv), C.byref(batch), _ptr(cu, C.c_int32), _ptr(n, C.c_int32),
+                                  _ptr(t, C.c_int32), int(appends))
+    if st:
+        raise WillametteError(st, "paged_batch_check")
+
+
+def paged_attention_workspace(kv: PagedKV, batch: PagedBatch, n_heads: int) -> int:
+    return int(lib.wm_paged_attention_workspace(C.byref(kv), C.byref(batch), n_heads))
+
+
+def token_logprobs_workspace(n_rows: int, vocab: int, top_k: int) -> int:
+    return int(lib.wm_token_logprobs_workspace(n_rows, vocab, top_k))
+
+
+def token_logprobs(ctx: Context, logits: np.ndarray, tokens=None, top_k: int = 0) -> dict:
+    """Per row of logits (rows x vocab, f32): the token's logprob and rank
+    (with tokens), the entropy, and the top_k first tokens with theirs."""
+    x = np.ascontiguousarray(logits, dtype=np.float32)
+    rows, vocab = x.shape
+    tok = None if tokens is None else np.ascontiguousarray(tokens, np.int32)
+    if tok is not None and tok.shape != (rows,):
+        raise ValueError("token_logprobs: one token per row")
+    out = {"entropy": np.empty(rows, np.float32)}
+    if tok is not None:
+        out.update(logprob=np.empty(rows, np.float32), rank=np.empty(rows, np.int32))
+    if top_k:
+        out.update(top_ids=np.empty((rows, top_k), np.int32), top_logprobs=np.empty((rows, top_k), np.float32))
+
+    def p(name, ct):
+        return _ptr(out[name], ct) if name in out else None
+    ctx.check(lib.wm_token_logprobs(ctx.h, _ptr(x, C.c_float), rows, vocab,
+                                    None if tok is None else _ptr(tok, C.c_int32), top_k, p("logprob", C.c_float),
+                                    p("entropy", C.c_float), p("rank", C.c_int32), p("top_ids", C.c_int32),
+                                    p("top_logprobs", C.c_float)))
+    return out
 
 
 # ---------------------------------------------------------------------------

@@ -33,6 +33,12 @@ pub const WM_FUSED_DEBUG_ATTN_LOOSE_COUNT: u32 = 16;
 pub const WM_TYPE_I2S: c_int = 36;
 pub const WM_TYPE_Q6K: c_int = 14;
 
+pub const WM_DTYPE_F32: c_int = 0;
+pub const WM_DTYPE_F16: c_int = 1;
+pub const WM_DTYPE_BF16: c_int = 30;
+pub const WM_ROPE_HALF: u32 = 0;
+pub const WM_ROPE_INTERLEAVED: u32 = 1;
+
 #[repr(C)]
 pub struct wm_ctx {
     _p: [u8; 0],
@@ -90,6 +96,45 @@ pub struct wm_sampling_params {
     pub has_top_p: u32,
     pub repetition_penalty: f32,
     pub has_repetition_penalty: u32,
+}
+
+/// One layer's page pool of the paged 8-bit KV cache (device pointers).
+#[repr(C)]
+#[derive(Debug, Clone, Copy, PartialEq)]
+pub struct wm_paged_kv {
+    pub k_codes: *mut i8,
+    pub v_codes: *mut i8,
+    pub k_scales: *mut f32,
+    pub v_scales: *mut f32,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub n_kv_heads: u32,
+    pub head_dim: u32,
+}
+
+/// A step's sequences over the page pool (device pointers, host bounds).
+#[repr(C)]
+#[derive(Debug, Clone, Copy, PartialEq)]
+pub struct wm_paged_batch {
+    pub cu_tokens: *const i32,
+    pub kv_len: *const i32,
+    pub page_table: *const i32,
+    pub n_seqs: u32,
+    pub table_stride: u32,
+    pub n_tokens: u32,
+    pub max_new: u32,
+    pub max_kv_len: u32,
+}
+
+/// Cosines and sines of the rotary positions (device pointers).
+#[repr(C)]
+#[derive(Debug, Clone, Copy, PartialEq)]
+pub struct wm_rope {
+    pub cos: *const f32,
+    pub sin: *const f32,
+    pub n_pos: u32,
+    pub n_rot: u32,
+    pub layout: u32,
 }
 
 extern "C" {
@@ -155,6 +200,14 @@ extern "C" {
     pub fn wm_server_step(s: *mut wm_server, n_active: *mut u32) -> wm_status;
     pub fn wm_server_result(s: *mut wm_server, request_id: u64, out_ids: *mut u32, cap: u32, n_out: *mut u32, finished: *mut c_int) -> wm_status;
     pub fn wm_server_release(s: *mut wm_server, request_id: u64) -> wm_status;
+    pub fn wm_paged_batch_check(kv: *const wm_paged_kv, batch: *const wm_paged_batch, cu_tokens: *const i32, kv_len: *const i32, page_table: *const i32, appends: c_int) -> wm_status;
+    pub fn wm_paged_kv_append_dev(ctx: *mut wm_ctx, kv: *const wm_paged_kv, batch: *const wm_paged_batch, rope: *const wm_rope, type_: c_int, d_q: *const c_void, q_stride: u64, n_heads: u32, d_k: *const c_void, k_stride: u64, d_v: *const c_void, v_stride: u64, d_q_out: *mut c_void, q_out_stride: u64) -> wm_status;
+    pub fn wm_paged_kv_read_dev(ctx: *mut wm_ctx, kv: *const wm_paged_kv, batch: *const wm_paged_batch, type_: c_int, d_k_out: *mut c_void, k_stride: u64, d_v_out: *mut c_void, v_stride: u64) -> wm_status;
+    pub fn wm_paged_attention_workspace(kv: *const wm_paged_kv, batch: *const wm_paged_batch, n_heads: u32) -> usize;
+    pub fn wm_paged_attention_dev(ctx: *mut wm_ctx, kv: *const wm_paged_kv, batch: *const wm_paged_batch, type_: c_int, d_q: *const c_void, q_stride: u64, n_heads: u32, scale: f32, d_out: *mut c_void, out_stride: u64, d_lse: *mut f32, d_work: *mut c_void, work_bytes: usize) -> wm_status;
+    pub fn wm_token_logprobs_workspace(n_rows: u32, vocab: u32, top_k: u32) -> usize;
+    pub fn wm_token_logprobs_dev(ctx: *mut wm_ctx, type_: c_int, d_logits: *const c_void, row_stride: u64, n_rows: u32, vocab: u32, d_tokens: *const i32, top_k: u32, d_logprob: *mut f32, d_entropy: *mut f32, d_rank: *mut i32, d_top_ids: *mut i32, d_top_logprobs: *mut f32, d_work: *mut c_void, work_bytes: usize) -> wm_status;
+    pub fn wm_token_logprobs(ctx: *mut wm_ctx, logits: *const f32, n_rows: u32, vocab: u32, tokens: *const i32, top_k: u32, logprob: *mut f32, entropy: *mut f32, rank: *mut i32, top_ids: *mut i32, top_logprobs: *mut f32) -> wm_status;
     pub fn wm_gguf_parse(data: *const u8, len: usize, out: *mut *mut wm_gguf, err: *mut c_char, err_len: usize) -> wm_status;
     pub fn wm_gguf_open(path: *const c_char, out: *mut *mut wm_gguf, err: *mut c_char, err_len: usize) -> wm_status;
     pub fn wm_gguf_close(g: *mut wm_gguf);
