@@ -80,8 +80,24 @@ __device__ __forceinline__ float group_sum(float v) {
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// A value as one f16 term, or as two whose sum holds its upper 22 bits: the
+// first is cut off, not rounded, so that both come from the same f32 value
+// (a rounded one, fused with the product that made the value, could round a
+// tie the other way than its copy that is subtracted).
+template <int TERMS>
+__device__ __forceinline__ void to_terms(float v, _Float16 *hi, _Float16 *lo) {
+    if (TERMS == 1) {
+        *hi = (_Float16)v;
+    } else {
+        const float h = __uint_as_float(__float_as_uint(v) & 0xFFFFE000u);
+        *hi = (_Float16)h;
+        *lo = (_Float16)(v - h);
+    }
+}
+// f32 inputs take two terms, the half types one.
+template <int TERMS>
 __device__ __forceinline__ wm_f4 load_q4(const attn_args &a, uint64_t at) {
-    if (a.type == WM_DTYPE_F32) return wm_ld4((const float *)a.q + at);
+    if (TERMS > 1) return wm_ld4((const float *)a.q + at);
     if (a.type == WM_DTYPE_F16) return wm_ld4((const _Float16 *)a.q + at);
     return wm_ld4((const __bf16 *)a.q + at);
 }
@@ -171,7 +187,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
-                const wm_f4 v = valid ? load_q4(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i) : wm_f4{0, 0, 0, 0};
+                const wm_f4 v = valid ? load_q4<TERMS>(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i) : wm_f4{0, 0, 0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
             }
@@ -181,10 +197,10 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float v = ldexpf(x[j][i], 15 - e);
-                const _Float16 hi = (_Float16)v;
+                _Float16 hi, lo;
+                to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &hi, &lo);
                 q[r][j][0][i] = hi;
-                if (TERMS > 1) q[r][j][TERMS - 1][i] = (_Float16)(v - (float)hi);
+                if (TERMS > 1) q[r][j][TERMS - 1][i] = lo;
             }
     }
     const int all = t.q.start + t.r0 / (int)a.group + 1;  // positions that every row attends to
@@ -318,9 +334,10 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
             l[r] = __builtin_fmaf(sum, unshift, l[r]);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const _Float16 hi = (_Float16)x[i];
+                _Float16 hi, lo;
+                to_terms<TERMS>(x[i], &hi, &lo);
                 w[r][i / 8][0][i % 8] = hi;
-                if (TERMS > 1) w[r][i / 8][TERMS - 1][i % 8] = (_Float16)(x[i] - (float)hi);
+                if (TERMS > 1) w[r][i / 8][TERMS - 1][i % 8] = lo;
             }
         }
 #pragma unroll
