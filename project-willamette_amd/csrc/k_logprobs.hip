@@ -1,5 +1,12 @@
 // Log probabilities of given tokens, the entropy of their distribution, the
 // token's rank and the top alternatives, per row of logits.
+//
+// A row's logits are read once, which is the bound: a workgroup takes a part
+// of a row into registers (64 VGPRs a lane, all its loads in flight at once),
+// and maximum, sums, rank and top tokens come from there.  The top tokens of a
+// part: the k-th largest of the lanes' maxima is a value that at least k
+// logits reach, and hardly more than k do, so those are listed and ranked by
+// counting.  The parts of a row are joined by a second launch.
 #include <cstdio>
 #include <cstring>
 
@@ -7,8 +14,14 @@
 
 namespace {
 
-constexpr int NT = 1024;
+constexpr int NT = 256;
 constexpr uint32_t MAX_TOP = 64;
+constexpr int LIST = 512;  // logits that may reach the threshold before the slow way is taken
+
+struct lp_part {  // of one part of a row; with `keys` what the join reads
+    float m, l, s;
+    int32_t before;
+};
 
 struct lp_args {
     const void *x;
@@ -18,91 +31,253 @@ struct lp_args {
     float *logprob, *entropy;
     int32_t *rank, *top_ids;
     float *top_logprobs;
+    uint32_t parts, part_vecs;  // parts of a row, 16-byte vectors of each
+    lp_part *part;              // [row][part]
+    uint64_t *keys;             // [row][part][top_k], in order
 };
 
 // Order of (logit descending, id): the larger key comes first.  Zeros are
-// one value; NaN is below every number.
+// one value; NaN is below every number; no logit has key 0.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
-    return x != x ? 0u : b ^ ((int)b < 0 ? 0xFFFFFFFFu : 0x80000000u);
+    return x != x ? 1u : b ^ ((int)b < 0 ? 0xFFFFFFFFu : 0x80000000u);
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t id) { return (uint64_t)ordered(x) << 32 | ~id; }
 __device__ __forceinline__ float key_value(uint64_t key) {
     const uint32_t o = (uint32_t)(key >> 32);
-    return o == 0 ? __uint_as_float(0x7FC00000u) : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+    return o <= 1 ? __uint_as_float(0x7FC00000u) : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
-
-// Sum of e^(x - m) and of e^(x - m) (x - m) under the running maximum m.
-struct stats {
-    float m, l, s;
-};
-__device__ __forceinline__ void add(stats &a, float x) {
-    if (x > a.m) {
-        const float d = a.m - x, e = expf(d);
-        a.s = e * (a.s + a.l * fmaxf(d, -200.0f));
-        a.l *= e;
-        a.m = x;
-    }
-    const float d = a.m == -INFINITY ? x : x - a.m, e = expf(d);
-    a.l += e;
-    a.s += e * fmaxf(d, -200.0f);
-}
-__device__ __forceinline__ stats join(stats a, stats b) {
-    const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
-    const float da = a.m - base, db = b.m - base, ea = expf(da), eb = expf(db);
-    return {m, a.l * ea + b.l * eb,
-            ea * (a.s + a.l * fmaxf(da, -200.0f)) + eb * (b.s + b.l * fmaxf(db, -200.0f))};
-}
-__device__ __forceinline__ float read(const float *x, uint64_t i) { return x[i]; }
-__device__ __forceinline__ float read(const _Float16 *x, uint64_t i) { return (float)x[i]; }
-__device__ __forceinline__ float read(const __bf16 *x, uint64_t i) { return (float)x[i]; }
-
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-    return (uint64_t)__shfl_xor((int)(v >> 32), o, 64) << 32 | (uint32_t)__shfl_xor((int)v, o, 64);
+    return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o, 64) << 32 | (uint32_t)__shfl_xor((int)v, o, 64);
 }
 
-template <typename T>
-__global__ __launch_bounds__(NT) void k_token_logprobs(lp_args a) {
-    __shared__ stats sh[NT / 64];
+constexpr float LOG2E = 1.4426950408889634f;
+
+// e^(x - m) sums of two parts under their common maximum.
+__device__ __forceinline__ lp_part join_parts(lp_part a, lp_part b) {
+    const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
+    const float da = a.m - base, db = b.m - base;
+    const float ea = __builtin_amdgcn_exp2f(da * LOG2E), eb = __builtin_amdgcn_exp2f(db * LOG2E);
+    return {m, a.l * ea + b.l * eb,
+            ea * (a.s + a.l * fmaxf(da, -200.0f)) + eb * (b.s + b.l * fmaxf(db, -200.0f)), a.before + b.before};
+}
+
+// What a finished row says.
+struct row_end {
+    float m, log_l;
+    bool none;  // every logit -inf
+};
+__device__ __forceinline__ row_end end_row(const lp_part &p) {
+    const bool none = p.m == -INFINITY && p.l == 0.0f;
+    return {p.m, none ? 0.0f : logf(p.l), none};
+}
+__device__ __forceinline__ float end_logprob(const row_end &e, float x) {
+    return e.none ? x : (x - e.m) - e.log_l;
+}
+__device__ __forceinline__ void write_row(const lp_args &a, uint32_t row, const lp_part &p, const row_end &e, bool known,
+                                          float xt) {
+    if (a.logprob) a.logprob[row] = known ? end_logprob(e, xt) : __uint_as_float(0x7FC00000u);
+    if (a.entropy) a.entropy[row] = e.none ? 0.0f : e.log_l - p.s / p.l;
+    if (a.rank) a.rank[row] = known ? p.before : -1;
+}
+__device__ __forceinline__ void write_top(const lp_args &a, uint32_t row, uint32_t i, const row_end &e, uint64_t key) {
+    const uint64_t at = (uint64_t)row * a.top_k + i;
+    if (a.top_ids) a.top_ids[at] = (int32_t)~(uint32_t)key;
+    if (a.top_logprobs) a.top_logprobs[at] = end_logprob(e, key_value(key));
+}
+
+// The elements of one 16-byte vector.
+template <typename T> struct vec;
+template <> struct vec<float> {
+    static constexpr int N = 4;
+    static constexpr uint32_t LOW = 0xFF800000u;  // -inf in every element of a word
+    static __device__ __forceinline__ float at(wm_u4 v, int i) { return __uint_as_float(v[i]); }
+    static __device__ __forceinline__ float one(const float *p) { return *p; }
+    static __device__ __forceinline__ uint32_t bits(const float *p) { return __float_as_uint(*p); }
+};
+template <> struct vec<_Float16> {
+    static constexpr int N = 8;
+    static constexpr uint32_t LOW = 0xFC00FC00u;
+    static __device__ __forceinline__ float at(wm_u4 v, int i) {
+        return (float)__builtin_bit_cast(wm_h2, (unsigned)v[i / 2])[i % 2];
+    }
+    static __device__ __forceinline__ float one(const _Float16 *p) { return (float)*p; }
+    static __device__ __forceinline__ uint32_t bits(const _Float16 *p) { return *(const uint16_t *)p; }
+};
+template <> struct vec<__bf16> {
+    static constexpr int N = 8;
+    static constexpr uint32_t LOW = 0xFF80FF80u;
+    static __device__ __forceinline__ float at(wm_u4 v, int i) {
+        return __uint_as_float(i % 2 ? v[i / 2] & 0xFFFF0000u : v[i / 2] << 16);
+    }
+    static __device__ __forceinline__ float one(const __bf16 *p) { return __uint_as_float((uint32_t)bits(p) << 16); }
+    static __device__ __forceinline__ uint32_t bits(const __bf16 *p) { return *(const uint16_t *)p; }
+};
+
+// In front of each use of a vector in a pass over the registers: without it
+// values unpacked in one pass stay alive for the next, or all of a pass are
+// unpacked at its beginning, and the registers overflow.
+__device__ __forceinline__ void repack(wm_u4 &v) { asm volatile("" : "+v"(v)); }
+
+template <typename T, int NV>
+__global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
+    using V = vec<T>;
+    constexpr int N = V::N;
+    __shared__ float sh_max[NT];
+    __shared__ uint64_t sh_list[LIST];
+    __shared__ lp_part sh_part[NT / 64];
     __shared__ uint64_t sh_key[NT / 64];
-    __shared__ int sh_n[NT / 64];
-    const T *x = (const T *)a.x + blockIdx.x * a.stride;
+    __shared__ int sh_n;
+    __shared__ float sh_thr;
+    const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const T *x = (const T *)a.x + row * a.stride;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int32_t token = a.tokens ? a.tokens[blockIdx.x] : -1;
+    const int32_t token = a.tokens ? a.tokens[row] : -1;
     const bool known = token >= 0 && (uint32_t)token < a.vocab;
-    const uint64_t mine = known ? key_of(read(x, token), token) : 0;
-    stats st = {-INFINITY, 0.0f, 0.0f};
+    // Vectors lie on 16-byte boundaries of the address; `skew` elements of
+    // the row's first are in front of it.
+    const int skew = (int)((uintptr_t)x % 16 / sizeof(T));
+    const int vocab = (int)a.vocab, v0 = (int)(part * a.part_vecs);
+    const int v_end = min(v0 + (int)a.part_vecs, (vocab + skew + N - 1) / N);
+    wm_u4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int at = v0 + tid + i * NT, id = at * N - skew;
+        v[i] = wm_u4{V::LOW, V::LOW, V::LOW, V::LOW};
+        if (at >= v_end) continue;
+        if (id >= 0 && id + N <= vocab) {
+            v[i] = __builtin_nontemporal_load((const wm_u4 *)(x + id));
+        } else {  // the row's ends: its own elements, one by one
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (id + e >= 0 && id + e < vocab) {
+                    if (N == 4) {
+                        v[i][e] = V::bits(x + id + e);
+                    } else {
+                        const uint32_t s = 16 * (e % 2);
+                        v[i][e / 2] = (v[i][e / 2] & ~(0xFFFFu << s)) | V::bits(x + id + e) << s;
+                    }
+                }
+        }
+    }
+    const float xt = known ? V::one(x + token) : 0.0f;
+    // the part's maximum
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        repack(v[i]);
+#pragma unroll
+        for (int e = 0; e < N; e++) top = fmaxf(top, V::at(v[i], e));
+    }
+    sh_max[tid] = top;
+    if (tid == 0) sh_n = 0;
+    __syncthreads();
+    float m = top;
+    if (a.top_k) {
+        // how many lanes' maxima come before this lane's; the k-th is the threshold
+        int rank = 0;
+        for (int i = 0; i < NT; i += 4) {
+            const wm_f4 o = *(const wm_f4 *)&sh_max[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                rank += o[j] > top || (o[j] == top && i + j < tid);
+                m = fmaxf(m, o[j]);
+            }
+        }
+        if (rank == (int)a.top_k - 1) sh_thr = top;
+    } else {
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if (lane == 0) sh_part[wave].m = m;
+    }
+    __syncthreads();
+    if (!a.top_k)
+#pragma unroll
+        for (int w = 0; w < NT / 64; w++) m = fmaxf(m, sh_part[w].m);
+    const float thr = a.top_k ? sh_thr : 0.0f, base = m == -INFINITY ? 0.0f : m;
+
+    // Sums, and the logits before the token: x > xt, or x >= xt below its id,
+    // which is x > the number before xt.  (A token at -inf or NaN: by keys.)
+    const bool plain = known && xt > -INFINITY;
+    const float below = xt == 0.0f ? -1.401298464e-45f : __uint_as_float(__float_as_uint(xt) + (xt > 0.0f ? -1 : 1));
+    float l = 0.0f, s = 0.0f;
     int before = 0;
-    for (uint64_t i = tid; i < a.vocab; i += NT) {
-        const float v = read(x, i);
-        add(st, v);
-        before += key_of(v, (uint32_t)i) > mine;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        repack(v[i]);
+        const int id = (v0 + tid + i * NT) * N - skew;
+        const float limit = id + N <= token ? below : xt;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float y = V::at(v[i], e), d = y - base, w = __builtin_amdgcn_exp2f(d * LOG2E);
+            l += w;
+            s = __builtin_fmaf(w, fmaxf(d, -200.0f), s);
+            before += y > limit;
+        }
+        if (id <= token && id + N > token)
+#pragma unroll
+            for (int e = 0; e < N; e++) before += id + e < token && V::at(v[i], e) == xt;
+    }
+    // the part's ids, for what reads them again
+    const int id0 = max(v0 * N - skew, 0), id1 = min(v_end * N - skew, vocab);
+    if (known && !plain) {
+        const uint64_t mine = key_of(xt, token);
+        before = 0;
+        for (int id = id0 + tid; id < id1; id += NT) before += key_of(V::one(x + id), (uint32_t)id) > mine;
     }
     for (int o = 32; o; o >>= 1) {
-        st = join(st, stats{__shfl_xor(st.m, o, 64), __shfl_xor(st.l, o, 64), __shfl_xor(st.s, o, 64)});
+        l += __shfl_xor(l, o, 64);
+        s += __shfl_xor(s, o, 64);
         before += __shfl_xor(before, o, 64);
     }
-    if (lane == 0) sh[wave] = st, sh_n[wave] = before;
-    __syncthreads();
-    st = sh[0], before = sh_n[0];
-    for (int w = 1; w < NT / 64; w++) st = join(st, sh[w]), before += sh_n[w];
-    const float log_l = logf(st.l);
-    auto logprob = [&](float v) {
-        // every logit -inf: its sum is 0 (log -inf), which only takes NaN or
-        // +inf to leave NaN
-        return st.m == -INFINITY && st.l == 0.0f ? v : (v - st.m) - log_l;
-    };
-    if (tid == 0) {
-        const bool none = st.m == -INFINITY && st.l == 0.0f;
-        if (a.logprob) a.logprob[blockIdx.x] = known ? logprob(read(x, token)) : __uint_as_float(0x7FC00000u);
-        if (a.entropy) a.entropy[blockIdx.x] = none ? 0.0f : log_l - st.s / st.l;
-        if (a.rank) a.rank[blockIdx.x] = known ? before : -1;
+    // the logits that reach the threshold
+    if (a.top_k && thr > -INFINITY && top >= thr) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            repack(v[i]);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float y = V::at(v[i], e);
+                if (y >= thr) {
+                    const int n = atomicAdd(&sh_n, 1);
+                    if (n < LIST) sh_list[n] = key_of(y, (uint32_t)((v0 + tid + i * NT) * N - skew + e));
+                }
+            }
+        }
     }
+    __syncthreads();  // sh_part's maxima are read
+    if (lane == 0) sh_part[wave] = {m, l, s, before};
+    __syncthreads();
+    lp_part p = sh_part[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) p.l += sh_part[w].l, p.s += sh_part[w].s, p.before += sh_part[w].before;
+    const bool whole = a.parts == 1;
+    const row_end end = end_row(p);
+    if (tid == 0) {
+        if (whole) write_row(a, row, p, end, known, xt);
+        else a.part[blockIdx.x] = p;
+    }
+    if (!a.top_k) return;
+    auto put = [&](uint32_t i, uint64_t key) {
+        if (whole) write_top(a, row, i, end, key);
+        else a.keys[(uint64_t)blockIdx.x * a.top_k + i] = key;
+    };
+    const int n = sh_n;
+    if (thr > -INFINITY && n <= LIST) {
+        for (int c = tid; c < n; c += NT) {
+            const uint64_t mine = sh_list[c];
+            uint32_t rank = 0;
+            for (int i = 0; i < n; i++) rank += sh_list[i] > mine;
+            if (rank < a.top_k) put(rank, mine);
+        }
+        return;
+    }
+    // Fewer than k lanes hold a number above -inf, or very many logits are
+    // equal: one more pass over the part per token.
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top_k; k++) {
         uint64_t best = 0;
-        for (uint64_t i = tid; i < a.vocab; i += NT) {
-            const uint64_t key = key_of(read(x, i), (uint32_t)i);
+        for (int id = id0 + tid; id < id1; id += NT) {
+            const uint64_t key = key_of(V::one(x + id), (uint32_t)id);
             if (key < last && key > best) best = key;
         }
         for (int o = 32; o; o >>= 1) best = max(best, shfl_xor64(best, o));
@@ -110,14 +285,93 @@ __global__ __launch_bounds__(NT) void k_token_logprobs(lp_args a) {
         if (lane == 0) sh_key[wave] = best;
         __syncthreads();
         best = sh_key[0];
+#pragma unroll
         for (int w = 1; w < NT / 64; w++) best = max(best, sh_key[w]);
-        last = best;
-        if (tid == 0) {
-            const uint64_t at = (uint64_t)blockIdx.x * a.top_k + k;
-            if (a.top_ids) a.top_ids[at] = (int32_t)~(uint32_t)best;
-            if (a.top_logprobs) a.top_logprobs[at] = logprob(key_value(best));
+        if (tid == 0) put(k, best);
+        if (best == 0) {  // the part has no more
+            for (uint32_t i = k + tid; i < a.top_k; i += NT) put(i, 0);
+            return;
         }
+        last = best;
     }
+}
+
+// Lane i of a wave holds the i-th of 64 keys in order; the first 64 of these
+// and of another such list: the larger of a[i] and b[63 - i] are they, in an
+// order that six exchanges sort.
+__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b_reversed, int lane) {
+    uint64_t v = max(a, b_reversed);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint64_t o = shfl_xor64(v, d);
+        v = (lane & d) ? min(v, o) : max(v, o);
+    }
+    return v;
+}
+
+// One workgroup per row: its parts' sums, and their lists merged.
+template <typename T>
+__global__ __launch_bounds__(NT) void k_logprobs_join(lp_args a) {
+    __shared__ lp_part sh_part[NT / 64];
+    __shared__ uint64_t sh_list[NT / 64][64];
+    const uint32_t row = blockIdx.x;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int32_t token = a.tokens ? a.tokens[row] : -1;
+    const bool known = token >= 0 && (uint32_t)token < a.vocab;
+    const float xt = known ? vec<T>::one((const T *)a.x + row * a.stride + token) : 0.0f;
+    const lp_part *part = a.part + (uint64_t)row * a.parts;
+    lp_part p = {-INFINITY, 0.0f, 0.0f, 0};
+    for (uint32_t i = tid; i < a.parts; i += NT) p = join_parts(p, part[i]);
+    for (int o = 32; o; o >>= 1)
+        p = join_parts(p, {__shfl_xor(p.m, o, 64), __shfl_xor(p.l, o, 64), __shfl_xor(p.s, o, 64), __shfl_xor(p.before, o, 64)});
+    if (lane == 0) sh_part[wave] = p;
+    uint64_t list = 0;
+    if (a.top_k) {
+        const uint64_t *keys = a.keys + (uint64_t)row * a.parts * a.top_k;
+        for (uint32_t i = wave; i < a.parts; i += NT / 64) {
+            const uint32_t j = 63 - lane;
+            list = merge64(list, j < a.top_k ? keys[(uint64_t)i * a.top_k + j] : 0, lane);
+        }
+        sh_list[wave][lane] = list;
+    }
+    __syncthreads();
+    p = sh_part[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) p = join_parts(p, sh_part[w]);
+    const row_end end = end_row(p);
+    if (tid == 0) write_row(a, row, p, end, known, xt);
+    if (wave == 0 && a.top_k) {
+#pragma unroll
+        for (int w = 1; w < NT / 64; w++) list = merge64(list, sh_list[w][63 - lane], lane);
+        if (lane < (int)a.top_k) write_top(a, row, lane, end, list);
+    }
+}
+
+// How a row is divided: as few parts as its lanes' registers allow, and of
+// few rows parts a quarter as long.  One row of 128256 f32 values: 8 long
+// parts against 32 short ones.
+struct lp_plan {
+    int nv;  // vectors per lane, at most
+    uint32_t parts, part_vecs;
+};
+lp_plan make_plan(uint32_t n_rows, uint32_t vocab, size_t elem) {
+    const uint64_t per = 16 / elem, vecs = ((uint64_t)vocab + 2 * per - 2) / per;  // with any skew
+    lp_plan p;
+    p.nv = n_rows * ((vecs + 16 * NT - 1) / (16 * NT)) <= 128 ? 4 : 16;
+    p.parts = (uint32_t)((vecs + (uint64_t)p.nv * NT - 1) / ((uint64_t)p.nv * NT));
+    p.part_vecs = (uint32_t)((vecs + p.parts - 1) / p.parts);
+    return p;
+}
+size_t plan_bytes(uint32_t n_rows, const lp_plan &p, uint32_t top_k) {
+    return p.parts > 1 ? (size_t)n_rows * p.parts * (sizeof(lp_part) + 8 * (size_t)top_k) : 0;
+}
+
+template <typename T>
+void launch(const lp_args &a, const lp_plan &p, hipStream_t s) {
+    const uint32_t grid = a.n_rows * a.parts;
+    if (p.nv == 4) k_logprobs_part<T, 4><<<grid, NT, 0, s>>>(a);
+    else k_logprobs_part<T, 16><<<grid, NT, 0, s>>>(a);
+    if (a.parts > 1) k_logprobs_join<T><<<a.n_rows, NT, 0, s>>>(a);
 }
 
 }  // namespace
@@ -125,8 +379,11 @@ __global__ __launch_bounds__(NT) void k_token_logprobs(lp_args a) {
 extern "C" {
 
 size_t wm_token_logprobs_workspace(uint32_t n_rows, uint32_t vocab, uint32_t top_k) {
-    (void)n_rows, (void)vocab, (void)top_k;
-    return 0;
+    if (vocab == 0 || top_k > MAX_TOP) return 0;
+    // of any type: f32 has the most parts
+    const size_t a = plan_bytes(n_rows, make_plan(n_rows, vocab, 4), top_k);
+    const size_t b = plan_bytes(n_rows, make_plan(n_rows, vocab, 2), top_k);
+    return a > b ? a : b;
 }
 
 wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uint64_t row_stride, uint32_t n_rows,
@@ -137,8 +394,9 @@ wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uin
     if (!ctx) return WM_E_ARG;
     const size_t elem = wm_dtype_size(type);
     if (!elem) return wm_set_error(ctx, WM_E_UNSUPPORTED_TYPE, "%s: type %d is not F32, F16 or BF16", who, type);
-    if (vocab == 0 || vocab > 0x7FFFFFFFu) return wm_set_error(ctx, WM_E_SHAPE, "%s: vocabulary of %u", who, vocab);
-    if (n_rows > 0x7FFFFFFFu / NT) return wm_set_error(ctx, WM_E_SHAPE, "%s: %u rows", who, n_rows);
+    if (vocab == 0 || vocab > 1u << 30) return wm_set_error(ctx, WM_E_SHAPE, "%s: vocabulary of %u", who, vocab);
+    if ((uint64_t)n_rows * make_plan(n_rows, vocab, elem).parts > 0x7FFFFFFFu / NT)  // the launch counts threads in 32 bits
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %u rows of %u", who, n_rows, vocab);
     if (top_k > MAX_TOP || top_k > vocab)
         return wm_set_error(ctx, WM_E_SHAPE, "%s: top_k %u of %u tokens, %u at most", who, top_k, vocab, MAX_TOP);
     if (n_rows > 1 && (row_stride < vocab || row_stride > 1ull << 40))
@@ -158,13 +416,21 @@ wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uin
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
                             d_work ? work_bytes : (size_t)0, need);
-    lp_args a{d_logits, row_stride, n_rows, vocab, top_k, d_tokens, d_logprob, d_entropy, d_rank, d_top_ids, d_top_logprobs};
-    if (!d_top_ids && !d_top_logprobs) a.top_k = 0;
+    const lp_plan p = make_plan(n_rows, vocab, elem);
+    lp_args a;
+    memset(&a, 0, sizeof a);
+    a.x = d_logits, a.stride = row_stride, a.n_rows = n_rows, a.vocab = vocab;
+    a.top_k = d_top_ids || d_top_logprobs ? top_k : 0;
+    a.tokens = d_tokens, a.logprob = d_logprob, a.entropy = d_entropy, a.rank = d_rank;
+    a.top_ids = d_top_ids, a.top_logprobs = d_top_logprobs;
+    a.parts = p.parts, a.part_vecs = p.part_vecs;
+    a.part = (lp_part *)d_work;
+    a.keys = d_work ? (uint64_t *)(a.part + (size_t)n_rows * p.parts) : nullptr;
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
-    if (type == WM_DTYPE_F32) k_token_logprobs<float><<<n_rows, NT, 0, ctx->stream>>>(a);
-    else if (type == WM_DTYPE_F16) k_token_logprobs<_Float16><<<n_rows, NT, 0, ctx->stream>>>(a);
-    else k_token_logprobs<__bf16><<<n_rows, NT, 0, ctx->stream>>>(a);
+    if (type == WM_DTYPE_F32) launch<float>(a, p, ctx->stream);
+    else if (type == WM_DTYPE_F16) launch<_Float16>(a, p, ctx->stream);
+    else launch<__bf16>(a, p, ctx->stream);
     WM_HIP(ctx, hipGetLastError());
     return WM_OK;
 }
