@@ -4,9 +4,8 @@
 // A row's logits are read once, which is the bound: a workgroup takes a part
 // of a row into registers (64 VGPRs a lane, all its loads in flight at once),
 // and maximum, sums, rank and top tokens come from there.  The top tokens of a
-// part: the k-th largest of the lanes' maxima is a value that at least k
-// logits reach, and hardly more than k do, so those are listed and ranked by
-// counting.  The parts of a row are joined by a second launch.
+// part: about the k-th largest of the lanes' maxima is a value that at least k
+// logits reach, and few more do, so those are listed and ranked by counting.  The parts of a row are joined by a second launch.
 #include <cstdio>
 #include <cstring>
 
@@ -123,12 +122,11 @@ template <typename T, int NV>
 __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
     using V = vec<T>;
     constexpr int N = V::N;
-    __shared__ float sh_max[NT];
     __shared__ uint64_t sh_list[LIST];
     __shared__ lp_part sh_part[NT / 64];
     __shared__ uint64_t sh_key[NT / 64];
     __shared__ int sh_n;
-    __shared__ float sh_thr;
+    __shared__ float sh_thr[2][NT / 64];
     const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const T *x = (const T *)a.x + row * a.stride;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -139,28 +137,36 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
     const int skew = (int)((uintptr_t)x % 16 / sizeof(T));
     const int vocab = (int)a.vocab, v0 = (int)(part * a.part_vecs);
     const int v_end = min(v0 + (int)a.part_vecs, (vocab + skew + N - 1) / N);
+    // All loads first, of whole vectors only (lanes without one load another's
+    // and drop it), so that nothing waits between them; then the row's ends,
+    // element by element.
+    const int whole0 = skew ? 1 : 0, whole1 = (vocab + skew) / N;
     wm_u4 v[NV];
+    if (whole1 > whole0) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int at = v0 + tid + i * NT, id = at * N - skew;
-        v[i] = wm_u4{V::LOW, V::LOW, V::LOW, V::LOW};
-        if (at >= v_end) continue;
-        if (id >= 0 && id + N <= vocab) {
-            v[i] = __builtin_nontemporal_load((const wm_u4 *)(x + id));
-        } else {  // the row's ends: its own elements, one by one
-#pragma unroll
-            for (int e = 0; e < N; e++)
-                if (id + e >= 0 && id + e < vocab) {
-                    if (N == 4) {
-                        v[i][e] = V::bits(x + id + e);
-                    } else {
-                        const uint32_t s = 16 * (e % 2);
-                        v[i][e / 2] = (v[i][e / 2] & ~(0xFFFFu << s)) | V::bits(x + id + e) << s;
-                    }
-                }
+        for (int i = 0; i < NV; i++) {
+            const int at = min(max(v0 + tid + i * NT, whole0), whole1 - 1);
+            v[i] = __builtin_nontemporal_load((const wm_u4 *)(x + (int64_t)at * N - skew));
         }
     }
     const float xt = known ? V::one(x + token) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int at = v0 + tid + i * NT;
+        if (at < whole0 || at >= whole1 || at >= v_end) {
+            v[i] = wm_u4{V::LOW, V::LOW, V::LOW, V::LOW};
+            if (at < v_end) {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int id = at * N - skew + e;
+                    if (id < 0 || id >= vocab) continue;
+                    const uint32_t b = V::bits(x + id), s = 16 * (e % 2);
+                    if (N == 4) v[i][e] = b;
+                    else v[i][e / 2] = (v[i][e / 2] & ~(0xFFFFu << s)) | b << s;
+                }
+            }
+        }
+    }
     // the part's maximum
     float top = -INFINITY;
 #pragma unroll
@@ -169,31 +175,34 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
 #pragma unroll
         for (int e = 0; e < N; e++) top = fmaxf(top, V::at(v[i], e));
     }
-    sh_max[tid] = top;
+    float m = top;
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (a.top_k) {
+        // The lanes' maxima in order, and two values that k of them reach: the
+        // smallest of the waves' k/4-th, and the largest of their k-th (where
+        // a wave holds few logits).
+        float y = top;
+#pragma unroll
+        for (int size = 2; size <= 64; size *= 2)
+#pragma unroll
+            for (int d = size / 2; d; d >>= 1) {
+                const float o = __shfl_xor(y, d, 64);
+                y = ((lane & d) != 0) == ((lane & size) != 0 && size < 64) ? fmaxf(y, o) : fminf(y, o);
+            }
+        const float quarter = __shfl(y, ((int)a.top_k + 3) / 4 - 1, 64), all = __shfl(y, (int)a.top_k - 1, 64);
+        if (lane == 0) sh_thr[0][wave] = quarter, sh_thr[1][wave] = all;
+    }
+    if (lane == 0) sh_part[wave].m = m;
     if (tid == 0) sh_n = 0;
     __syncthreads();
-    float m = top;
-    if (a.top_k) {
-        // how many lanes' maxima come before this lane's; the k-th is the threshold
-        int rank = 0;
-        for (int i = 0; i < NT; i += 4) {
-            const wm_f4 o = *(const wm_f4 *)&sh_max[i];
+    float thr = -INFINITY, least = INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                rank += o[j] > top || (o[j] == top && i + j < tid);
-                m = fmaxf(m, o[j]);
-            }
-        }
-        if (rank == (int)a.top_k - 1) sh_thr = top;
-    } else {
-        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        if (lane == 0) sh_part[wave].m = m;
+    for (int w = 0; w < NT / 64; w++) {
+        m = fmaxf(m, sh_part[w].m);
+        if (a.top_k) thr = fmaxf(thr, sh_thr[1][w]), least = fminf(least, sh_thr[0][w]);
     }
-    __syncthreads();
-    if (!a.top_k)
-#pragma unroll
-        for (int w = 0; w < NT / 64; w++) m = fmaxf(m, sh_part[w].m);
-    const float thr = a.top_k ? sh_thr : 0.0f, base = m == -INFINITY ? 0.0f : m;
+    if (a.top_k) thr = fmaxf(thr, least);
+    const float base = m == -INFINITY ? 0.0f : m;
 
     // Sums, and the logits before the token: x > xt, or x >= xt below its id,
     // which is x > the number before xt.  (A token at -inf or NaN: by keys.)
@@ -348,18 +357,19 @@ __global__ __launch_bounds__(NT) void k_logprobs_join(lp_args a) {
 }
 
 // How a row is divided: as few parts as its lanes' registers allow, and of
-// few rows parts a quarter as long.  One row of 128256 f32 values: 8 long
-// parts against 32 short ones.
+// few rows parts a quarter as long.
+constexpr uint32_t LONG_PART = 64 * NT, SHORT_PART = 16 * NT;  // elements, at most
 struct lp_plan {
-    int nv;  // vectors per lane, at most
+    bool small;
     uint32_t parts, part_vecs;
 };
 lp_plan make_plan(uint32_t n_rows, uint32_t vocab, size_t elem) {
-    const uint64_t per = 16 / elem, vecs = ((uint64_t)vocab + 2 * per - 2) / per;  // with any skew
+    const uint32_t per = (uint32_t)(16 / elem), vecs = (vocab + 2 * per - 2) / per;  // with any skew
     lp_plan p;
-    p.nv = n_rows * ((vecs + 16 * NT - 1) / (16 * NT)) <= 128 ? 4 : 16;
-    p.parts = (uint32_t)((vecs + (uint64_t)p.nv * NT - 1) / ((uint64_t)p.nv * NT));
-    p.part_vecs = (uint32_t)((vecs + p.parts - 1) / p.parts);
+    p.small = (uint64_t)n_rows * ((vocab + LONG_PART - 1) / LONG_PART) <= 128;
+    const uint32_t most = (p.small ? SHORT_PART : LONG_PART) / per;
+    p.parts = (vecs + most - 1) / most;
+    p.part_vecs = (vecs + p.parts - 1) / p.parts;
     return p;
 }
 size_t plan_bytes(uint32_t n_rows, const lp_plan &p, uint32_t top_k) {
@@ -369,8 +379,8 @@ size_t plan_bytes(uint32_t n_rows, const lp_plan &p, uint32_t top_k) {
 template <typename T>
 void launch(const lp_args &a, const lp_plan &p, hipStream_t s) {
     const uint32_t grid = a.n_rows * a.parts;
-    if (p.nv == 4) k_logprobs_part<T, 4><<<grid, NT, 0, s>>>(a);
-    else k_logprobs_part<T, 16><<<grid, NT, 0, s>>>(a);
+    if (p.small) k_logprobs_part<T, SHORT_PART / NT / vec<T>::N><<<grid, NT, 0, s>>>(a);
+    else k_logprobs_part<T, LONG_PART / NT / vec<T>::N><<<grid, NT, 0, s>>>(a);
     if (a.parts > 1) k_logprobs_join<T><<<a.n_rows, NT, 0, s>>>(a);
 }
 
