@@ -168,9 +168,11 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
         }
     }
     // the part's maximum
+    const int rounds = (v_end - v0 + NT - 1) / NT;  // of the NV, those that hold logits
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
+        if (i >= rounds) continue;
         repack(v[i]);
 #pragma unroll
         for (int e = 0; e < N; e++) top = fmaxf(top, V::at(v[i], e));
@@ -209,9 +211,10 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
     const bool plain = known && xt > -INFINITY;
     const float below = xt == 0.0f ? -1.401298464e-45f : __uint_as_float(__float_as_uint(xt) + (xt > 0.0f ? -1 : 1));
     float l = 0.0f, s = 0.0f;
-    int before = 0;
+    int before = 0;  // of the wave
 #pragma unroll
     for (int i = 0; i < NV; i++) {
+        if (i >= rounds) continue;
         repack(v[i]);
         const int id = (v0 + tid + i * NT) * N - skew;
         const float limit = id + N <= token ? below : xt;
@@ -220,11 +223,15 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
             const float y = V::at(v[i], e), d = y - base, w = __builtin_amdgcn_exp2f(d * LOG2E);
             l += w;
             s = __builtin_fmaf(w, fmaxf(d, -200.0f), s);
-            before += y > limit;
+            before += __popcll(__ballot(y > limit));
         }
-        if (id <= token && id + N > token)
+        if (__ballot(id <= token && id + N > token)) {
+            int same = 0;
 #pragma unroll
-            for (int e = 0; e < N; e++) before += id + e < token && V::at(v[i], e) == xt;
+            for (int e = 0; e < N; e++) same += id <= token && id + e < token && id + N > token && V::at(v[i], e) == xt;
+            for (int o = 32; o; o >>= 1) same += __shfl_xor(same, o, 64);
+            before += same;
+        }
     }
     // the part's ids, for what reads them again
     const int id0 = max(v0 * N - skew, 0), id1 = min(v_end * N - skew, vocab);
@@ -232,16 +239,17 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
         const uint64_t mine = key_of(xt, token);
         before = 0;
         for (int id = id0 + tid; id < id1; id += NT) before += key_of(V::one(x + id), (uint32_t)id) > mine;
+        for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o, 64);
     }
     for (int o = 32; o; o >>= 1) {
         l += __shfl_xor(l, o, 64);
         s += __shfl_xor(s, o, 64);
-        before += __shfl_xor(before, o, 64);
     }
     // the logits that reach the threshold
     if (a.top_k && thr > -INFINITY && top >= thr) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
+            if (i >= rounds) continue;
             repack(v[i]);
 #pragma unroll
             for (int e = 0; e < N; e++) {
@@ -336,10 +344,19 @@ __global__ __launch_bounds__(NT) void k_logprobs_join(lp_args a) {
     if (lane == 0) sh_part[wave] = p;
     uint64_t list = 0;
     if (a.top_k) {
+        // eight lists at a time, their loads ahead of the merges
         const uint64_t *keys = a.keys + (uint64_t)row * a.parts * a.top_k;
-        for (uint32_t i = wave; i < a.parts; i += NT / 64) {
-            const uint32_t j = 63 - lane;
-            list = merge64(list, j < a.top_k ? keys[(uint64_t)i * a.top_k + j] : 0, lane);
+        const uint32_t j = 63 - lane;
+        for (uint32_t i0 = wave; i0 < a.parts; i0 += 8 * (NT / 64)) {
+            uint64_t next[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const uint32_t i = i0 + u * (NT / 64);
+                next[u] = i < a.parts && j < a.top_k ? keys[(uint64_t)i * a.top_k + j] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (i0 + u * (NT / 64) < a.parts) list = merge64(list, next[u], lane);
         }
         sh_list[wave][lane] = list;
     }
