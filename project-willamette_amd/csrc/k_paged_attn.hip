@@ -24,8 +24,11 @@ namespace {
 
 constexpr int NT = 256;    // threads per workgroup, four waves
 constexpr int TILE = 64;   // positions per tile of one wave
-constexpr int W_EXP = 14;  // weights are formed times 2^W_EXP
+constexpr int W_EXP = 7;   // weights are formed times 2^W_EXP
+constexpr float GROWTH = 8.0f;  // and may grow by 2^GROWTH (below f16's 2^16) before the sums are scaled anew
 constexpr int E_NONE = -200;  // the exponent of a zero scale
+constexpr int FEW = 32;    // rows (tokens x group) of a sequence and kv head up to which a workgroup takes them all
+constexpr int MANY = 128;  // rows of a workgroup beyond
 
 struct attn_args {
     wm_paged_kv kv;
@@ -37,11 +40,24 @@ struct attn_args {
     uint32_t n_heads, group;
     int type;
     float scale_log2;  // scale * log2 e
-    // the split of the positions: n_splits workgroups of split_len each, and
-    // where they leave their partial rows (n_splits 1: none)
-    uint32_t split_len, n_splits, row_tiles;
+    // The positions are split over workgroups of split_len each where there
+    // are few rows; n splits of a sequence with few rows, and of one with many.
+    struct split {
+        uint32_t len, n;
+    } few, many;
+    uint32_t few_blocks;   // workgroups of sequences with few rows, in front of the others
+    uint32_t many_tiles;   // row tiles of MANY of a sequence and kv head, at most
+    // partial rows: [sequence][kv head][FEW rows][few.n], then [token][head][many.n]
     float *part_o, *part_lse;
 };
+// Where a row's partial results begin, in splits.
+__device__ __forceinline__ uint64_t few_part(const attn_args &a, uint32_t s, uint32_t h, int r) {
+    return (((uint64_t)s * a.kv.n_kv_heads + h) * FEW + r) * a.few.n;
+}
+__device__ __forceinline__ uint64_t many_part(const attn_args &a, uint64_t token, uint64_t head) {
+    return (a.few.n > 1 ? (uint64_t)a.b.n_seqs * a.kv.n_kv_heads * FEW * a.few.n : 0) +
+           (token * a.n_heads + head) * a.many.n;
+}
 
 // Sixteen codes to f16: 0x6400 | (code + 128) is 1024 + 128 + code.
 __device__ __forceinline__ void codes_to_f16(wm_u4 w, wm_h8 &lo, wm_h8 &hi) {
@@ -94,6 +110,21 @@ __device__ __forceinline__ void to_terms(float v, _Float16 *hi, _Float16 *lo) {
         *lo = (_Float16)(v - h);
     }
 }
+// Over the two halves of a wave.
+__device__ __forceinline__ float half_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float read_lane(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+// Score c (of 8) of the lane's half of the 16-position group g, in two 32 x 32 tiles.
+__device__ __forceinline__ float &s_at(wm_f16v (&s)[2], int g, int c) { return ((float *)&s[g / 2])[8 * (g % 2) + c]; }
+
 // f32 inputs take two terms, the half types one.
 template <int TERMS>
 __device__ __forceinline__ wm_f4 load_q4(const attn_args &a, uint64_t at) {
@@ -119,7 +150,7 @@ __device__ __forceinline__ row_tile load_tile(const attn_args &a, uint32_t s, ui
     row_tile r;
     r.q = wm_load_seq(a.b, s);
     r.s = s, r.h = h;
-    r.rows = r.q.n * (int)a.group;
+    r.rows = r.q.ok ? r.q.n * (int)a.group : 0;
     r.r0 = (int)t * per;
     const int last = (min(r.r0 + per, r.rows) - 1) / (int)a.group;
     r.len = min(max(r.q.start + last + 1, 0), r.q.len);
@@ -132,44 +163,43 @@ __device__ __forceinline__ uint64_t row_head(const attn_args &a, const row_tile 
     return (uint64_t)t.h * a.group + r % (int)a.group;
 }
 
-// A bad sequence's rows.
-__device__ __forceinline__ void poison_rows(const attn_args &a, const row_tile &t, int per, int d) {
+// Every row of a sequence whose lengths break their bounds, by one workgroup.
+__device__ __forceinline__ void poison_sequence(const attn_args &a, const row_tile &t, int d) {
     const float nan = __uint_as_float(0x7FC00000u);
-    const int n = min(per, t.rows - t.r0);
-    for (int i = threadIdx.x; i < n * (d / 4); i += NT) {
-        const int r = t.r0 + i / (d / 4);
-        const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r);
+    const int64_t per = (int64_t)a.group * (d / 4), n = t.q.n * per;
+    for (int64_t i = threadIdx.x; i < n; i += NT) {
+        const uint64_t tok = t.q.tok0 + i / per, head = (uint64_t)t.h * a.group + i % per / (d / 4);
         store_out4(a, tok * a.os + head * d + i % (d / 4) * 4, wm_f4{nan, nan, nan, nan});
         if (a.lse && i % (d / 4) == 0) a.lse[tok * a.n_heads + head] = nan;
     }
 }
 
-// One workgroup: NR row tiles of 16 rows, one split of the positions; its
+// Few rows.  One workgroup: NR row tiles of 16 rows, one split of the positions; its
 // four waves take the split's tiles in turn, each with sums of its own, and
 // meet in LDS at the end.  Decode reads every code once from HBM, which is
 // its bound; a tile's 16 KB are in flight per wave while the tile before is
 // worked on (K's registers are loaded again as soon as the scores are out,
 // V's after the second product).
+template <int D, int NR>
+struct few_shared {
+    float o[4][16 * NR][D + 4];
+    float lse[4][16 * NR];
+};
 template <int D, int NR, int TERMS>
-__global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
-    constexpr int ROWS = 16 * NR, KS = D / 32, DT = D / 16, LDO = D + 4;
-    __shared__ float sh_o[4][ROWS][LDO];
-    __shared__ float sh_lse[4][ROWS];
-    uint32_t id = blockIdx.x;
-    const uint32_t split = id % a.n_splits;
-    id /= a.n_splits;
-    const uint32_t rt = id % a.row_tiles;
-    id /= a.row_tiles;
-    const row_tile t = load_tile(a, id / a.kv.n_kv_heads, id % a.kv.n_kv_heads, rt, ROWS);
-    if (t.r0 >= t.rows) return;
+__device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_shared<D, NR> &sh) {
+    constexpr int ROWS = 16 * NR, KS = D / 32, DT = D / 16;
+    const uint32_t split = id % a.few.n;
+    id /= a.few.n;
+    const row_tile t = load_tile(a, id / a.kv.n_kv_heads, id % a.kv.n_kv_heads, 0, ROWS);
     if (!t.q.ok) {
-        if (split == 0) poison_rows(a, t, ROWS, D);
+        if (split == 0) poison_sequence(a, t, D);
         return;
     }
-    const int p0 = (int)(split * a.split_len);
+    if (t.rows == 0 || t.rows > FEW) return;
+    const int p0 = (int)(split * a.few.len);
     if (split && p0 >= t.len) return;
-    const int p1 = (int)min((int64_t)p0 + a.split_len, (int64_t)t.len);
-    const bool whole = t.len <= (int)a.split_len;
+    const int p1 = (int)min((int64_t)p0 + a.few.len, (int64_t)t.len);
+    const bool whole = t.len <= (int)a.few.len;
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
     // queries
@@ -298,7 +328,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
         const int eb0 = sc.v != 0.0f ? __builtin_amdgcn_frexp_expf(sc.v) : E_NONE;
         const int e_new = max(e_ref, group_max(eb0)), eb = max(eb0, e_new - 60);
         const float shift = (float)(eb - e_new), unshift = ldexpf(1.0f, e_new - eb), fb = ldexpf(sc.v, W_EXP - eb);
-        const float dm = (float)(e_new - e_ref);
+        const float dm = (float)(e_new - e_ref), regrow = ldexpf(1.0f, min(e_new - e_ref, 126));
         e_ref = e_new;
         const bool masked = p + TILE > all;
         wm_h8 w[NR][2][TERMS];
@@ -315,15 +345,20 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
             }
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, x[i]);
-            const float m_old = m[r] - dm, m_new = fmaxf(m_old, group_max(top));
-            const float base = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = __builtin_amdgcn_exp2f(m_old - base);
-            l[r] *= __builtin_amdgcn_exp2f(m[r] - base);
-            m[r] = m_new;
-            if (__ballot(alpha != 1.0f)) {
+            const float m_old = m[r] - dm;
+            top = group_max(top);
+            if (__ballot(top > m_old + GROWTH)) {
+                const float m_new = fmaxf(m_old, top), to = m_new == -INFINITY ? 0.0f : m_new;
+                const float alpha = __builtin_amdgcn_exp2f(m_old - to);
+                l[r] *= __builtin_amdgcn_exp2f(m[r] - to);
+                m[r] = m_new;
 #pragma unroll
                 for (int i = 0; i < DT; i++) o[r][i] *= alpha;
+            } else {
+                l[r] *= regrow;
+                m[r] = m_old;
             }
+            const float base = m[r] == -INFINITY ? 0.0f : m[r];
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -367,10 +402,10 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
             wm_f4 v = o[r][i] * inv;
 #pragma unroll
             for (int c = 0; c < 4; c++) v[c] = ldexpf(v[c], e_ref - W_EXP);
-            *(wm_f4 *)&sh_o[wave][16 * r + n][16 * i + 4 * g] = v;
+            *(wm_f4 *)&sh.o[wave][16 * r + n][16 * i + 4 * g] = v;
         }
         // a sum of 0 is that of a row without positions, or without a tile
-        if (g == 0) sh_lse[wave][16 * r + n] = sum == 0.0f ? -INFINITY : m[r] + __builtin_amdgcn_logf(sum);
+        if (g == 0) sh.lse[wave][16 * r + n] = sum == 0.0f ? -INFINITY : m[r] + __builtin_amdgcn_logf(sum);
     }
     __syncthreads();
     const int rows = min(ROWS, t.rows - t.r0);
@@ -378,7 +413,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
         const int row = i / (D / 4), c = i % (D / 4) * 4;
         float ls[4], top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; w++) ls[w] = sh_lse[w][row], top = fmaxf(top, ls[w]);
+        for (int w = 0; w < 4; w++) ls[w] = sh.lse[w][row], top = fmaxf(top, ls[w]);
         const float base = top == -INFINITY ? 0.0f : top;
         wm_f4 v = {0, 0, 0, 0};
         float sum = 0.0f;
@@ -386,35 +421,299 @@ __global__ __launch_bounds__(NT) void k_paged_attn_rows(attn_args a) {
         for (int w = 0; w < 4; w++) {
             const float e = __builtin_amdgcn_exp2f(ls[w] - base);
             sum += e;
-            v += *(const wm_f4 *)&sh_o[w][row][c] * e;
+            v += *(const wm_f4 *)&sh.o[w][row][c] * e;
         }
         if (sum != 0.0f) v *= 1.0f / sum;
         const float lse2 = sum == 0.0f ? -INFINITY : base + __builtin_amdgcn_logf(sum);
         const int r = t.r0 + row;
-        const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r), at = tok * a.n_heads + head;
+        const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r);
         if (whole) {
             store_out4(a, tok * a.os + head * D + c, v);
-            if (a.lse && c == 0) a.lse[at] = lse2 * 0.6931471805599453f;
+            if (a.lse && c == 0) a.lse[tok * a.n_heads + head] = lse2 * 0.6931471805599453f;
         } else {
-            *(wm_f4 *)(a.part_o + (at * a.n_splits + split) * D + c) = v;
-            if (c == 0) a.part_lse[at * a.n_splits + split] = lse2;
+            const uint64_t part = few_part(a, t.s, t.h, r) + split;
+            *(wm_f4 *)(a.part_o + part * D + c) = v;
+            if (c == 0) a.part_lse[part] = lse2;
         }
     }
 }
 
-// The splits' rows joined: weights 2^(lse - max), one thread per four dims.
+template <int D, int NR, int TERMS>
+__global__ __launch_bounds__(NT) void k_paged_attn_few(attn_args a) {
+    __shared__ few_shared<D, NR> sh;
+    attend_few<D, NR, TERMS>(a, blockIdx.x, sh);
+}
+
+// Many rows.  One workgroup: 128 rows of one sequence and kv head, 32 to a
+// wave, one split of the positions (all of them where there are workgroups
+// enough).  Its four waves share each tile of 64 positions: converted once to
+// f16 in LDS, K [position][dim], V [dim][position] with each 16 positions in
+// the order that a lane's half of the second product's K = 16 step takes
+// them (0-3, 8-11 | 4-7, 12-15), so both operands are 16-byte reads.  Rows are
+// padded by 16 bytes: 16 lanes' reads then fall into all 64 banks.  Two
+// buffers, one barrier per tile: the next tile's codes are loaded a tile
+// ahead and converted while the matrix cores work on this one.
 template <int D>
-__global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, int per) {
+struct many_shared {
+    _Float16 k[2][TILE][D + 8];
+    _Float16 v[2][D][TILE + 8];
+};
+template <int D, int TERMS>
+__device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, many_shared<D> &sh) {
+    constexpr int KS = D / 16, DT = D / 32, U = D / 64;  // units of 16 codes per thread, of K and of V
+    // the longest row tiles first: theirs are the last rows of the sequences
+    const uint32_t split = id % a.many.n;
+    id /= a.many.n;
+    const uint32_t unit = id % (a.b.n_seqs * a.kv.n_kv_heads), rt = a.many_tiles - 1 - id / (a.b.n_seqs * a.kv.n_kv_heads);
+    const row_tile t = load_tile(a, unit / a.kv.n_kv_heads, unit % a.kv.n_kv_heads, rt, MANY);
+    if (!t.q.ok || t.rows <= FEW || t.r0 >= t.rows) return;
+    const int p0 = (int)(split * a.many.len);
+    if (split && p0 >= t.len) return;
+    const int p1 = (int)min((int64_t)p0 + a.many.len, (int64_t)t.len);
+    const bool whole = t.len <= (int)a.many.len;
+
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
+    // this wave's rows; positions that all of them, and that any, attend to
+    const int w0 = t.r0 + 32 * wave, row = w0 + n;
+    const bool valid = row < t.rows;
+    const int all = t.q.start + w0 / (int)a.group + 1;
+    const int any = w0 < t.rows ? t.q.start + (min(w0 + 32, t.rows) - 1) / (int)a.group + 1 : 0;
+    const int count = valid ? t.q.start + row / (int)a.group + 1 : t.len;
+    wm_h8 q[KS][TERMS];
+    float kfac;
+    {
+        float x[KS][8], m = 0.0f;
+        const uint64_t at = valid ? row_token(a, t, row) * a.qs + row_head(a, t, row) * D : 0;
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                const wm_f4 v = valid ? load_q4<TERMS>(a, at + 16 * j + 8 * hi + i) : wm_f4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
+            }
+        const int e = __builtin_amdgcn_frexp_expf(half_max(m));
+        kfac = ldexpf(a.scale_log2, e - 15);
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                _Float16 h, lo;
+                to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &h, &lo);
+                q[j][0][i] = h;
+                if (TERMS > 1) q[j][TERMS - 1][i] = lo;
+            }
+    }
+    wm_f16v o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int c = 0; c < 16; c++) o[i][c] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    int e_ref = -300;
+
+    const uint32_t ps = a.kv.page_size, ps_log = 31 - __builtin_clz(ps);
+    const int32_t *table = a.b.page_table + (uint64_t)t.s * a.b.table_stride;
+    const uint64_t block = (uint64_t)ps * D;
+    // This thread's units: K's 16 dims (tid % (D / 16)) of one position each,
+    // V's 16 positions (group tid % 4) of one dim each.
+    const int kdim = tid % (D / 16) * 16, kpos = tid / (D / 16), vgrp = tid & 3, vdim = tid >> 2;
+    constexpr int KSTEP = NT / (D / 16), VSTEP = NT / 4;
+    int pk[U], pv;
+    auto load_pages = [&](int p) {
+        const int last = t.len - 1;
+#pragma unroll
+        for (int u = 0; u < U; u++) pk[u] = table[min(p + kpos + u * KSTEP, last) >> ps_log];
+        pv = table[min(p + 16 * vgrp, last) >> ps_log];
+    };
+    wm_u4 kr[U], vr[U];
+    float ks, vs;
+    auto load_codes = [&](int p) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint64_t pg = (uint32_t)pk[u] < a.kv.n_pages ? (uint32_t)pk[u] : 0;
+            kr[u] = *(const wm_u4 *)(a.kv.k_codes + (pg * a.kv.n_kv_heads + t.h) * block +
+                                     ((p + kpos + u * KSTEP) & (int)(ps - 1)) * D + kdim);
+        }
+        const bool good = (uint32_t)pv < a.kv.n_pages;
+        const uint64_t at = (good ? (uint64_t)(uint32_t)pv : 0) * a.kv.n_kv_heads + t.h;
+        const int8_t *src = a.kv.v_codes + at * block + ((p + 16 * vgrp) & (int)(ps - 1));
+#pragma unroll
+        for (int u = 0; u < U; u++) vr[u] = *(const wm_u4 *)(src + (uint64_t)(vdim + u * VSTEP) * ps);
+        ks = good ? a.kv.k_scales[at] : __uint_as_float(0x7FC00000u);
+        vs = good ? a.kv.v_scales[at] : 0.0f;
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            wm_h8 c0, c1;
+            codes_to_f16(kr[u], c0, c1);
+            *(wm_h8 *)&sh.k[buf][kpos + u * KSTEP][kdim] = c0;
+            *(wm_h8 *)&sh.k[buf][kpos + u * KSTEP][kdim + 8] = c1;
+            codes_to_f16(wm_u4{vr[u].x, vr[u].z, vr[u].y, vr[u].w}, c0, c1);
+            *(wm_h8 *)&sh.v[buf][vdim + u * VSTEP][16 * vgrp] = c0;
+            *(wm_h8 *)&sh.v[buf][vdim + u * VSTEP][16 * vgrp + 8] = c1;
+        }
+    };
+    if (p0 < p1) {
+        load_pages(p0);
+        load_codes(p0);
+        load_pages(p0 + TILE);
+        stage(0);
+    }
+    int buf = 0;
+    for (int p = p0; p < p1; p += TILE, buf ^= 1) {
+        // of this tile's scales, before the next tile's are loaded: as for few
+        // rows, the lane's group of 16 positions
+        const int eb0 = vs != 0.0f ? __builtin_amdgcn_frexp_expf(vs) : E_NONE;
+        int e_new = max(eb0, __builtin_amdgcn_mov_dpp(eb0, 0xB1, 0xF, 0xF, true));
+        e_new = max(e_ref, max(e_new, __builtin_amdgcn_mov_dpp(e_new, 0x4E, 0xF, 0xF, true)));
+        const int eb = max(eb0, e_new - 60);
+        const float my_shift = (float)(eb - e_new), my_unshift = ldexpf(1.0f, e_new - eb), my_fb = ldexpf(vs, W_EXP - eb);
+        const float my_ks = ks, dm = (float)(e_new - e_ref), regrow = ldexpf(1.0f, min(e_new - e_ref, 126));
+        e_ref = e_new;
+        const bool more = p + TILE < p1;
+        if (more) {
+            load_codes(p + TILE);
+            load_pages(p + 2 * TILE);
+        }
+        __syncthreads();
+        const bool live = p < any;
+        wm_h8 w[4][TERMS];
+        if (live) {
+            wm_f16v s[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int c = 0; c < 16; c++) s[i][c] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    const wm_h8 k = *(const wm_h8 *)&sh.k[buf][32 * i + n][16 * j + 8 * hi];
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++)
+                        s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[j][x], s[i], 0, 0, 0);
+                }
+            }
+            float top = -INFINITY;
+            const bool masked = p + TILE > all;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float f = kfac * read_lane(my_ks, g), shift = read_lane(my_shift, g);
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    float &x = s_at(s, g, c);
+                    x = __builtin_fmaf(x, f, shift);
+                }
+            }
+            if (masked) {
+                const int left = count - p - 4 * hi;
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        float &x = s_at(s, g, c);
+                        x = 16 * g + 8 * (c / 4) + c % 4 < left ? x : -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int c = 0; c < 8; c++) top = fmaxf(top, s_at(s, g, c));
+            top = half_max(top);
+            const float m_old = m - dm;
+            if (__ballot(top > m_old + GROWTH)) {
+                const float m_new = fmaxf(m_old, top), to = m_new == -INFINITY ? 0.0f : m_new;
+                const float alpha = __builtin_amdgcn_exp2f(m_old - to);
+                l *= __builtin_amdgcn_exp2f(m - to);
+                m = m_new;
+#pragma unroll
+                for (int i = 0; i < DT; i++) o[i] *= alpha;
+            } else {
+                l *= regrow;
+                m = m_old;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float fb = read_lane(my_fb, g), unshift = read_lane(my_unshift, g);
+                float sum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    const float e = __builtin_amdgcn_exp2f(s_at(s, g, c) - base);
+                    sum += e;
+                    _Float16 h, lo;
+                    to_terms<TERMS>(e * fb, &h, &lo);
+                    w[g][0][c] = h;
+                    if (TERMS > 1) w[g][TERMS - 1][c] = lo;
+                }
+                l = __builtin_fmaf(sum, unshift, l);
+            }
+        }
+        if (more) stage(buf ^ 1);
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const wm_h8 v = *(const wm_h8 *)&sh.v[buf][32 * i + n][16 * g + 8 * hi];
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[g][x], o[i], 0, 0, 0);
+                }
+        }
+    }
+    if (!valid) return;
+    const float sum = half_sum(l), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float lse2 = sum == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
+    const uint64_t tok = row_token(a, t, row), head = row_head(a, t, row);
+    const uint64_t part = whole ? 0 : many_part(a, tok, head) + split;
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int c = 0; c < 16; c += 4) {
+            wm_f4 v;
+#pragma unroll
+            for (int x = 0; x < 4; x++) v[x] = ldexpf(o[i][c + x] * inv, e_ref - W_EXP);
+            const int d = 32 * i + 2 * c + 4 * hi;
+            if (whole) store_out4(a, tok * a.os + head * D + d, v);
+            else *(wm_f4 *)(a.part_o + part * D + d) = v;
+        }
+    if (hi == 0) {
+        if (!whole) a.part_lse[part] = lse2;
+        else if (a.lse) a.lse[tok * a.n_heads + head] = lse2 * 0.6931471805599453f;
+    }
+}
+
+// A step with sequences of many rows; those with few are the first
+// workgroups.
+template <int D, int TERMS>
+__global__ __launch_bounds__(NT) void k_paged_attn_many(attn_args a) {
+    __shared__ union {
+        few_shared<D, FEW / 16> few;
+        many_shared<D> many;
+    } sh;
+    if (blockIdx.x < a.few_blocks) attend_few<D, FEW / 16, TERMS>(a, blockIdx.x, sh.few);
+    else attend_many<D, TERMS>(a, blockIdx.x - a.few_blocks, sh.many);
+}
+
+// The splits' rows joined: weights 2^(lse - max), one thread per four dims;
+// one workgroup per FEW rows of a sequence and kv head.
+template <int D>
+__global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t chunks) {
     uint32_t id = blockIdx.x;
-    const uint32_t rt = id % a.row_tiles;
-    id /= a.row_tiles;
-    const row_tile t = load_tile(a, id / a.kv.n_kv_heads, id % a.kv.n_kv_heads, rt, per);
-    if (t.r0 >= t.rows || !t.q.ok || t.len <= (int)a.split_len) return;
-    const int n = (t.len + (int)a.split_len - 1) / (int)a.split_len, rows = min(per, t.rows - t.r0);
+    const uint32_t chunk = id % chunks;
+    id /= chunks;
+    const uint32_t s = id / a.kv.n_kv_heads, h = id % a.kv.n_kv_heads;
+    row_tile t = load_tile(a, s, h, chunk / (MANY / FEW), MANY);
+    const bool few = t.rows <= FEW;
+    const auto split = few ? a.few : a.many;
+    const int r0 = (int)chunk * FEW, rows = min(FEW, t.rows - r0);
+    if (rows <= 0 || !t.q.ok || t.len <= (int)split.len) return;
+    const int n = (t.len + (int)split.len - 1) / (int)split.len;
     for (int i = threadIdx.x; i < rows * (D / 4); i += NT) {
-        const int r = t.r0 + i / (D / 4), c = i % (D / 4) * 4;
-        const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r), at = tok * a.n_heads + head;
-        const float *ls = a.part_lse + at * a.n_splits, *os = a.part_o + at * a.n_splits * D + c;
+        const int r = r0 + i / (D / 4), c = i % (D / 4) * 4;
+        const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r);
+        const uint64_t part = few ? few_part(a, s, h, r) : many_part(a, tok, head);
+        const float *ls = a.part_lse + part, *os = a.part_o + part * D + c;
         float top = -INFINITY;
         for (int s = 0; s < n; s++) top = fmaxf(top, ls[s]);
         const float base = top == -INFINITY ? 0.0f : top;
@@ -427,30 +726,48 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, int per) {
         }
         if (sum != 0.0f) v *= 1.0f / sum;
         store_out4(a, tok * a.os + head * D + c, v);
-        if (a.lse && c == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+        if (a.lse && c == 0)
+            a.lse[tok * a.n_heads + head] = sum == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
     }
 }
 
 // How a step is divided: from the host's bounds alone.
 struct attn_plan {
-    int nr;  // row tiles of 16 per workgroup
-    uint32_t split_len, n_splits, row_tiles;
-    uint64_t grid;
+    bool many;         // a sequence may have more than FEW rows
+    int nr;            // row tiles of 16 of the few
+    uint32_t many_tiles;
+    attn_args::split few_split, many_split;
+    uint64_t few_blocks, many_blocks;
+    size_t parts;      // partial rows
 };
+// Splits of `len` positions so that `units` workgroups become about `want`,
+// in whole multiples of `step`.
+attn_args::split make_split(uint64_t units, uint64_t want, uint32_t len, uint32_t step) {
+    const uint32_t steps = (len + step - 1) / step;
+    const uint64_t n = units ? (want + units - 1) / units : 1;
+    uint32_t per = (uint32_t)(n < steps ? steps / n : 1);
+    if (per < 1) per = 1;
+    return {per * step, steps ? (steps + per - 1) / per : 1};
+}
 attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
     attn_plan p;
-    const uint64_t rows = (uint64_t)b->max_new * (n_heads / kv->n_kv_heads);
+    const uint64_t rows = (uint64_t)b->max_new * (n_heads / kv->n_kv_heads), units = (uint64_t)b->n_seqs * kv->n_kv_heads;
+    p.many = rows > FEW;
     p.nr = rows > 16 ? 2 : 1;
-    p.row_tiles = (uint32_t)((rows + 16 * p.nr - 1) / (16 * p.nr));
-    const uint64_t units = (uint64_t)b->n_seqs * kv->n_kv_heads * p.row_tiles;
-    // splits of whole rounds of the four waves' tiles
-    const uint32_t round = 4 * TILE, rounds = (b->max_kv_len + round - 1) / round;
-    const uint64_t want = units ? 1024 / units + 1 : 1;
-    uint32_t per = rounds / (uint32_t)want;
-    if (per < 1) per = 1;
-    p.split_len = per * round;
-    p.n_splits = rounds ? (rounds + per - 1) / per : 1;
-    p.grid = units * p.n_splits;
+    // whole rounds of the four waves' tiles
+    p.few_split = make_split(units, 1024, b->max_kv_len, 4 * TILE);
+    p.few_blocks = units * p.few_split.n;
+    p.parts = p.few_split.n > 1 ? units * FEW * p.few_split.n : 0;
+    p.many_tiles = 0, p.many_blocks = 0, p.many_split = {0, 1};
+    if (p.many) {
+        p.many_tiles = (uint32_t)((rows + MANY - 1) / MANY);
+        // as many row tiles as the packed tokens can fill, not as many as the longest would in every sequence
+        const uint64_t full = (uint64_t)b->n_tokens * (n_heads / kv->n_kv_heads) / MANY + b->n_seqs;
+        const uint64_t tiles = full < (uint64_t)p.many_tiles * b->n_seqs ? full : (uint64_t)p.many_tiles * b->n_seqs;
+        p.many_split = make_split(tiles * kv->n_kv_heads, 512, b->max_kv_len, 4 * TILE);
+        p.many_blocks = units * p.many_tiles * p.many_split.n;
+        if (p.many_split.n > 1) p.parts += (size_t)b->n_tokens * n_heads * p.many_split.n;
+    }
     return p;
 }
 
@@ -460,9 +777,7 @@ extern "C" {
 
 size_t wm_paged_attention_workspace(const wm_paged_kv *kv, const wm_paged_batch *batch, uint32_t n_heads) {
     if (!kv || !batch || !kv->n_kv_heads || n_heads % kv->n_kv_heads) return 0;
-    const attn_plan p = make_plan(kv, batch, n_heads);
-    if (p.n_splits <= 1) return 0;
-    return (size_t)batch->n_tokens * n_heads * p.n_splits * (kv->head_dim + 1) * sizeof(float);
+    return make_plan(kv, batch, n_heads).parts * (kv->head_dim + 1) * sizeof(float);
 }
 
 wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
@@ -481,12 +796,13 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
     if ((st = wm_paged_check_array(ctx, who, "out", d_out, out_stride, n_heads, kv->head_dim, elem))) return st;
     if ((uintptr_t)d_lse % 4) return wm_set_error(ctx, WM_E_ARG, "%s: misaligned lse", who);
-    if ((uint64_t)batch->max_new * (n_heads / kv->n_kv_heads) > 0x7FFFFFFFull - 64)
+    if ((uint64_t)batch->max_new * (n_heads / kv->n_kv_heads) > 1u << 30)
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %u tokens of %u heads in one sequence", who, batch->max_new, n_heads);
     const attn_plan p = make_plan(kv, batch, n_heads);
-    if (p.grid > 0x7FFFFFFFull / NT)
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups in one step", who, (unsigned long long)p.grid);
-    const size_t need = wm_paged_attention_workspace(kv, batch, n_heads);
+    if (p.few_blocks + p.many_blocks > 0x7FFFFFFFull / NT)  // the launch counts threads in 32 bits
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups in one step", who,
+                            (unsigned long long)(p.few_blocks + p.many_blocks));
+    const size_t need = p.parts * (kv->head_dim + 1) * sizeof(float);
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
                             d_work ? work_bytes : (size_t)0, need);
@@ -498,32 +814,33 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.n_heads = n_heads, a.group = n_heads / kv->n_kv_heads;
     a.type = type;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.split_len = p.split_len, a.n_splits = p.n_splits, a.row_tiles = p.row_tiles;
+    a.few = p.few_split, a.many = p.many_split;
+    a.few_blocks = (uint32_t)p.few_blocks, a.many_tiles = p.many_tiles;
     a.part_o = (float *)d_work;
-    a.part_lse = a.part_o ? a.part_o + (size_t)batch->n_tokens * n_heads * p.n_splits * kv->head_dim : nullptr;
+    a.part_lse = a.part_o ? a.part_o + p.parts * kv->head_dim : nullptr;
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
-    const uint32_t grid = (uint32_t)p.grid;
+    const uint32_t grid = (uint32_t)(p.few_blocks + p.many_blocks);
     hipStream_t s = ctx->stream;
     const bool two = type == WM_DTYPE_F32;
-#define WM_ROWS(D_, NR_)                                                              \
-    do {                                                                              \
-        if (two) k_paged_attn_rows<D_, NR_, 2><<<grid, NT, 0, s>>>(a);                 \
-        else k_paged_attn_rows<D_, NR_, 1><<<grid, NT, 0, s>>>(a);                     \
+#define WM_ATTEND(D_)                                                                  \
+    do {                                                                               \
+        if (p.many && two) k_paged_attn_many<D_, 2><<<grid, NT, 0, s>>>(a);             \
+        else if (p.many) k_paged_attn_many<D_, 1><<<grid, NT, 0, s>>>(a);               \
+        else if (p.nr == 2 && two) k_paged_attn_few<D_, 2, 2><<<grid, NT, 0, s>>>(a);   \
+        else if (p.nr == 2) k_paged_attn_few<D_, 2, 1><<<grid, NT, 0, s>>>(a);          \
+        else if (two) k_paged_attn_few<D_, 1, 2><<<grid, NT, 0, s>>>(a);                \
+        else k_paged_attn_few<D_, 1, 1><<<grid, NT, 0, s>>>(a);                         \
     } while (0)
-    if (kv->head_dim == 64) {
-        if (p.nr == 1) WM_ROWS(64, 1);
-        else WM_ROWS(64, 2);
-    } else {
-        if (p.nr == 1) WM_ROWS(128, 1);
-        else WM_ROWS(128, 2);
-    }
-#undef WM_ROWS
+    if (kv->head_dim == 64) WM_ATTEND(64);
+    else WM_ATTEND(128);
+#undef WM_ATTEND
     WM_HIP(ctx, hipGetLastError());
-    if (p.n_splits > 1) {
-        const uint32_t g = grid / p.n_splits;
-        if (kv->head_dim == 64) k_paged_attn_join<64><<<g, NT, 0, s>>>(a, 16 * p.nr);
-        else k_paged_attn_join<128><<<g, NT, 0, s>>>(a, 16 * p.nr);
+    if (p.parts) {
+        const uint32_t chunks = p.many_split.n > 1 ? p.many_tiles * (MANY / FEW) : 1;
+        const uint64_t g = (uint64_t)batch->n_seqs * kv->n_kv_heads * chunks;
+        if (kv->head_dim == 64) k_paged_attn_join<64><<<(uint32_t)g, NT, 0, s>>>(a, chunks);
+        else k_paged_attn_join<128><<<(uint32_t)g, NT, 0, s>>>(a, chunks);
         WM_HIP(ctx, hipGetLastError());
     }
     return WM_OK;
