@@ -181,7 +181,7 @@ __device__ __forceinline__ void poison_sequence(const attn_args &a, const row_ti
 // worked on (K's registers are loaded again as soon as the scores are out,
 // V's after the second product).
 template <int D, int NR>
-struct few_shared {
+struct alignas(16) few_shared {
     float o[4][16 * NR][D + 4];
     float lse[4][16 * NR];
 };
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_few(attn_args a) {
 // buffers, one barrier per tile: the next tile's codes are loaded a tile
 // ahead and converted while the matrix cores work on this one.
 template <int D>
-struct many_shared {
+struct alignas(16) many_shared {
     _Float16 k[2][TILE][D + 8];
     _Float16 v[2][D][TILE + 8];
 };
@@ -687,7 +687,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
 // workgroups.
 template <int D, int TERMS>
 __global__ __launch_bounds__(NT) void k_paged_attn_many(attn_args a) {
-    __shared__ union {
+    __shared__ union alignas(16) {
         few_shared<D, FEW / 16> few;
         many_shared<D> many;
     } sh;
