@@ -5,9 +5,11 @@
 // v_mfma_f32_*_f16 multiplies them by f16 queries (weights) with f32 sums.
 // A query row is scaled by a power of two to [2^14, 2^15) and taken as one
 // f16 term (f16 and bf16 inputs: exact but for elements 2^-28 below the row's
-// largest) or two (f32: 22 bits).  Weights e^(s - max) * v_scale are scaled
-// the same way; one f16 term for half outputs (2^-12, under the output's
-// own rounding), two for f32.  Maxima, sums and accumulators are f32.
+// largest) or two (f32: 22 bits).  A weight 2^(s - max) * v_scale comes out of
+// one exponential, the scale's logarithm in its argument: the product of
+// the scores becomes the argument by one fma.  It is one f16 term for half
+// outputs (2^-11, no more than the output's own rounding), two for f32.
+// Maxima, sums and accumulators are f32.
 //
 // A wave holds scores transposed, S^T = K Q^T: lane l has query row l % 16
 // and 16 positions in a row, (l / 16) * 16 .. + 15 of a 64-position tile,
@@ -24,9 +26,9 @@ namespace {
 
 constexpr int NT = 256;    // threads per workgroup, four waves
 constexpr int TILE = 64;   // positions per tile of one wave
-constexpr int W_EXP = 7;   // weights are formed times 2^W_EXP
-constexpr float GROWTH = 8.0f;  // and may grow by 2^GROWTH (below f16's 2^16) before the sums are scaled anew
-constexpr int E_NONE = -200;  // the exponent of a zero scale
+constexpr float W_EXP = 7.0f;   // the largest weight is 2^W_EXP when the sums are scaled,
+constexpr float W_MOST = 15.0f; // and may grow to this before they are scaled anew (f16 ends at 2^16)
+constexpr int E_NONE = -200;    // the exponent of a zero scale
 constexpr int FEW = 32;    // rows (tokens x group) of a sequence and kv head up to which a workgroup takes them all
 constexpr int MANY = 128;  // rows of a workgroup beyond
 
@@ -122,8 +124,46 @@ __device__ __forceinline__ float half_sum(float v) {
 __device__ __forceinline__ float read_lane(float v, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
-// Score c (of 8) of the lane's half of the 16-position group g, in two 32 x 32 tiles.
-__device__ __forceinline__ float &s_at(wm_f16v (&s)[2], int g, int c) { return ((float *)&s[g / 2])[8 * (g % 2) + c]; }
+// The value scales' reference exponent over the tiles so far: what is held
+// is O 2^-e_ref, and the running maximum m is that of score + log2(scale) -
+// e_ref, so that the f16 weights hold their 11 bits relative to the largest
+// product of weight and scale, however the scales differ.  l = sum 2^(score -
+// m) has no e_ref in it.
+struct scale_ref {
+    int e = E_NONE;
+    float down = 0.0f;   // what m falls by in this tile, and l grows by 2^down
+    int excess = 0;      // what O falls by beyond that (scales more than 2^60 apart), almost never
+    __device__ __forceinline__ void raise(int to) {
+        const int d = e == E_NONE ? 0 : max(to - e, 0);  // before the first scale, O is 0
+        down = (float)min(d, 60), excess = d - min(d, 60);
+        e = max(e, to);
+    }
+    // log2 of a block's scale (of exponent eb) relative to e.  One 2^60 below
+    // it, or 0, counts as 2^-60: such a weight is 0 in f16.
+    __device__ __forceinline__ float part(float v, int eb) const {
+        return v == 0.0f || eb < e - 60 ? -60.0f : (float)(eb - e) + __builtin_amdgcn_logf(ldexpf(v, -eb));
+    }
+};
+// Under a new tile's largest relative score `top` (of the row): m, l and what
+// O is to be scaled by; `from` is what the scores are relative to.  True where
+// any row of the wave needs it.
+struct row_max {
+    float m = -INFINITY, l = 0.0f, from = 0.0f;
+    __device__ __forceinline__ void begin(const scale_ref &r) {
+        if (r.down != 0.0f) m -= r.down, l *= __builtin_amdgcn_exp2f(r.down);
+        from = m == -INFINITY ? 0.0f : m;
+    }
+    // Every lane's scores have then to be lowered by `by`, O scaled by `alpha`.
+    __device__ __forceinline__ bool grows(float top, float &by, float &alpha) {
+        if (!__ballot(top > (m == -INFINITY ? -INFINITY : W_MOST))) return false;
+        const float to = fmaxf(m, from + top - W_EXP), base = to == -INFINITY ? 0.0f : to;
+        alpha = __builtin_amdgcn_exp2f(m - base);
+        l *= alpha;
+        m = to;
+        by = base - from;
+        return true;
+    }
+};
 
 // f32 inputs take two terms, the half types one.
 template <int TERMS>
@@ -208,11 +248,11 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
     int count[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const int row = t.r0 + 16 * r + n;
-        const bool valid = row < t.rows;
-        count[r] = valid ? t.q.start + row / (int)a.group + 1 : t.len;
+        const int at_row = t.r0 + 16 * r + n;
+        const bool valid = at_row < t.rows;
+        count[r] = valid ? t.q.start + at_row / (int)a.group + 1 : t.len;
         float x[KS][8], m = 0.0f;
-        const uint64_t at = valid ? row_token(a, t, row) * a.qs + row_head(a, t, row) * D : 0;
+        const uint64_t at = valid ? row_token(a, t, at_row) * a.qs + row_head(a, t, at_row) * D : 0;
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
@@ -236,14 +276,12 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
     const int all = t.q.start + t.r0 / (int)a.group + 1;  // positions that every row attends to
 
     wm_f4 o[NR][DT];
-    float m[NR], l[NR];
+    row_max row[NR];
+    scale_ref ref;
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        m[r] = -INFINITY, l[r] = 0.0f;
+    for (int r = 0; r < NR; r++)
 #pragma unroll
         for (int i = 0; i < DT; i++) o[r][i] = wm_f4{0, 0, 0, 0};
-    }
-    int e_ref = -300;
 
     const uint32_t ps = a.kv.page_size, ps_log = 31 - __builtin_clz(ps);
     const int32_t *table = a.b.page_table + (uint64_t)t.s * a.b.table_stride;
@@ -320,24 +358,23 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
             sc_next = load_scales(pg_next.v);
             if (p + 8 * TILE < p1) pg_after = load_pages(p + 8 * TILE);
         }
-        // The values' scale 2^eb * [1/2, 1) goes into the weight: the score
-        // gets eb - e_ref (e_ref: the largest exponent so far, of any lane),
-        // so that the running maximum is that of the products and the f16
-        // weights hold their 11 bits relative to it, however the scales
-        // differ; the sum of the weights is taken without it.
-        const int eb0 = sc.v != 0.0f ? __builtin_amdgcn_frexp_expf(sc.v) : E_NONE;
-        const int e_new = max(e_ref, group_max(eb0)), eb = max(eb0, e_new - 60);
-        const float shift = (float)(eb - e_new), unshift = ldexpf(1.0f, e_new - eb), fb = ldexpf(sc.v, W_EXP - eb);
-        const float dm = (float)(e_new - e_ref), regrow = ldexpf(1.0f, min(e_new - e_ref, 126));
-        e_ref = e_new;
+        const int eb = sc.v != 0.0f ? __builtin_amdgcn_frexp_expf(sc.v) : E_NONE;
+        ref.raise(group_max(eb));
+        const float part = ref.part(sc.v, eb), back = __builtin_amdgcn_exp2f(-part);
+        if (ref.excess)
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+#pragma unroll
+                for (int i = 0; i < DT; i++) o[r][i] *= ldexpf(1.0f, -ref.excess);
         const bool masked = p + TILE > all;
         wm_h8 w[NR][2][TERMS];
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            const float f = kfac[r] * sc.k;
+            row[r].begin(ref);
+            const float f = kfac[r] * sc.k, c = part - row[r].from;
             float x[16], top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(s[r][i / 4][i % 4], f, shift);
+            for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(s[r][i / 4][i % 4], f, c);
             if (masked) {
                 const int left = count[r] - (p + g * 16);
 #pragma unroll
@@ -345,35 +382,24 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
             }
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, x[i]);
-            const float m_old = m[r] - dm;
-            top = group_max(top);
-            if (__ballot(top > m_old + GROWTH)) {
-                const float m_new = fmaxf(m_old, top), to = m_new == -INFINITY ? 0.0f : m_new;
-                const float alpha = __builtin_amdgcn_exp2f(m_old - to);
-                l[r] *= __builtin_amdgcn_exp2f(m[r] - to);
-                m[r] = m_new;
+            float by, alpha;
+            if (row[r].grows(group_max(top), by, alpha)) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[i] -= by;
 #pragma unroll
                 for (int i = 0; i < DT; i++) o[r][i] *= alpha;
-            } else {
-                l[r] *= regrow;
-                m[r] = m_old;
             }
-            const float base = m[r] == -INFINITY ? 0.0f : m[r];
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float e = __builtin_amdgcn_exp2f(x[i] - base);
+                const float e = __builtin_amdgcn_exp2f(x[i]);
                 sum += e;
-                x[i] = e * fb;
-            }
-            l[r] = __builtin_fmaf(sum, unshift, l[r]);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
                 _Float16 hi, lo;
-                to_terms<TERMS>(x[i], &hi, &lo);
+                to_terms<TERMS>(e, &hi, &lo);
                 w[r][i / 8][0][i % 8] = hi;
                 if (TERMS > 1) w[r][i / 8][TERMS - 1][i % 8] = lo;
             }
+            row[r].l = __builtin_fmaf(sum, back, row[r].l);
         }
 #pragma unroll
         for (int i = 0; i < DT; i++) {
@@ -395,17 +421,17 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
     // rows of this wave, normalised, with the log2 of their sums
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const float sum = group_sum(l[r]);
+        const float sum = group_sum(row[r].l);
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int i = 0; i < DT; i++) {
             wm_f4 v = o[r][i] * inv;
 #pragma unroll
-            for (int c = 0; c < 4; c++) v[c] = ldexpf(v[c], e_ref - W_EXP);
+            for (int c = 0; c < 4; c++) v[c] = ldexpf(v[c], ref.e);
             *(wm_f4 *)&sh.o[wave][16 * r + n][16 * i + 4 * g] = v;
         }
         // a sum of 0 is that of a row without positions, or without a tile
-        if (g == 0) sh.lse[wave][16 * r + n] = sum == 0.0f ? -INFINITY : m[r] + __builtin_amdgcn_logf(sum);
+        if (g == 0) sh.lse[wave][16 * r + n] = sum == 0.0f ? -INFINITY : row[r].m + __builtin_amdgcn_logf(sum);
     }
     __syncthreads();
     const int rows = min(ROWS, t.rows - t.r0);
@@ -474,16 +500,16 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     // this wave's rows; positions that all of them, and that any, attend to
-    const int w0 = t.r0 + 32 * wave, row = w0 + n;
-    const bool valid = row < t.rows;
+    const int w0 = t.r0 + 32 * wave, at_row = w0 + n;
+    const bool valid = at_row < t.rows;
     const int all = t.q.start + w0 / (int)a.group + 1;
     const int any = w0 < t.rows ? t.q.start + (min(w0 + 32, t.rows) - 1) / (int)a.group + 1 : 0;
-    const int count = valid ? t.q.start + row / (int)a.group + 1 : t.len;
+    const int count = valid ? t.q.start + at_row / (int)a.group + 1 : t.len;
     wm_h8 q[KS][TERMS];
     float kfac;
     {
         float x[KS][8], m = 0.0f;
-        const uint64_t at = valid ? row_token(a, t, row) * a.qs + row_head(a, t, row) * D : 0;
+        const uint64_t at = valid ? row_token(a, t, at_row) * a.qs + row_head(a, t, at_row) * D : 0;
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
@@ -509,8 +535,8 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
     for (int i = 0; i < DT; i++)
 #pragma unroll
         for (int c = 0; c < 16; c++) o[i][c] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    int e_ref = -300;
+    row_max row;
+    scale_ref ref;
 
     const uint32_t ps = a.kv.page_size, ps_log = 31 - __builtin_clz(ps);
     const int32_t *table = a.b.page_table + (uint64_t)t.s * a.b.table_stride;
@@ -565,13 +591,11 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
     for (int p = p0; p < p1; p += TILE, buf ^= 1) {
         // of this tile's scales, before the next tile's are loaded: as for few
         // rows, the lane's group of 16 positions
-        const int eb0 = vs != 0.0f ? __builtin_amdgcn_frexp_expf(vs) : E_NONE;
-        int e_new = max(eb0, __builtin_amdgcn_mov_dpp(eb0, 0xB1, 0xF, 0xF, true));
-        e_new = max(e_ref, max(e_new, __builtin_amdgcn_mov_dpp(e_new, 0x4E, 0xF, 0xF, true)));
-        const int eb = max(eb0, e_new - 60);
-        const float my_shift = (float)(eb - e_new), my_unshift = ldexpf(1.0f, e_new - eb), my_fb = ldexpf(vs, W_EXP - eb);
-        const float my_ks = ks, dm = (float)(e_new - e_ref), regrow = ldexpf(1.0f, min(e_new - e_ref, 126));
-        e_ref = e_new;
+        const int eb = vs != 0.0f ? __builtin_amdgcn_frexp_expf(vs) : E_NONE;
+        int e = max(eb, __builtin_amdgcn_mov_dpp(eb, 0xB1, 0xF, 0xF, true));  // over lanes l ^ 1, l ^ 2
+        e = max(e, __builtin_amdgcn_mov_dpp(e, 0x4E, 0xF, 0xF, true));
+        ref.raise(e);
+        const float my_ks = ks, my_part = ref.part(vs, eb), my_back = __builtin_amdgcn_exp2f(-my_part);
         const bool more = p + TILE < p1;
         if (more) {
             load_codes(p + TILE);
@@ -580,73 +604,68 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         __syncthreads();
         const bool live = p < any;
         wm_h8 w[4][TERMS];
+        row.begin(ref);
+        if (ref.excess)
+#pragma unroll
+            for (int i = 0; i < DT; i++) o[i] *= ldexpf(1.0f, -ref.excess);
         if (live) {
-            wm_f16v s[2];
+            // scores relative to the maximum so far, the values' scale included
+            float x[4][8];
+            {
+                wm_f16v s[2];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
+                for (int i = 0; i < 2; i++) {
+                    s[i] = wm_f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < 16; c++) s[i][c] = 0.0f;
+                    for (int j = 0; j < KS; j++) {
+                        const wm_h8 k = *(const wm_h8 *)&sh.k[buf][32 * i + n][16 * j + 8 * hi];
 #pragma unroll
-                for (int j = 0; j < KS; j++) {
-                    const wm_h8 k = *(const wm_h8 *)&sh.k[buf][32 * i + n][16 * j + 8 * hi];
+                        for (int y = 0; y < TERMS; y++)
+                            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[j][y], s[i], 0, 0, 0);
+                    }
+                }
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++)
-                        s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[j][x], s[i], 0, 0, 0);
+                for (int g = 0; g < 4; g++) {
+                    const float f = kfac * read_lane(my_ks, g), c = read_lane(my_part, g) - row.from;
+#pragma unroll
+                    for (int y = 0; y < 8; y++) x[g][y] = __builtin_fmaf(s[g / 2][8 * (g % 2) + y], f, c);
                 }
             }
-            float top = -INFINITY;
-            const bool masked = p + TILE > all;
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const float f = kfac * read_lane(my_ks, g), shift = read_lane(my_shift, g);
-#pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    float &x = s_at(s, g, c);
-                    x = __builtin_fmaf(x, f, shift);
-                }
-            }
-            if (masked) {
+            if (p + TILE > all) {
                 const int left = count - p - 4 * hi;
 #pragma unroll
                 for (int g = 0; g < 4; g++)
 #pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        float &x = s_at(s, g, c);
-                        x = 16 * g + 8 * (c / 4) + c % 4 < left ? x : -INFINITY;
-                    }
+                    for (int y = 0; y < 8; y++) x[g][y] = 16 * g + 8 * (y / 4) + y % 4 < left ? x[g][y] : -INFINITY;
             }
+            float top = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; g++)
 #pragma unroll
-                for (int c = 0; c < 8; c++) top = fmaxf(top, s_at(s, g, c));
-            top = half_max(top);
-            const float m_old = m - dm;
-            if (__ballot(top > m_old + GROWTH)) {
-                const float m_new = fmaxf(m_old, top), to = m_new == -INFINITY ? 0.0f : m_new;
-                const float alpha = __builtin_amdgcn_exp2f(m_old - to);
-                l *= __builtin_amdgcn_exp2f(m - to);
-                m = m_new;
+                for (int y = 0; y < 8; y++) top = fmaxf(top, x[g][y]);
+            float by, alpha;
+            if (row.grows(half_max(top), by, alpha)) {
 #pragma unroll
                 for (int i = 0; i < DT; i++) o[i] *= alpha;
-            } else {
-                l *= regrow;
-                m = m_old;
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int y = 0; y < 8; y++) x[g][y] -= by;
             }
-            const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const float fb = read_lane(my_fb, g), unshift = read_lane(my_unshift, g);
+                const float back = read_lane(my_back, g);
                 float sum = 0.0f;
 #pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    const float e = __builtin_amdgcn_exp2f(s_at(s, g, c) - base);
+                for (int y = 0; y < 8; y++) {
+                    const float e = __builtin_amdgcn_exp2f(x[g][y]);
                     sum += e;
                     _Float16 h, lo;
-                    to_terms<TERMS>(e * fb, &h, &lo);
-                    w[g][0][c] = h;
-                    if (TERMS > 1) w[g][TERMS - 1][c] = lo;
+                    to_terms<TERMS>(e, &h, &lo);
+                    w[g][0][y] = h;
+                    if (TERMS > 1) w[g][TERMS - 1][y] = lo;
                 }
-                l = __builtin_fmaf(sum, unshift, l);
+                row.l = __builtin_fmaf(sum, back, row.l);
             }
         }
         if (more) stage(buf ^ 1);
@@ -662,9 +681,9 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         }
     }
     if (!valid) return;
-    const float sum = half_sum(l), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float lse2 = sum == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(sum);
-    const uint64_t tok = row_token(a, t, row), head = row_head(a, t, row);
+    const float sum = half_sum(row.l), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float lse2 = sum == 0.0f ? -INFINITY : row.m + __builtin_amdgcn_logf(sum);
+    const uint64_t tok = row_token(a, t, at_row), head = row_head(a, t, at_row);
     const uint64_t part = whole ? 0 : many_part(a, tok, head) + split;
 #pragma unroll
     for (int i = 0; i < DT; i++)
@@ -672,7 +691,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         for (int c = 0; c < 16; c += 4) {
             wm_f4 v;
 #pragma unroll
-            for (int x = 0; x < 4; x++) v[x] = ldexpf(o[i][c + x] * inv, e_ref - W_EXP);
+            for (int x = 0; x < 4; x++) v[x] = ldexpf(o[i][c + x] * inv, ref.e);
             const int d = 32 * i + 2 * c + 4 * hi;
             if (whole) store_out4(a, tok * a.os + head * D + d, v);
             else *(wm_f4 *)(a.part_o + part * D + d) = v;
