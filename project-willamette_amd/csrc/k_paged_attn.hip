@@ -242,39 +242,6 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
     const bool whole = t.len <= (int)a.few.len;
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
-    // queries
-    wm_h8 q[NR][KS][TERMS];
-    float kfac[NR];
-    int count[NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const int at_row = t.r0 + 16 * r + n;
-        const bool valid = at_row < t.rows;
-        count[r] = valid ? t.q.start + at_row / (int)a.group + 1 : t.len;
-        float x[KS][8], m = 0.0f;
-        const uint64_t at = valid ? row_token(a, t, at_row) * a.qs + row_head(a, t, at_row) * D : 0;
-#pragma unroll
-        for (int j = 0; j < KS; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                const wm_f4 v = valid ? load_q4<TERMS>(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i) : wm_f4{0, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
-            }
-        const int e = __builtin_amdgcn_frexp_expf(group_max(m));
-        kfac[r] = ldexpf(a.scale_log2, e - 15);
-#pragma unroll
-        for (int j = 0; j < KS; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                _Float16 hi, lo;
-                to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &hi, &lo);
-                q[r][j][0][i] = hi;
-                if (TERMS > 1) q[r][j][TERMS - 1][i] = lo;
-            }
-    }
-    const int all = t.q.start + t.r0 / (int)a.group + 1;  // positions that every row attends to
-
     wm_f4 o[NR][DT];
     row_max row[NR];
     scale_ref ref;
@@ -332,6 +299,39 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
         load_v(p, pg.v);
         if (p + 4 * TILE < p1) pg_next = load_pages(p + 4 * TILE);
     }
+    // queries, behind the first codes' loads
+    wm_h8 q[NR][KS][TERMS];
+    float kfac[NR];
+    int count[NR];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        const int at_row = t.r0 + 16 * r + n;
+        const bool valid = at_row < t.rows;
+        count[r] = valid ? t.q.start + at_row / (int)a.group + 1 : t.len;
+        float x[KS][8], m = 0.0f;
+        const uint64_t at = valid ? row_token(a, t, at_row) * a.qs + row_head(a, t, at_row) * D : 0;
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                const wm_f4 v = valid ? load_q4<TERMS>(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i) : wm_f4{0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
+            }
+        const int e = __builtin_amdgcn_frexp_expf(group_max(m));
+        kfac[r] = ldexpf(a.scale_log2, e - 15);
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                _Float16 hi, lo;
+                to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &hi, &lo);
+                q[r][j][0][i] = hi;
+                if (TERMS > 1) q[r][j][TERMS - 1][i] = lo;
+            }
+    }
+    const int all = t.q.start + t.r0 / (int)a.group + 1;  // positions that every row attends to
+
     for (; p < p1; p += 4 * TILE) {
         const bool more = p + 4 * TILE < p1;
         wm_f4 s[NR][4];
@@ -733,16 +733,34 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
         const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r);
         const uint64_t part = few ? few_part(a, s, h, r) : many_part(a, tok, head);
         const float *ls = a.part_lse + part, *os = a.part_o + part * D + c;
-        float top = -INFINITY;
-        for (int s = 0; s < n; s++) top = fmaxf(top, ls[s]);
-        const float base = top == -INFINITY ? 0.0f : top;
+        // eight splits at a time, their loads together
         wm_f4 v = {0, 0, 0, 0};
-        float sum = 0.0f;
-        for (int s = 0; s < n; s++) {
-            const float e = __builtin_amdgcn_exp2f(ls[s] - base);
-            sum += e;
-            v += *(const wm_f4 *)(os + (uint64_t)s * D) * e;
+        float top = -INFINITY, sum = 0.0f;
+        for (int s0 = 0; s0 < n; s0 += 8) {
+            float z[8];
+            wm_f4 x[8];
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const int at = min(s0 + s, n - 1);
+                z[s] = ls[at];
+                x[s] = *(const wm_f4 *)(os + (uint64_t)at * D);
+            }
+            float m = top;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                if (s0 + s >= n) z[s] = -INFINITY;
+                m = fmaxf(m, z[s]);
+            }
+            const float to = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(top - to);
+            sum *= alpha, v *= alpha, top = m;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const float e = __builtin_amdgcn_exp2f(z[s] - to);
+                sum += e;
+                v += x[s] * e;
+            }
         }
+        const float base = top == -INFINITY ? 0.0f : top;
         if (sum != 0.0f) v *= 1.0f / sum;
         store_out4(a, tok * a.os + head * D + c, v);
         if (a.lse && c == 0)
