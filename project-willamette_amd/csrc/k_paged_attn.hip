@@ -40,6 +40,7 @@ struct attn_args {
     float *lse;
     uint64_t qs, os;
     uint32_t n_heads, group;
+    uint32_t few_recip;  // row * few_recip >> 16 is row / group for the first FEW rows
     int type;
     float scale_log2;  // scale * log2 e
     // The positions are split over workgroups of split_len each where there
@@ -305,16 +306,16 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
     int count[NR];
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        const int at_row = t.r0 + 16 * r + n;
-        const bool valid = at_row < t.rows;
-        count[r] = valid ? t.q.start + at_row / (int)a.group + 1 : t.len;
+        // (rows past the last repeat it, and are not written)
+        const int at_row = min(16 * r + n, t.rows - 1), j = (int)(at_row * a.few_recip >> 16);
+        count[r] = t.q.start + j + 1;
         float x[KS][8], m = 0.0f;
-        const uint64_t at = valid ? row_token(a, t, at_row) * a.qs + row_head(a, t, at_row) * D : 0;
+        const uint64_t at = (uint64_t)(t.q.tok0 + j) * a.qs + ((uint64_t)t.h * a.group + at_row - j * a.group) * D;
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
-                const wm_f4 v = valid ? load_q4<TERMS>(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i) : wm_f4{0, 0, 0, 0};
+                const wm_f4 v = load_q4<TERMS>(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i);
 #pragma unroll
                 for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
             }
@@ -422,14 +423,9 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         const float sum = group_sum(row[r].l);
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
 #pragma unroll
-        for (int i = 0; i < DT; i++) {
-            wm_f4 v = o[r][i] * inv;
-#pragma unroll
-            for (int c = 0; c < 4; c++) v[c] = ldexpf(v[c], ref.e);
-            *(wm_f4 *)&sh.o[wave][16 * r + n][16 * i + 4 * g] = v;
-        }
+        for (int i = 0; i < DT; i++) *(wm_f4 *)&sh.o[wave][16 * r + n][16 * i + 4 * g] = o[r][i] * inv;
         // a sum of 0 is that of a row without positions, or without a tile
         if (g == 0) sh.lse[wave][16 * r + n] = sum == 0.0f ? -INFINITY : row[r].m + __builtin_amdgcn_logf(sum);
     }
@@ -501,20 +497,22 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     // this wave's rows; positions that all of them, and that any, attend to
     const int w0 = t.r0 + 32 * wave, at_row = w0 + n;
+    // (rows past the last repeat it, and are not written)
     const bool valid = at_row < t.rows;
+    const int row = min(at_row, t.rows - 1), j = row / (int)a.group, count = t.q.start + j + 1;
     const int all = t.q.start + w0 / (int)a.group + 1;
     const int any = w0 < t.rows ? t.q.start + (min(w0 + 32, t.rows) - 1) / (int)a.group + 1 : 0;
-    const int count = valid ? t.q.start + at_row / (int)a.group + 1 : t.len;
+    const uint64_t tok = (uint64_t)(t.q.tok0 + j), head = (uint64_t)t.h * a.group + row - j * (int)a.group;
     wm_h8 q[KS][TERMS];
     float kfac;
     {
         float x[KS][8], m = 0.0f;
-        const uint64_t at = valid ? row_token(a, t, at_row) * a.qs + row_head(a, t, at_row) * D : 0;
+        const uint64_t at = tok * a.qs + head * D;
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
-                const wm_f4 v = valid ? load_q4<TERMS>(a, at + 16 * j + 8 * hi + i) : wm_f4{0, 0, 0, 0};
+                const wm_f4 v = load_q4<TERMS>(a, at + 16 * j + 8 * hi + i);
 #pragma unroll
                 for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
             }
@@ -535,7 +533,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
     for (int i = 0; i < DT; i++)
 #pragma unroll
         for (int c = 0; c < 16; c++) o[i][c] = 0.0f;
-    row_max row;
+    row_max sums;
     scale_ref ref;
 
     const uint32_t ps = a.kv.page_size, ps_log = 31 - __builtin_clz(ps);
@@ -604,7 +602,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         __syncthreads();
         const bool live = p < any;
         wm_h8 w[4][TERMS];
-        row.begin(ref);
+        sums.begin(ref);
         if (ref.excess)
 #pragma unroll
             for (int i = 0; i < DT; i++) o[i] *= ldexpf(1.0f, -ref.excess);
@@ -626,7 +624,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
                 }
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
-                    const float f = kfac * read_lane(my_ks, g), c = read_lane(my_part, g) - row.from;
+                    const float f = kfac * read_lane(my_ks, g), c = read_lane(my_part, g) - sums.from;
 #pragma unroll
                     for (int y = 0; y < 8; y++) x[g][y] = __builtin_fmaf(s[g / 2][8 * (g % 2) + y], f, c);
                 }
@@ -644,7 +642,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
 #pragma unroll
                 for (int y = 0; y < 8; y++) top = fmaxf(top, x[g][y]);
             float by, alpha;
-            if (row.grows(half_max(top), by, alpha)) {
+            if (sums.grows(half_max(top), by, alpha)) {
 #pragma unroll
                 for (int i = 0; i < DT; i++) o[i] *= alpha;
 #pragma unroll
@@ -665,7 +663,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
                     w[g][0][y] = h;
                     if (TERMS > 1) w[g][TERMS - 1][y] = lo;
                 }
-                row.l = __builtin_fmaf(sum, back, row.l);
+                sums.l = __builtin_fmaf(sum, back, sums.l);
             }
         }
         if (more) stage(buf ^ 1);
@@ -681,9 +679,8 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         }
     }
     if (!valid) return;
-    const float sum = half_sum(row.l), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float lse2 = sum == 0.0f ? -INFINITY : row.m + __builtin_amdgcn_logf(sum);
-    const uint64_t tok = row_token(a, t, at_row), head = row_head(a, t, at_row);
+    const float sum = half_sum(sums.l), inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
+    const float lse2 = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
     const uint64_t part = whole ? 0 : many_part(a, tok, head) + split;
 #pragma unroll
     for (int i = 0; i < DT; i++)
@@ -691,7 +688,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         for (int c = 0; c < 16; c += 4) {
             wm_f4 v;
 #pragma unroll
-            for (int x = 0; x < 4; x++) v[x] = ldexpf(o[i][c + x] * inv, ref.e);
+            for (int x = 0; x < 4; x++) v[x] = o[i][c + x] * inv;
             const int d = 32 * i + 2 * c + 4 * hi;
             if (whole) store_out4(a, tok * a.os + head * D + d, v);
             else *(wm_f4 *)(a.part_o + part * D + d) = v;
@@ -705,7 +702,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
 // A step with sequences of many rows; those with few are the first
 // workgroups.
 template <int D, int TERMS>
-__global__ __launch_bounds__(NT) void k_paged_attn_many(attn_args a) {
+__global__ __launch_bounds__(NT, 2) void k_paged_attn_many(attn_args a) {
     __shared__ union alignas(16) {
         few_shared<D, FEW / 16> few;
         many_shared<D> many;
@@ -849,6 +846,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.q = d_q, a.out = d_out, a.lse = d_lse;
     a.qs = q_stride, a.os = out_stride;
     a.n_heads = n_heads, a.group = n_heads / kv->n_kv_heads;
+    a.few_recip = (0x10000 + a.group - 1) / a.group;
     a.type = type;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.few = p.few_split, a.many = p.many_split;
