@@ -29,7 +29,7 @@ constexpr int TILE = 64;   // positions per tile of one wave
 constexpr float W_EXP = 7.0f;   // the largest weight is 2^W_EXP when the sums are scaled,
 constexpr float W_MOST = 15.0f; // and may grow to this before they are scaled anew (f16 ends at 2^16)
 constexpr int E_NONE = -200;    // the exponent of a zero scale
-constexpr int FEW = 32;    // rows (tokens x group) of a sequence and kv head up to which a workgroup takes them all
+constexpr int FEW = 16;    // rows (tokens x group) of a sequence and kv head up to which a wave takes them all
 constexpr int MANY = 128;  // rows of a workgroup beyond
 
 struct attn_args {
@@ -43,24 +43,68 @@ struct attn_args {
     uint32_t few_recip;  // row * few_recip >> 16 is row / group for the first FEW rows
     int type;
     float scale_log2;  // scale * log2 e
-    // The positions are split over workgroups of split_len each where there
-    // are few rows; n splits of a sequence with few rows, and of one with many.
-    struct split {
-        uint32_t len, n;
-    } few, many;
-    uint32_t few_blocks;   // workgroups of sequences with few rows, in front of the others
-    uint32_t many_tiles;   // row tiles of MANY of a sequence and kv head, at most
-    // partial rows: [sequence][kv head][FEW rows][few.n], then [token][head][many.n]
+    // Sequences of few rows: few_blocks workgroups share all their positions
+    // evenly (few_share).  Those of many: many_n workgroups of many_len
+    // positions each per row tile, many_tiles row tiles of MANY at most.
+    uint32_t few_blocks, many_tiles, many_len, many_n;
+    // partial rows: FEW of each few_share::slot, then [token][head][many_n]
     float *part_o, *part_lse;
 };
-// Where a row's partial results begin, in splits.
-__device__ __forceinline__ uint64_t few_part(const attn_args &a, uint32_t s, uint32_t h, int r) {
-    return (((uint64_t)s * a.kv.n_kv_heads + h) * FEW + r) * a.few.n;
-}
+constexpr int ROUND = 4 * TILE;  // positions that a workgroup's four waves take at once
+__host__ __device__ inline uint64_t few_slots(uint32_t blocks, uint32_t units) { return (uint64_t)blocks + units; }
 __device__ __forceinline__ uint64_t many_part(const attn_args &a, uint64_t token, uint64_t head) {
-    return (a.few.n > 1 ? (uint64_t)a.b.n_seqs * a.kv.n_kv_heads * FEW * a.few.n : 0) +
-           (token * a.n_heads + head) * a.many.n;
+    return (a.few_blocks ? few_slots(a.few_blocks, a.b.n_seqs * a.kv.n_kv_heads) * FEW : 0) +
+           (token * a.n_heads + head) * a.many_n;
 }
+
+// The rounds of all sequences of few rows, (sequence, kv head, round) in
+// order, dealt to the workgroups in runs of `per`: as even as lengths that
+// only the device knows allow, and a workgroup has more than one (sequence,
+// kv head) only where its run goes past an end.  Every wave scans the
+// lengths by itself, 64 sequences at a time.
+struct few_share {
+    uint32_t per;
+    // the rounds of sequence s for one kv head (one to write empty or bad rows)
+    static __device__ __forceinline__ int rounds(const attn_args &a, uint32_t s) {
+        if (s >= a.b.n_seqs) return 0;
+        const wm_seq q = wm_load_seq(a.b, s);
+        if (!q.ok) return 1;
+        if (q.n == 0 || (int64_t)q.n * a.group > FEW) return 0;
+        return max(1, (q.len + ROUND - 1) / ROUND);
+    }
+    uint32_t total = 0;  // the host keeps it below 2^31
+    __device__ __forceinline__ few_share(const attn_args &a) {
+        for (uint32_t s = 0; s < a.b.n_seqs; s += 64) total += wm_wave_total_i32(rounds(a, s + (threadIdx.x & 63)));
+        total *= a.kv.n_kv_heads;
+        per = max((total + a.few_blocks - 1) / a.few_blocks, 1u);
+    }
+    // The sequence that round x is of, its rounds and the first of them.
+    struct place {
+        uint32_t s, rounds, first;
+    };
+    static __device__ __forceinline__ place find(const attn_args &a, uint32_t x) {
+        uint32_t base = 0;
+        for (uint32_t s = 0;; s += 64) {
+            const int r = rounds(a, s + (threadIdx.x & 63)), upto = wm_wave_scan_i32(r);
+            const uint64_t hit = __ballot(base + upto * a.kv.n_kv_heads > x);
+            if (hit) {
+                const int lane = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(r, lane);
+                return {s + lane, (uint32_t)n, base + (__builtin_amdgcn_readlane(upto, lane) - n) * a.kv.n_kv_heads};
+            }
+            base += __builtin_amdgcn_readlane(upto, 63) * a.kv.n_kv_heads;
+        }
+    }
+    // The first round of sequence s.
+    static __device__ __forceinline__ uint32_t first_of(const attn_args &a, uint32_t s) {
+        uint32_t n = 0;
+        for (uint32_t i = 0; i < s; i += 64)
+            n += wm_wave_total_i32(i + (threadIdx.x & 63) < s ? rounds(a, i + (threadIdx.x & 63)) : 0);
+        return n * a.kv.n_kv_heads;
+    }
+    // Where workgroup w leaves its part of a unit (sequence, kv head): along
+    // the runs either grows by one at a time.
+    static __device__ __forceinline__ uint64_t slot(uint64_t w, uint64_t unit) { return w + unit; }
+};
 
 // Sixteen codes to f16: 0x6400 | (code + 128) is 1024 + 128 + code.
 __device__ __forceinline__ void codes_to_f16(wm_u4 w, wm_h8 &lo, wm_h8 &hi) {
@@ -125,6 +169,8 @@ __device__ __forceinline__ float half_sum(float v) {
 __device__ __forceinline__ float read_lane(float v, int lane) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // The value scales' reference exponent over the tiles so far: what is held
 // is O 2^-e_ref, and the running maximum m is that of score + log2(scale) -
 // e_ref, so that the f16 weights hold their 11 bits relative to the largest
@@ -190,6 +236,9 @@ struct row_tile {
 __device__ __forceinline__ row_tile load_tile(const attn_args &a, uint32_t s, uint32_t h, uint32_t t, int per) {
     row_tile r;
     r.q = wm_load_seq(a.b, s);
+    // of the whole workgroup: in scalar registers
+    r.q.tok0 = uniform(r.q.tok0), r.q.n = uniform(r.q.n), r.q.start = uniform(r.q.start), r.q.len = uniform(r.q.len);
+    r.q.ok = uniform(r.q.ok);
     r.s = s, r.h = h;
     r.rows = r.q.ok ? r.q.n * (int)a.group : 0;
     r.r0 = (int)t * per;
@@ -215,41 +264,34 @@ __device__ __forceinline__ void poison_sequence(const attn_args &a, const row_ti
     }
 }
 
-// Few rows.  One workgroup: NR row tiles of 16 rows, one split of the positions; its
-// four waves take the split's tiles in turn, each with sums of its own, and
-// meet in LDS at the end.  Decode reads every code once from HBM, which is
+// Few rows.  One workgroup: the 16 rows of one MFMA tile, some rounds of one
+// sequence's positions; its four waves take a tile of each round, each with
+// sums of its own, and meet in LDS at the end.  Decode reads every code once from HBM, which is
 // its bound; a tile's 16 KB are in flight per wave while the tile before is
 // worked on (K's registers are loaded again as soon as the scores are out,
 // V's after the second product).
-template <int D, int NR>
+template <int D>
 struct alignas(16) few_shared {
-    float o[4][16 * NR][D + 4];
-    float lse[4][16 * NR];
+    float o[4][FEW][D + 4];
+    float lse[4][FEW];
 };
-template <int D, int NR, int TERMS>
-__device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_shared<D, NR> &sh) {
-    constexpr int ROWS = 16 * NR, KS = D / 32, DT = D / 16;
-    const uint32_t split = id % a.few.n;
-    id /= a.few.n;
-    const row_tile t = load_tile(a, id / a.kv.n_kv_heads, id % a.kv.n_kv_heads, 0, ROWS);
+template <int D, int TERMS>
+__device__ __forceinline__ void attend_few_part(const attn_args &a, uint32_t s, uint32_t h, uint32_t k0, uint32_t k1, bool whole,
+                                                uint64_t slot, few_shared<D> &sh) {
+    constexpr int KS = D / 32, DT = D / 16;
+    const row_tile t = load_tile(a, s, h, 0, FEW);
     if (!t.q.ok) {
-        if (split == 0) poison_sequence(a, t, D);
+        poison_sequence(a, t, D);
         return;
     }
-    if (t.rows == 0 || t.rows > FEW) return;
-    const int p0 = (int)(split * a.few.len);
-    if (split && p0 >= t.len) return;
-    const int p1 = (int)min((int64_t)p0 + a.few.len, (int64_t)t.len);
-    const bool whole = t.len <= (int)a.few.len;
+    const int p0 = (int)k0 * ROUND, p1 = min((int)k1 * ROUND, t.len);
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
-    wm_f4 o[NR][DT];
-    row_max row[NR];
+    wm_f4 o[DT];
+    row_max sums;
     scale_ref ref;
 #pragma unroll
-    for (int r = 0; r < NR; r++)
-#pragma unroll
-        for (int i = 0; i < DT; i++) o[r][i] = wm_f4{0, 0, 0, 0};
+    for (int i = 0; i < DT; i++) o[i] = wm_f4{0, 0, 0, 0};
 
     const uint32_t ps = a.kv.page_size, ps_log = 31 - __builtin_clz(ps);
     const int32_t *table = a.b.page_table + (uint64_t)t.s * a.b.table_stride;
@@ -301,14 +343,13 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
         if (p + 4 * TILE < p1) pg_next = load_pages(p + 4 * TILE);
     }
     // queries, behind the first codes' loads
-    wm_h8 q[NR][KS][TERMS];
-    float kfac[NR];
-    int count[NR];
-#pragma unroll
-    for (int r = 0; r < NR; r++) {
+    wm_h8 q[KS][TERMS];
+    float kfac;
+    int count;
+    {
         // (rows past the last repeat it, and are not written)
-        const int at_row = min(16 * r + n, t.rows - 1), j = (int)(at_row * a.few_recip >> 16);
-        count[r] = t.q.start + j + 1;
+        const int at_row = min(n, t.rows - 1), j = (int)(at_row * a.few_recip >> 16);
+        count = t.q.start + j + 1;
         float x[KS][8], m = 0.0f;
         const uint64_t at = (uint64_t)(t.q.tok0 + j) * a.qs + ((uint64_t)t.h * a.group + at_row - j * a.group) * D;
 #pragma unroll
@@ -320,37 +361,34 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
                 for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
             }
         const int e = __builtin_amdgcn_frexp_expf(group_max(m));
-        kfac[r] = ldexpf(a.scale_log2, e - 15);
+        kfac = ldexpf(a.scale_log2, e - 15);
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 _Float16 hi, lo;
                 to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &hi, &lo);
-                q[r][j][0][i] = hi;
-                if (TERMS > 1) q[r][j][TERMS - 1][i] = lo;
+                q[j][0][i] = hi;
+                if (TERMS > 1) q[j][TERMS - 1][i] = lo;
             }
     }
     const int all = t.q.start + t.r0 / (int)a.group + 1;  // positions that every row attends to
 
     for (; p < p1; p += 4 * TILE) {
         const bool more = p + 4 * TILE < p1;
-        wm_f4 s[NR][4];
+        wm_f4 s[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-#pragma unroll
-            for (int r = 0; r < NR; r++) s[r][i] = wm_f4{0, 0, 0, 0};
+            s[i] = wm_f4{0, 0, 0, 0};
 #pragma unroll
             for (int j = 0; j < D / 64; j++) {
                 wm_h8 k0, k1;
                 codes_to_f16(kr[i][j], k0, k1);
 #pragma unroll
-                for (int r = 0; r < NR; r++)
-#pragma unroll
-                    for (int w = 0; w < TERMS; w++) {
-                        s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[r][2 * j][w], s[r][i], 0, 0, 0);
-                        s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[r][2 * j + 1][w], s[r][i], 0, 0, 0);
-                    }
+                for (int w = 0; w < TERMS; w++) {
+                    s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q[2 * j][w], s[i], 0, 0, 0);
+                    s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q[2 * j + 1][w], s[i], 0, 0, 0);
+                }
             }
         }
         pages pg_after{0, 0};
@@ -364,55 +402,48 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
         const float part = ref.part(sc.v, eb), back = __builtin_amdgcn_exp2f(-part);
         if (ref.excess)
 #pragma unroll
-            for (int r = 0; r < NR; r++)
-#pragma unroll
-                for (int i = 0; i < DT; i++) o[r][i] *= ldexpf(1.0f, -ref.excess);
+            for (int i = 0; i < DT; i++) o[i] *= ldexpf(1.0f, -ref.excess);
         const bool masked = p + TILE > all;
-        wm_h8 w[NR][2][TERMS];
+        wm_h8 w[2][TERMS];
+        sums.begin(ref);
+        const float f = kfac * sc.k, c = part - sums.from;
+        float x[16], top = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            row[r].begin(ref);
-            const float f = kfac[r] * sc.k, c = part - row[r].from;
-            float x[16], top = -INFINITY;
+        for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(s[i / 4][i % 4], f, c);
+        if (masked) {
+            const int left = count - (p + g * 16);
 #pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(s[r][i / 4][i % 4], f, c);
-            if (masked) {
-                const int left = count[r] - (p + g * 16);
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] = i < left ? x[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, x[i]);
-            float by, alpha;
-            if (row[r].grows(group_max(top), by, alpha)) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) x[i] -= by;
-#pragma unroll
-                for (int i = 0; i < DT; i++) o[r][i] *= alpha;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float e = __builtin_amdgcn_exp2f(x[i]);
-                sum += e;
-                _Float16 hi, lo;
-                to_terms<TERMS>(e, &hi, &lo);
-                w[r][i / 8][0][i % 8] = hi;
-                if (TERMS > 1) w[r][i / 8][TERMS - 1][i % 8] = lo;
-            }
-            row[r].l = __builtin_fmaf(sum, back, row[r].l);
+            for (int i = 0; i < 16; i++) x[i] = i < left ? x[i] : -INFINITY;
         }
+#pragma unroll
+        for (int i = 0; i < 16; i++) top = fmaxf(top, x[i]);
+        float by, alpha;
+        if (sums.grows(group_max(top), by, alpha)) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] -= by;
+#pragma unroll
+            for (int i = 0; i < DT; i++) o[i] *= alpha;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float e = __builtin_amdgcn_exp2f(x[i]);
+            sum += e;
+            _Float16 hi, lo;
+            to_terms<TERMS>(e, &hi, &lo);
+            w[i / 8][0][i % 8] = hi;
+            if (TERMS > 1) w[i / 8][TERMS - 1][i % 8] = lo;
+        }
+        sums.l = __builtin_fmaf(sum, back, sums.l);
 #pragma unroll
         for (int i = 0; i < DT; i++) {
             wm_h8 v0, v1;
             codes_to_f16(vr[i], v0, v1);
 #pragma unroll
-            for (int r = 0; r < NR; r++)
-#pragma unroll
-                for (int x = 0; x < TERMS; x++) {
-                    o[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[r][0][x], o[r][i], 0, 0, 0);
-                    o[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[r][1][x], o[r][i], 0, 0, 0);
-                }
+            for (int y = 0; y < TERMS; y++) {
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w[0][y], o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w[1][y], o[i], 0, 0, 0);
+            }
         }
         if (more) load_v(p + 4 * TILE, pg_next.v);
         pg_next = pg_after;
@@ -420,17 +451,15 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
     }
 
     // rows of this wave, normalised, with the log2 of their sums
+    {
+        const float sum = group_sum(sums.l), inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        const float sum = group_sum(row[r].l);
-        const float inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
-#pragma unroll
-        for (int i = 0; i < DT; i++) *(wm_f4 *)&sh.o[wave][16 * r + n][16 * i + 4 * g] = o[r][i] * inv;
+        for (int i = 0; i < DT; i++) *(wm_f4 *)&sh.o[wave][n][16 * i + 4 * g] = o[i] * inv;
         // a sum of 0 is that of a row without positions, or without a tile
-        if (g == 0) sh.lse[wave][16 * r + n] = sum == 0.0f ? -INFINITY : row[r].m + __builtin_amdgcn_logf(sum);
+        if (g == 0) sh.lse[wave][n] = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
     }
     __syncthreads();
-    const int rows = min(ROWS, t.rows - t.r0);
+    const int rows = t.rows;
     for (int i = tid; i < rows * (D / 4); i += NT) {
         const int row = i / (D / 4), c = i % (D / 4) * 4;
         float ls[4], top = -INFINITY;
@@ -453,17 +482,35 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t id, few_
             store_out4(a, tok * a.os + head * D + c, v);
             if (a.lse && c == 0) a.lse[tok * a.n_heads + head] = lse2 * 0.6931471805599453f;
         } else {
-            const uint64_t part = few_part(a, t.s, t.h, r) + split;
+            const uint64_t part = slot * FEW + row;
             *(wm_f4 *)(a.part_o + part * D + c) = v;
             if (c == 0) a.part_lse[part] = lse2;
         }
     }
 }
 
-template <int D, int NR, int TERMS>
-__global__ __launch_bounds__(NT) void k_paged_attn_few(attn_args a) {
-    __shared__ few_shared<D, NR> sh;
-    attend_few<D, NR, TERMS>(a, blockIdx.x, sh);
+template <int D, int TERMS>
+__device__ __forceinline__ void attend_few(const attn_args &a, uint32_t w, few_shared<D> &sh) {
+    const few_share all(a);
+    const uint32_t end = uniform(min((w + 1) * all.per, all.total));
+    for (uint32_t x = uniform(w * all.per); x < end;) {
+        const auto f = few_share::find(a, x);
+        // its kv heads from round x on
+        while (x < end && x < f.first + f.rounds * a.kv.n_kv_heads) {
+            const uint32_t h = uniform((x - f.first) / f.rounds), k0 = x - f.first - h * f.rounds;
+            const uint32_t k1 = min(f.rounds, k0 + (end - x));
+            attend_few_part<D, TERMS>(a, f.s, h, k0, k1, k1 - k0 == f.rounds,
+                                          few_share::slot(w, (uint64_t)f.s * a.kv.n_kv_heads + h), sh);
+            x += k1 - k0;
+            if (x < end) __syncthreads();  // the next part writes where this one was joined
+        }
+    }
+}
+
+template <int D, int TERMS>
+__global__ __launch_bounds__(NT, 2) void k_paged_attn_few(attn_args a) {
+    __shared__ few_shared<D> sh;
+    attend_few<D, TERMS>(a, blockIdx.x, sh);
 }
 
 // Many rows.  One workgroup: 128 rows of one sequence and kv head, 32 to a
@@ -484,15 +531,15 @@ template <int D, int TERMS>
 __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, many_shared<D> &sh) {
     constexpr int KS = D / 16, DT = D / 32, U = D / 64;  // units of 16 codes per thread, of K and of V
     // the longest row tiles first: theirs are the last rows of the sequences
-    const uint32_t split = id % a.many.n;
-    id /= a.many.n;
+    const uint32_t split = id % a.many_n;
+    id /= a.many_n;
     const uint32_t unit = id % (a.b.n_seqs * a.kv.n_kv_heads), rt = a.many_tiles - 1 - id / (a.b.n_seqs * a.kv.n_kv_heads);
     const row_tile t = load_tile(a, unit / a.kv.n_kv_heads, unit % a.kv.n_kv_heads, rt, MANY);
     if (!t.q.ok || t.rows <= FEW || t.r0 >= t.rows) return;
-    const int p0 = (int)(split * a.many.len);
+    const int p0 = (int)(split * a.many_len);
     if (split && p0 >= t.len) return;
-    const int p1 = (int)min((int64_t)p0 + a.many.len, (int64_t)t.len);
-    const bool whole = t.len <= (int)a.many.len;
+    const int p1 = (int)min((int64_t)p0 + a.many_len, (int64_t)t.len);
+    const bool whole = t.len <= (int)a.many_len;
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
     // this wave's rows; positions that all of them, and that any, attend to
@@ -704,14 +751,14 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
 template <int D, int TERMS>
 __global__ __launch_bounds__(NT, 2) void k_paged_attn_many(attn_args a) {
     __shared__ union alignas(16) {
-        few_shared<D, FEW / 16> few;
+        few_shared<D> few;
         many_shared<D> many;
     } sh;
-    if (blockIdx.x < a.few_blocks) attend_few<D, FEW / 16, TERMS>(a, blockIdx.x, sh.few);
+    if (blockIdx.x < a.few_blocks) attend_few<D, TERMS>(a, blockIdx.x, sh.few);
     else attend_many<D, TERMS>(a, blockIdx.x - a.few_blocks, sh.many);
 }
 
-// The splits' rows joined: weights 2^(lse - max), one thread per four dims;
+// The rows' parts joined: weights 2^(lse - max), one thread per four dims;
 // one workgroup per FEW rows of a sequence and kv head.
 template <int D>
 __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t chunks) {
@@ -721,14 +768,25 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
     const uint32_t s = id / a.kv.n_kv_heads, h = id % a.kv.n_kv_heads;
     row_tile t = load_tile(a, s, h, chunk / (MANY / FEW), MANY);
     const bool few = t.rows <= FEW;
-    const auto split = few ? a.few : a.many;
     const int r0 = (int)chunk * FEW, rows = min(FEW, t.rows - r0);
-    if (rows <= 0 || !t.q.ok || t.len <= (int)split.len) return;
-    const int n = (t.len + (int)split.len - 1) / (int)split.len;
+    if (rows <= 0 || !t.q.ok || (few && !a.few_blocks)) return;
+    int n;
+    uint64_t first = 0;
+    if (few) {
+        const few_share all(a);
+        const uint32_t r = few_share::rounds(a, s), x = few_share::first_of(a, s) + r * h;
+        const uint32_t w0 = x / all.per, w1 = (x + r - 1) / all.per;
+        n = (int)(w1 - w0) + 1;
+        first = few_share::slot(w0, (uint64_t)s * a.kv.n_kv_heads + h) * FEW;
+    } else {
+        n = (t.len + (int)a.many_len - 1) / (int)a.many_len;
+    }
+    if (n <= 1) return;  // written whole
+    const uint64_t step = few ? FEW : 1;  // rows from one part of a row to its next
     for (int i = threadIdx.x; i < rows * (D / 4); i += NT) {
         const int r = r0 + i / (D / 4), c = i % (D / 4) * 4;
         const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r);
-        const uint64_t part = few ? few_part(a, s, h, r) : many_part(a, tok, head);
+        const uint64_t part = few ? first + r : many_part(a, tok, head);
         const float *ls = a.part_lse + part, *os = a.part_o + part * D + c;
         // eight splits at a time, their loads together
         wm_f4 v = {0, 0, 0, 0};
@@ -739,8 +797,8 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
 #pragma unroll
             for (int s = 0; s < 8; s++) {
                 const int at = min(s0 + s, n - 1);
-                z[s] = ls[at];
-                x[s] = *(const wm_f4 *)(os + (uint64_t)at * D);
+                z[s] = ls[at * step];
+                x[s] = *(const wm_f4 *)(os + at * step * D);
             }
             float m = top;
 #pragma unroll
@@ -768,39 +826,38 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
 // How a step is divided: from the host's bounds alone.
 struct attn_plan {
     bool many;         // a sequence may have more than FEW rows
-    int nr;            // row tiles of 16 of the few
-    uint32_t many_tiles;
-    attn_args::split few_split, many_split;
+    uint32_t many_tiles, many_len, many_n;
     uint64_t few_blocks, many_blocks;
+    bool join;
     size_t parts;      // partial rows
+    uint64_t rounds;   // of all sequences and kv heads, at most
 };
-// Splits of `len` positions so that `units` workgroups become about `want`,
-// in whole multiples of `step`.
-attn_args::split make_split(uint64_t units, uint64_t want, uint32_t len, uint32_t step) {
-    const uint32_t steps = (len + step - 1) / step;
-    const uint64_t n = units ? (want + units - 1) / units : 1;
-    uint32_t per = (uint32_t)(n < steps ? steps / n : 1);
-    if (per < 1) per = 1;
-    return {per * step, steps ? (steps + per - 1) / per : 1};
-}
+// Two workgroups of the kernel for few rows fit a compute unit.
+constexpr uint64_t FEW_BLOCKS = 512;
 attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
     attn_plan p;
     const uint64_t rows = (uint64_t)b->max_new * (n_heads / kv->n_kv_heads), units = (uint64_t)b->n_seqs * kv->n_kv_heads;
+    const uint32_t rounds = b->max_kv_len > ROUND ? (b->max_kv_len + ROUND - 1) / ROUND : 1;
     p.many = rows > FEW;
-    p.nr = rows > 16 ? 2 : 1;
-    // whole rounds of the four waves' tiles
-    p.few_split = make_split(units, 1024, b->max_kv_len, 4 * TILE);
-    p.few_blocks = units * p.few_split.n;
-    p.parts = p.few_split.n > 1 ? units * FEW * p.few_split.n : 0;
-    p.many_tiles = 0, p.many_blocks = 0, p.many_split = {0, 1};
+    p.few_blocks = units * rounds < FEW_BLOCKS ? units * rounds : FEW_BLOCKS;
+    p.parts = rounds > 1 ? (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW : 0;
+    p.join = rounds > 1;
+    p.rounds = units * rounds;
+    p.many_tiles = 0, p.many_blocks = 0, p.many_len = 0, p.many_n = 1;
     if (p.many) {
         p.many_tiles = (uint32_t)((rows + MANY - 1) / MANY);
         // as many row tiles as the packed tokens can fill, not as many as the longest would in every sequence
         const uint64_t full = (uint64_t)b->n_tokens * (n_heads / kv->n_kv_heads) / MANY + b->n_seqs;
         const uint64_t tiles = full < (uint64_t)p.many_tiles * b->n_seqs ? full : (uint64_t)p.many_tiles * b->n_seqs;
-        p.many_split = make_split(tiles * kv->n_kv_heads, 512, b->max_kv_len, 4 * TILE);
-        p.many_blocks = units * p.many_tiles * p.many_split.n;
-        if (p.many_split.n > 1) p.parts += (size_t)b->n_tokens * n_heads * p.many_split.n;
+        const uint64_t want = (512 + tiles * kv->n_kv_heads - 1) / (tiles * kv->n_kv_heads);
+        const uint32_t per = want < rounds ? (uint32_t)(rounds / want) : 1;
+        p.many_len = per * ROUND;
+        p.many_n = (rounds + per - 1) / per;
+        p.many_blocks = units * p.many_tiles * p.many_n;
+        if (p.many_n > 1) {
+            p.parts = (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW;
+            p.parts += (size_t)b->n_tokens * n_heads * p.many_n;
+        }
     }
     return p;
 }
@@ -833,7 +890,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if ((uint64_t)batch->max_new * (n_heads / kv->n_kv_heads) > 1u << 30)
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %u tokens of %u heads in one sequence", who, batch->max_new, n_heads);
     const attn_plan p = make_plan(kv, batch, n_heads);
-    if (p.few_blocks + p.many_blocks > 0x7FFFFFFFull / NT)  // the launch counts threads in 32 bits
+    if (p.few_blocks + p.many_blocks > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups in one step", who,
                             (unsigned long long)(p.few_blocks + p.many_blocks));
     const size_t need = p.parts * (kv->head_dim + 1) * sizeof(float);
@@ -849,8 +906,8 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.few_recip = (0x10000 + a.group - 1) / a.group;
     a.type = type;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.few = p.few_split, a.many = p.many_split;
-    a.few_blocks = (uint32_t)p.few_blocks, a.many_tiles = p.many_tiles;
+    a.few_blocks = (uint32_t)p.few_blocks;
+    a.many_tiles = p.many_tiles, a.many_len = p.many_len, a.many_n = p.many_n;
     a.part_o = (float *)d_work;
     a.part_lse = a.part_o ? a.part_o + p.parts * kv->head_dim : nullptr;
     wm_device_guard dev(ctx->device);
@@ -862,17 +919,15 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     do {                                                                               \
         if (p.many && two) k_paged_attn_many<D_, 2><<<grid, NT, 0, s>>>(a);             \
         else if (p.many) k_paged_attn_many<D_, 1><<<grid, NT, 0, s>>>(a);               \
-        else if (p.nr == 2 && two) k_paged_attn_few<D_, 2, 2><<<grid, NT, 0, s>>>(a);   \
-        else if (p.nr == 2) k_paged_attn_few<D_, 2, 1><<<grid, NT, 0, s>>>(a);          \
-        else if (two) k_paged_attn_few<D_, 1, 2><<<grid, NT, 0, s>>>(a);                \
-        else k_paged_attn_few<D_, 1, 1><<<grid, NT, 0, s>>>(a);                         \
+        else if (two) k_paged_attn_few<D_, 2><<<grid, NT, 0, s>>>(a);                   \
+        else k_paged_attn_few<D_, 1><<<grid, NT, 0, s>>>(a);                            \
     } while (0)
     if (kv->head_dim == 64) WM_ATTEND(64);
     else WM_ATTEND(128);
 #undef WM_ATTEND
     WM_HIP(ctx, hipGetLastError());
-    if (p.parts) {
-        const uint32_t chunks = p.many_split.n > 1 ? p.many_tiles * (MANY / FEW) : 1;
+    if (p.join) {
+        const uint32_t chunks = p.many_n > 1 ? p.many_tiles * (MANY / FEW) : 1;
         const uint64_t g = (uint64_t)batch->n_seqs * kv->n_kv_heads * chunks;
         if (kv->head_dim == 64) k_paged_attn_join<64><<<(uint32_t)g, NT, 0, s>>>(a, chunks);
         else k_paged_attn_join<128><<<(uint32_t)g, NT, 0, s>>>(a, chunks);
