@@ -49,8 +49,15 @@ struct attn_args {
     uint32_t few_blocks, many_tiles, many_len, many_n;
     // partial rows: FEW of each few_share::slot, then [token][head][many_n]
     float *part_o, *part_lse;
+    // of each (sequence of few rows, kv head): the first workgroup that has a part of it, and how many have
+    uint32_t *few_parts;
 };
 constexpr int ROUND = 4 * TILE;  // positions that a workgroup's four waves take at once
+// Two workgroups of the kernel for few rows fit a compute unit.  Up to twice
+// as many rounds are one workgroup's each; more are shared by those that fit:
+// 318 rounds twice against 636 took 20.7 us against 19.5, 11400 rounds over
+// 1024 workgroups 144 us against 139 over 512.
+constexpr uint32_t FEW_RESIDENT = 512;
 __host__ __device__ inline uint64_t few_slots(uint32_t blocks, uint32_t units) { return (uint64_t)blocks + units; }
 __device__ __forceinline__ uint64_t many_part(const attn_args &a, uint64_t token, uint64_t head) {
     return (a.few_blocks ? few_slots(a.few_blocks, a.b.n_seqs * a.kv.n_kv_heads) * FEW : 0) +
@@ -63,43 +70,57 @@ __device__ __forceinline__ uint64_t many_part(const attn_args &a, uint64_t token
 // kv head) only where its run goes past an end.  Every wave scans the
 // lengths by itself, 64 sequences at a time.
 struct few_share {
-    uint32_t per;
-    // the rounds of sequence s for one kv head (one to write empty or bad rows)
-    static __device__ __forceinline__ int rounds(const attn_args &a, uint32_t s) {
-        if (s >= a.b.n_seqs) return 0;
-        const wm_seq q = wm_load_seq(a.b, s);
+    uint32_t per, total = 0;  // the host keeps the total below 2^31
+    // the first 64 sequences, one to a lane, as the scan found them
+    wm_seq q;
+    uint32_t mine, upto;
+    // the rounds of a sequence for one kv head (one to write empty or bad rows)
+    static __device__ __forceinline__ uint32_t rounds(const attn_args &a, const wm_seq &q) {
         if (!q.ok) return 1;
         if (q.n == 0 || (int64_t)q.n * a.group > FEW) return 0;
         return max(1, (q.len + ROUND - 1) / ROUND);
     }
-    uint32_t total = 0;  // the host keeps it below 2^31
+    static __device__ __forceinline__ void scan(const attn_args &a, uint32_t s0, wm_seq &q, uint32_t &mine, uint32_t &upto) {
+        const uint32_t s = s0 + (threadIdx.x & 63);
+        q = wm_load_seq(a.b, min(s, a.b.n_seqs - 1));
+        mine = s < a.b.n_seqs ? rounds(a, q) : 0;
+        upto = wm_wave_scan_i32(mine);
+    }
     __device__ __forceinline__ few_share(const attn_args &a) {
-        for (uint32_t s = 0; s < a.b.n_seqs; s += 64) total += wm_wave_total_i32(rounds(a, s + (threadIdx.x & 63)));
+        scan(a, 0, q, mine, upto);
+        total = __builtin_amdgcn_readlane(upto, 63);
+        for (uint32_t s = 64; s < a.b.n_seqs; s += 64) {
+            wm_seq x;
+            uint32_t m, u;
+            scan(a, s, x, m, u);
+            total += __builtin_amdgcn_readlane(u, 63);
+        }
         total *= a.kv.n_kv_heads;
-        per = max((total + a.few_blocks - 1) / a.few_blocks, 1u);
+        per = total <= a.few_blocks ? 1 : (total + FEW_RESIDENT - 1) / FEW_RESIDENT;
     }
     // The sequence that round x is of, its rounds and the first of them.
     struct place {
+        wm_seq q;
         uint32_t s, rounds, first;
     };
-    static __device__ __forceinline__ place find(const attn_args &a, uint32_t x) {
-        uint32_t base = 0;
+    __device__ __forceinline__ place find(const attn_args &a, uint32_t x) const {
+        uint32_t base = 0, m = mine, u = upto;
+        wm_seq at = q;
         for (uint32_t s = 0;; s += 64) {
-            const int r = rounds(a, s + (threadIdx.x & 63)), upto = wm_wave_scan_i32(r);
-            const uint64_t hit = __ballot(base + upto * a.kv.n_kv_heads > x);
+            if (s) scan(a, s, at, m, u);
+            const uint64_t hit = __ballot(base + u * a.kv.n_kv_heads > x);
             if (hit) {
-                const int lane = __builtin_ctzll(hit), n = __builtin_amdgcn_readlane(r, lane);
-                return {s + lane, (uint32_t)n, base + (__builtin_amdgcn_readlane(upto, lane) - n) * a.kv.n_kv_heads};
+                const int lane = __builtin_ctzll(hit);
+                const uint32_t n = __builtin_amdgcn_readlane(m, lane);
+                place p;
+                p.s = s + lane, p.rounds = n, p.first = base + (__builtin_amdgcn_readlane(u, lane) - n) * a.kv.n_kv_heads;
+                p.q.tok0 = __builtin_amdgcn_readlane(at.tok0, lane), p.q.n = __builtin_amdgcn_readlane(at.n, lane);
+                p.q.start = __builtin_amdgcn_readlane(at.start, lane), p.q.len = __builtin_amdgcn_readlane(at.len, lane);
+                p.q.ok = __builtin_amdgcn_readlane(at.ok, lane);
+                return p;
             }
-            base += __builtin_amdgcn_readlane(upto, 63) * a.kv.n_kv_heads;
+            base += __builtin_amdgcn_readlane(u, 63) * a.kv.n_kv_heads;
         }
-    }
-    // The first round of sequence s.
-    static __device__ __forceinline__ uint32_t first_of(const attn_args &a, uint32_t s) {
-        uint32_t n = 0;
-        for (uint32_t i = 0; i < s; i += 64)
-            n += wm_wave_total_i32(i + (threadIdx.x & 63) < s ? rounds(a, i + (threadIdx.x & 63)) : 0);
-        return n * a.kv.n_kv_heads;
     }
     // Where workgroup w leaves its part of a unit (sequence, kv head): along
     // the runs either grows by one at a time.
@@ -233,18 +254,22 @@ struct row_tile {
     int rows, r0;  // rows of the sequence and head; the tile's first
     int len;       // positions that the tile's last row attends to
 };
-__device__ __forceinline__ row_tile load_tile(const attn_args &a, uint32_t s, uint32_t h, uint32_t t, int per) {
+__device__ __forceinline__ row_tile make_tile(const attn_args &a, const wm_seq &q, uint32_t s, uint32_t h, uint32_t t, int per) {
     row_tile r;
-    r.q = wm_load_seq(a.b, s);
-    // of the whole workgroup: in scalar registers
-    r.q.tok0 = uniform(r.q.tok0), r.q.n = uniform(r.q.n), r.q.start = uniform(r.q.start), r.q.len = uniform(r.q.len);
-    r.q.ok = uniform(r.q.ok);
+    r.q = q;
     r.s = s, r.h = h;
     r.rows = r.q.ok ? r.q.n * (int)a.group : 0;
     r.r0 = (int)t * per;
     const int last = (min(r.r0 + per, r.rows) - 1) / (int)a.group;
     r.len = min(max(r.q.start + last + 1, 0), r.q.len);
     return r;
+}
+__device__ __forceinline__ row_tile load_tile(const attn_args &a, uint32_t s, uint32_t h, uint32_t t, int per) {
+    wm_seq q = wm_load_seq(a.b, s);
+    // of the whole workgroup: in scalar registers
+    q.tok0 = uniform(q.tok0), q.n = uniform(q.n), q.start = uniform(q.start), q.len = uniform(q.len);
+    q.ok = uniform(q.ok);
+    return make_tile(a, q, s, h, t, per);
 }
 __device__ __forceinline__ uint64_t row_token(const attn_args &a, const row_tile &t, int r) {
     return (uint64_t)(t.q.tok0 + r / (int)a.group);
@@ -276,10 +301,10 @@ struct alignas(16) few_shared {
     float lse[4][FEW];
 };
 template <int D, int TERMS>
-__device__ __forceinline__ void attend_few_part(const attn_args &a, uint32_t s, uint32_t h, uint32_t k0, uint32_t k1, bool whole,
-                                                uint64_t slot, few_shared<D> &sh) {
+__device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq &seq, uint32_t s, uint32_t h, uint32_t k0,
+                                                uint32_t k1, bool whole, uint64_t slot, few_shared<D> &sh) {
     constexpr int KS = D / 32, DT = D / 16;
-    const row_tile t = load_tile(a, s, h, 0, FEW);
+    const row_tile t = make_tile(a, seq, s, h, 0, FEW);
     if (!t.q.ok) {
         poison_sequence(a, t, D);
         return;
@@ -337,41 +362,45 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, uint32_t s, 
     scales sc{0, 0}, sc_next{0, 0};
     if (p < p1) {
         pg = load_pages(p);
-        sc = load_scales(pg.v);
-        load_k(p, pg.k);
-        load_v(p, pg.v);
         if (p + 4 * TILE < p1) pg_next = load_pages(p + 4 * TILE);
     }
-    // queries, behind the first codes' loads
-    wm_h8 q[KS][TERMS];
-    float kfac;
-    int count;
+    // The queries' loads go out with the page ids', in front of the codes'.
+    // Rows past the last repeat it, and are not written.
+    const int at_row = min(n, t.rows - 1), j_row = (int)(at_row * a.few_recip >> 16), count = t.q.start + j_row + 1;
+    float x_q[KS][8], q_max = 0.0f;
     {
-        // (rows past the last repeat it, and are not written)
-        const int at_row = min(n, t.rows - 1), j = (int)(at_row * a.few_recip >> 16);
-        count = t.q.start + j + 1;
-        float x[KS][8], m = 0.0f;
-        const uint64_t at = (uint64_t)(t.q.tok0 + j) * a.qs + ((uint64_t)t.h * a.group + at_row - j * a.group) * D;
+        const uint64_t at = (uint64_t)(t.q.tok0 + j_row) * a.qs + ((uint64_t)t.h * a.group + at_row - j_row * a.group) * D;
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
                 const wm_f4 v = load_q4<TERMS>(a, at + j / 2 * 64 + g * 16 + j % 2 * 8 + i);
 #pragma unroll
-                for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
-            }
-        const int e = __builtin_amdgcn_frexp_expf(group_max(m));
-        kfac = ldexpf(a.scale_log2, e - 15);
-#pragma unroll
-        for (int j = 0; j < KS; j++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                _Float16 hi, lo;
-                to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &hi, &lo);
-                q[j][0][i] = hi;
-                if (TERMS > 1) q[j][TERMS - 1][i] = lo;
+                for (int c = 0; c < 4; c++) x_q[j][i + c] = v[c];
             }
     }
+    if (p < p1) {
+        load_k(p, pg.k);
+        load_v(p, pg.v);
+        sc = load_scales(pg.v);
+    }
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) q_max = fmaxf(q_max, fabsf(x_q[j][i]));
+    // queries
+    wm_h8 q[KS][TERMS];
+    const int e = __builtin_amdgcn_frexp_expf(group_max(q_max));
+    const float kfac = ldexpf(a.scale_log2, e - 15), q_scale = ldexpf(1.0f, 15 - e);
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            _Float16 hi, lo;
+            to_terms<TERMS>(x_q[j][i] * q_scale, &hi, &lo);
+            q[j][0][i] = hi;
+            if (TERMS > 1) q[j][TERMS - 1][i] = lo;
+        }
     const int all = t.q.start + t.r0 / (int)a.group + 1;  // positions that every row attends to
 
     for (; p < p1; p += 4 * TILE) {
@@ -494,13 +523,15 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t w, few_s
     const few_share all(a);
     const uint32_t end = uniform(min((w + 1) * all.per, all.total));
     for (uint32_t x = uniform(w * all.per); x < end;) {
-        const auto f = few_share::find(a, x);
+        const auto f = all.find(a, x);
         // its kv heads from round x on
         while (x < end && x < f.first + f.rounds * a.kv.n_kv_heads) {
             const uint32_t h = uniform((x - f.first) / f.rounds), k0 = x - f.first - h * f.rounds;
             const uint32_t k1 = min(f.rounds, k0 + (end - x));
-            attend_few_part<D, TERMS>(a, f.s, h, k0, k1, k1 - k0 == f.rounds,
-                                          few_share::slot(w, (uint64_t)f.s * a.kv.n_kv_heads + h), sh);
+            const uint32_t unit = f.s * a.kv.n_kv_heads + h;
+            if (k0 == 0 && a.few_parts && threadIdx.x == 0)
+                *(wm_u2 *)(a.few_parts + 2 * unit) = wm_u2{w, (x + f.rounds - 1) / all.per - w + 1};
+            attend_few_part<D, TERMS>(a, f.q, f.s, h, k0, k1, k1 - k0 == f.rounds, few_share::slot(w, unit), sh);
             x += k1 - k0;
             if (x < end) __syncthreads();  // the next part writes where this one was joined
         }
@@ -766,18 +797,17 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
     const uint32_t chunk = id % chunks;
     id /= chunks;
     const uint32_t s = id / a.kv.n_kv_heads, h = id % a.kv.n_kv_heads;
-    row_tile t = load_tile(a, s, h, chunk / (MANY / FEW), MANY);
+    const uint32_t unit = s * a.kv.n_kv_heads + h;
+    const wm_u2 parts = a.few_blocks ? *(const wm_u2 *)(a.few_parts + 2 * unit) : wm_u2{0, 0};  // where its rows are few
+    const row_tile t = load_tile(a, s, h, chunk / (MANY / FEW), MANY);
     const bool few = t.rows <= FEW;
     const int r0 = (int)chunk * FEW, rows = min(FEW, t.rows - r0);
-    if (rows <= 0 || !t.q.ok || (few && !a.few_blocks)) return;
+    if (rows <= 0 || !t.q.ok) return;
     int n;
     uint64_t first = 0;
     if (few) {
-        const few_share all(a);
-        const uint32_t r = few_share::rounds(a, s), x = few_share::first_of(a, s) + r * h;
-        const uint32_t w0 = x / all.per, w1 = (x + r - 1) / all.per;
-        n = (int)(w1 - w0) + 1;
-        first = few_share::slot(w0, (uint64_t)s * a.kv.n_kv_heads + h) * FEW;
+        n = (int)parts.y;
+        first = few_share::slot(parts.x, unit) * FEW;
     } else {
         n = (t.len + (int)a.many_len - 1) / (int)a.many_len;
     }
@@ -832,14 +862,12 @@ struct attn_plan {
     size_t parts;      // partial rows
     uint64_t rounds;   // of all sequences and kv heads, at most
 };
-// Two workgroups of the kernel for few rows fit a compute unit.
-constexpr uint64_t FEW_BLOCKS = 512;
 attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
     attn_plan p;
     const uint64_t rows = (uint64_t)b->max_new * (n_heads / kv->n_kv_heads), units = (uint64_t)b->n_seqs * kv->n_kv_heads;
     const uint32_t rounds = b->max_kv_len > ROUND ? (b->max_kv_len + ROUND - 1) / ROUND : 1;
     p.many = rows > FEW;
-    p.few_blocks = units * rounds < FEW_BLOCKS ? units * rounds : FEW_BLOCKS;
+    p.few_blocks = units * rounds < 2 * FEW_RESIDENT ? units * rounds : 2 * FEW_RESIDENT;
     p.parts = rounds > 1 ? (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW : 0;
     p.join = rounds > 1;
     p.rounds = units * rounds;
@@ -856,10 +884,15 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
         p.many_blocks = units * p.many_tiles * p.many_n;
         if (p.many_n > 1) {
             p.parts = (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW;
-            p.parts += (size_t)b->n_tokens * n_heads * p.many_n;
+            p.parts += ((size_t)b->n_tokens * n_heads * p.many_n + 1) & ~(size_t)1;
         }
     }
     return p;
+}
+
+// Partial rows, the log2 of their sums, and each unit's parts.
+size_t plan_bytes(const attn_plan &p, const wm_paged_kv *kv, const wm_paged_batch *b) {
+    return p.join ? p.parts * (kv->head_dim + 1) * sizeof(float) + (size_t)b->n_seqs * kv->n_kv_heads * sizeof(wm_u2) : 0;
 }
 
 }  // namespace
@@ -868,7 +901,7 @@ extern "C" {
 
 size_t wm_paged_attention_workspace(const wm_paged_kv *kv, const wm_paged_batch *batch, uint32_t n_heads) {
     if (!kv || !batch || !kv->n_kv_heads || n_heads % kv->n_kv_heads) return 0;
-    return make_plan(kv, batch, n_heads).parts * (kv->head_dim + 1) * sizeof(float);
+    return plan_bytes(make_plan(kv, batch, n_heads), kv, batch);
 }
 
 wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
@@ -893,7 +926,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if (p.few_blocks + p.many_blocks > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups in one step", who,
                             (unsigned long long)(p.few_blocks + p.many_blocks));
-    const size_t need = p.parts * (kv->head_dim + 1) * sizeof(float);
+    const size_t need = plan_bytes(p, kv, batch);
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
                             d_work ? work_bytes : (size_t)0, need);
@@ -909,7 +942,10 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.few_blocks = (uint32_t)p.few_blocks;
     a.many_tiles = p.many_tiles, a.many_len = p.many_len, a.many_n = p.many_n;
     a.part_o = (float *)d_work;
-    a.part_lse = a.part_o ? a.part_o + p.parts * kv->head_dim : nullptr;
+    if (p.join) {
+        a.part_lse = a.part_o + p.parts * kv->head_dim;
+        a.few_parts = (uint32_t *)(a.part_lse + p.parts);  // FEW rows to a part: an even count
+    }
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
     const uint32_t grid = (uint32_t)(p.few_blocks + p.many_blocks);
