@@ -28,6 +28,9 @@ __device__ __forceinline__ int quotient_code(float a, double inv) {
 __device__ __forceinline__ uint32_t pack_codes(int a, int b, int c, int d) {
     return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | (uint32_t)d << 24;
 }
+__device__ __forceinline__ uint32_t quotient4(wm_f4 v, double inv) {
+    return pack_codes(quotient_code(v.x, inv), quotient_code(v.y, inv), quotient_code(v.z, inv), quotient_code(v.w, inv));
+}
 __device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)(w << (24 - 8 * i)) >> 24; }
 // Earlier codes under a grown scale: c * s_old is exact in f32's products
 // only as f64 (7 + 24 bits), so the quotient is rounded the same way.
@@ -127,141 +130,193 @@ __device__ __forceinline__ block_place place_block(const wm_paged_kv &kv, const 
 // Append.  Bound by the bytes of q, k, v in and q out (the codes are a
 // quarter of f32's), and for a decode step by latency: the chain is lengths,
 // page id, old scale, and the earlier codes of a block are loaded with the
-// scale, before it is known whether they change.  Thread units: K (position,
-// 8 dims), V (4 positions, 4 dims) so that its transposed codes leave as
-// whole dwords.
+// scale, before it is known whether they change.  A block's keys, its values
+// and the queries of 16 of its positions are a workgroup each: one workgroup
+// for all three left 250 long ones in a step of 24 sequences in pages of 64
+// positions (21 us; three kinds: see below).
+
+// Queries of slots [first, hi) of 16: a thread has 8 dims of one position in
+// every head of the kv head's group, so the angles are loaded once.
+template <typename T, int D>
+__device__ __forceinline__ void append_queries(const append_args &a, const block_place &p, int base, int first, int hi,
+                                               int64_t tok) {
+    const int n_rot = (int)a.rope.n_rot, slot = (int)threadIdx.x / (D / 8), u = (int)threadIdx.x % (D / 8);
+    const bool half = a.rope.layout == WM_ROPE_HALF;
+    for (int t = first + slot; t < hi; t += NT / (D / 8)) {
+        const unit_dims d = dims_of(u, n_rot, half);
+        const T *row = (const T *)a.q + (uint64_t)(tok + t) * a.qs + (uint64_t)p.h * a.group * D;
+        T *out = (T *)a.q_out + (uint64_t)(tok + t) * a.qos + (uint64_t)p.h * a.group * D;
+        wm_f4 c = {1, 1, 1, 1}, s = {0, 0, 0, 0};
+        if (d.rot) {
+            const uint64_t at = (uint64_t)(base + t) * (n_rot / 2) + 4 * u;
+            c = *(const wm_f4 *)(a.rope.cos + at), s = *(const wm_f4 *)(a.rope.sin + at);
+        }
+        for (uint32_t g0 = 0; g0 < a.group; g0 += 4) {  // four heads' loads together
+            wm_f4 x[4], y[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint32_t h = min(g0 + g, a.group - 1) * D;
+                x[g] = wm_ld4(row + h + d.a), y[g] = wm_ld4(row + h + d.b);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                if (g0 + g >= a.group) break;
+                if (d.rot) rotate_unit(x[g], y[g], c, s, half);
+                wm_st4(out + (g0 + g) * D + d.a, x[g]);
+                wm_st4(out + (g0 + g) * D + d.b, y[g]);
+            }
+        }
+    }
+}
+
+// The block's new scale from its new values' maximum and its old scale, and
+// what quotients by it need.
+struct block_scale {
+    float s;
+    double inv, ratio;
+    bool grew;
+    __device__ __forceinline__ block_scale(float most, float old, float *red) {
+        most = wm_wave_max_nonneg(most);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NT / 64; w++) most = fmaxf(most, red[w]);
+        s = fmaxf(old, (float)((double)most / 127.0));
+        inv = s > 0.0f ? 1.0 / (double)s : 0.0;
+        ratio = (double)old * inv;
+        grew = s > old;
+    }
+};
+
+// Keys: a thread's units are 8 dims of one position.
 template <typename T, int PS, int D>
-__global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
-    constexpr int NK = (PS * D / 8 + NT - 1) / NT;   // K units per thread
-    constexpr int NV = (PS * D / 16 + NT - 1) / NT;  // V units per thread
-    __shared__ float red[2][NT / 64];
-    const block_place p = place_block(a.kv, a.b, a.touch, blockIdx.x);
-    if (!p.live) return;
+__device__ __forceinline__ void append_keys(const append_args &a, const block_place &p, int base, int first, int hi,
+                                            int64_t tok, uint64_t blk, float *red) {
+    constexpr int N = (PS * D / 8 + NT - 1) / NT;
     const int tid = threadIdx.x, n_rot = (int)a.rope.n_rot;
     const bool half = a.rope.layout == WM_ROPE_HALF;
-    const int base = p.lp * PS;  // first position of the page
-    const int lo = max(p.q.start, 0) - base, hi = min(p.q.len - base, PS);  // its new slots: [max(lo, 0), hi)
-    const int first = max(lo, 0);
-    const int64_t tok = (int64_t)p.q.tok0 + base - p.q.start;  // packed token of slot 0
-    const uint64_t blk = (uint64_t)(p.stored ? p.page : 0) * a.kv.n_kv_heads + p.h;
-    int8_t *kc = a.kv.k_codes + blk * (PS * D), *vc = a.kv.v_codes + blk * (PS * D);
-    const T *k = (const T *)a.k + (uint64_t)p.h * D, *v = (const T *)a.v + (uint64_t)p.h * D;
-    float sk_old = 0.0f, sv_old = 0.0f;
-    if (first > 0 && p.stored) sk_old = a.kv.k_scales[blk], sv_old = a.kv.v_scales[blk];
-
-    wm_f4 ka[NK], kb[NK];
-    uint32_t oa[NK], ob[NK];
-    float mk = 0.0f, mv = 0.0f;
+    int8_t *codes = a.kv.k_codes + blk * (PS * D);
+    const float old = first > 0 ? a.kv.k_scales[blk] : 0.0f;
+    const T *k = (const T *)a.k + (uint64_t)p.h * D;
+    wm_f4 x[N], y[N], c[N], s[N];
+    uint32_t ox[N], oy[N];
 #pragma unroll
-    for (int i = 0; i < NK; i++) {
-        const int unit = tid + i * NT, slot = unit / (D / 8);
-        const unit_dims d = dims_of(unit % (D / 8), n_rot, half);
-        ka[i] = kb[i] = wm_f4{0, 0, 0, 0};
-        oa[i] = ob[i] = 0;
-        if (unit >= PS * D / 8) continue;
-        if (slot >= first && slot < hi) {
+    for (int i = 0; i < N; i++) {
+        const int unit = tid + i * NT, slot = unit / (D / 8), u = unit % (D / 8);
+        const unit_dims d = dims_of(u, n_rot, half);
+        x[i] = y[i] = wm_f4{0, 0, 0, 0};
+        c[i] = s[i] = wm_f4{0, 0, 0, 0};
+        ox[i] = oy[i] = 0;
+        if (slot >= hi) continue;
+        if (slot >= first) {
             const T *row = k + (uint64_t)(tok + slot) * a.ks;
-            ka[i] = wm_ld4(row + d.a);
-            kb[i] = wm_ld4(row + d.b);
-        } else if (slot < first && p.stored) {
-            oa[i] = *(const uint32_t *)(kc + slot * D + d.a);
-            ob[i] = *(const uint32_t *)(kc + slot * D + d.b);
-        }
-    }
-    wm_f4 vv[NV][4];
-    uint32_t ov[NV][4];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
-#pragma unroll
-        for (int j = 0; j < 4; j++) vv[i][j] = wm_f4{0, 0, 0, 0}, ov[i][j] = 0;
-        if (unit >= PS * D / 16 || quad >= hi) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (quad + j >= first && quad + j < hi) vv[i][j] = wm_ld4(v + (uint64_t)(tok + quad + j) * a.vs + dim);
-        if ((quad < first || quad + 4 > hi) && p.stored) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) ov[i][j] = *(const uint32_t *)(vc + (dim + j) * PS + quad);
-        }
-    }
-    if (a.group) {
-        const int n_units = (hi - first) * (int)a.group * (D / 8);
-        for (int w = tid; w < n_units; w += NT) {
-            const int u = w % (D / 8), hg = w / (D / 8), slot = first + hg / (int)a.group;
-            const uint64_t head = (uint64_t)p.h * a.group + hg % a.group;
-            const unit_dims d = dims_of(u, n_rot, half);
-            const T *row = (const T *)a.q + (uint64_t)(tok + slot) * a.qs + head * D;
-            T *out = (T *)a.q_out + (uint64_t)(tok + slot) * a.qos + head * D;
-            wm_f4 x = wm_ld4(row + d.a), y = wm_ld4(row + d.b);
+            x[i] = wm_ld4(row + d.a), y[i] = wm_ld4(row + d.b);
             if (d.rot) {
                 const uint64_t at = (uint64_t)(base + slot) * (n_rot / 2) + 4 * u;
-                rotate_unit(x, y, *(const wm_f4 *)(a.rope.cos + at), *(const wm_f4 *)(a.rope.sin + at), half);
+                c[i] = *(const wm_f4 *)(a.rope.cos + at), s[i] = *(const wm_f4 *)(a.rope.sin + at);
             }
-            wm_st4(out + d.a, x);
-            wm_st4(out + d.b, y);
+        } else {
+            ox[i] = *(const uint32_t *)(codes + slot * D + d.a);
+            oy[i] = *(const uint32_t *)(codes + slot * D + d.b);
         }
     }
-    if (!p.stored) return;
+    float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NK; i++) {
-        const int unit = tid + i * NT, slot = unit / (D / 8), u = unit % (D / 8);
-        if (unit < PS * D / 8 && slot >= first && slot < hi) {
-            if (8 * u < n_rot) {
-                const uint64_t at = (uint64_t)(base + slot) * (n_rot / 2) + 4 * u;
-                rotate_unit(ka[i], kb[i], *(const wm_f4 *)(a.rope.cos + at), *(const wm_f4 *)(a.rope.sin + at), half);
-            }
-            mk = fmaxf(mk, fmaxf(finite_abs4(ka[i]), finite_abs4(kb[i])));
-        }
+    for (int i = 0; i < N; i++) {
+        const int u = (tid + i * NT) % (D / 8);
+        if (8 * u < n_rot) rotate_unit(x[i], y[i], c[i], s[i], half);
+        most = fmaxf(most, fmaxf(finite_abs4(x[i]), finite_abs4(y[i])));
     }
+    const block_scale b(most, old, red);
 #pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) mv = fmaxf(mv, finite_abs4(vv[i][j]));
-    mk = wm_wave_max_nonneg(mk);
-    mv = wm_wave_max_nonneg(mv);
-    if ((tid & 63) == 0) red[0][tid >> 6] = mk, red[1][tid >> 6] = mv;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; w++) mk = fmaxf(mk, red[0][w]), mv = fmaxf(mv, red[1][w]);
-    const float sk = fmaxf(sk_old, (float)((double)mk / 127.0)), sv = fmaxf(sv_old, (float)((double)mv / 127.0));
-    const double ik = sk > 0.0f ? 1.0 / (double)sk : 0.0, iv = sv > 0.0f ? 1.0 / (double)sv : 0.0;
-    const bool grew_k = sk > sk_old && first > 0, grew_v = sv > sv_old && first > 0;
-    const double rk = (double)sk_old * ik, rv = (double)sv_old * iv;
-#pragma unroll
-    for (int i = 0; i < NK; i++) {
+    for (int i = 0; i < N; i++) {
         const int unit = tid + i * NT, slot = unit / (D / 8);
         const unit_dims d = dims_of(unit % (D / 8), n_rot, half);
-        if (unit >= PS * D / 8) continue;
-        uint32_t *wa = (uint32_t *)(kc + slot * D + d.a), *wb = (uint32_t *)(kc + slot * D + d.b);
-        if (slot >= first && slot < hi) {
-            *wa = pack_codes(quotient_code(ka[i].x, ik), quotient_code(ka[i].y, ik), quotient_code(ka[i].z, ik),
-                             quotient_code(ka[i].w, ik));
-            *wb = pack_codes(quotient_code(kb[i].x, ik), quotient_code(kb[i].y, ik), quotient_code(kb[i].z, ik),
-                             quotient_code(kb[i].w, ik));
-        } else if (slot < first && grew_k) {
-            *wa = rescale4(oa[i], rk);
-            *wb = rescale4(ob[i], rk);
+        uint32_t *wx = (uint32_t *)(codes + slot * D + d.a), *wy = (uint32_t *)(codes + slot * D + d.b);
+        if (slot >= hi) continue;
+        if (slot >= first) {
+            *wx = quotient4(x[i], b.inv);
+            *wy = quotient4(y[i], b.inv);
+        } else if (b.grew) {
+            *wx = rescale4(ox[i], b.ratio);
+            *wy = rescale4(oy[i], b.ratio);
+        }
+    }
+    if (tid == 0) a.kv.k_scales[blk] = b.s;
+}
+
+// Values: a thread's units are 4 positions x 4 dims, so that the transposed
+// codes leave as whole dwords.
+template <typename T, int PS, int D>
+__device__ __forceinline__ void append_values(const append_args &a, const block_place &p, int first, int hi, int64_t tok,
+                                              uint64_t blk, float *red) {
+    constexpr int N = (PS * D / 16 + NT - 1) / NT;
+    const int tid = threadIdx.x;
+    int8_t *codes = a.kv.v_codes + blk * (PS * D);
+    const float old = first > 0 ? a.kv.v_scales[blk] : 0.0f;
+    const T *v = (const T *)a.v + (uint64_t)p.h * D;
+    wm_f4 x[N][4];
+    uint32_t o[N][4];
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[i][j] = wm_f4{0, 0, 0, 0}, o[i][j] = 0;
+        if (quad >= hi) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (quad + j >= first && quad + j < hi) x[i][j] = wm_ld4(v + (uint64_t)(tok + quad + j) * a.vs + dim);
+        if (quad < first || quad + 4 > hi) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][j] = *(const uint32_t *)(codes + (dim + j) * PS + quad);
         }
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) most = fmaxf(most, finite_abs4(x[i][j]));
+    const block_scale b(most, old, red);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
         const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
-        if (unit >= PS * D / 16 || quad >= hi || (quad + 4 <= first && !grew_v)) continue;
+        if (quad >= hi || (quad + 4 <= first && !b.grew)) continue;
 #pragma unroll
         for (int j = 0; j < 4; j++) {  // dim + j of four positions
-            const uint32_t old = ov[i][j], kept = grew_v ? rescale4(old, rv) : old;
+            const uint32_t kept = b.grew ? rescale4(o[i][j], b.ratio) : o[i][j];
             uint32_t w = 0;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 const uint32_t mask = 255u << (8 * t);
                 const int slot = quad + t;
-                const uint32_t fresh = (uint32_t)(quotient_code(vv[i][t][j], iv) & 255) << (8 * t);
-                w |= slot < first ? kept & mask : slot < hi ? fresh : old & mask;
+                const uint32_t fresh = (uint32_t)(quotient_code(x[i][t][j], b.inv) & 255) << (8 * t);
+                w |= slot < first ? kept & mask : slot < hi ? fresh : o[i][j] & mask;
             }
-            *(uint32_t *)(vc + (dim + j) * PS + quad) = w;
+            *(uint32_t *)(codes + (dim + j) * PS + quad) = w;
         }
     }
-    if (tid == 0) a.kv.k_scales[blk] = sk, a.kv.v_scales[blk] = sv;
+    if (tid == 0) a.kv.v_scales[blk] = b.s;
+}
+
+template <typename T, int PS, int D>
+__global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
+    static_assert(PS * D % (16 * NT) == 0 || PS * D < 16 * NT, "whole units per thread");
+    __shared__ float red[NT / 64];
+    const uint32_t kinds = a.group ? 2 + PS / 16 : 2, kind = blockIdx.x % kinds;
+    const block_place p = place_block(a.kv, a.b, a.touch, blockIdx.x / kinds);
+    if (!p.live) return;
+    const int base = p.lp * PS;  // first position of the page
+    const int first = max(max(p.q.start, 0) - base, 0), hi = min(p.q.len - base, PS);  // its new slots
+    const int64_t tok = (int64_t)p.q.tok0 + base - p.q.start;  // packed token of slot 0
+    if (kind >= 2) {
+        const int s0 = 16 * (int)(kind - 2);
+        append_queries<T, D>(a, p, base, max(first, s0), min(hi, s0 + 16), tok);
+        return;
+    }
+    if (!p.stored) return;
+    const uint64_t blk = (uint64_t)p.page * a.kv.n_kv_heads + p.h;
+    if (kind == 0) append_keys<T, PS, D>(a, p, base, first, hi, tok, blk, red);
+    else append_values<T, PS, D>(a, p, first, hi, tok, blk, red);
 }
 
 struct read_args {
@@ -317,7 +372,7 @@ uint32_t touched_pages(const wm_paged_kv *kv, const wm_paged_batch *b) {
 }
 wm_status block_grid(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t *grid) {
     const uint64_t n = (uint64_t)touched_pages(kv, b) * b->n_seqs * kv->n_kv_heads;
-    if (n > 0x7FFFFFFFull / NT)  // the launch counts threads in 32 bits
+    if (n > 0x7FFFFFFFull / NT / 6)  // the launch counts threads in 32 bits, and an append has up to six workgroups a block
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu blocks in one step", who, (unsigned long long)n);
     *grid = (uint32_t)n;
     return WM_OK;
@@ -325,7 +380,7 @@ wm_status block_grid(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const 
 
 template <typename T, int PS, int D> struct launch_append {
     static void go(const append_args &a, uint32_t grid, hipStream_t s) {
-        k_paged_append<T, PS, D><<<grid, NT, 0, s>>>(a);
+        k_paged_append<T, PS, D><<<grid * (a.group ? 2 + PS / 16 : 2), NT, 0, s>>>(a);
     }
 };
 template <typename T, int PS, int D> struct launch_read {
