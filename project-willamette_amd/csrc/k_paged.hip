@@ -112,7 +112,9 @@ struct append_args {
 struct block_place {
     wm_seq q;
     int lp, h, page;
-    bool live, stored;  // positions of the step lie in it; its page is in the pool
+    uint32_t n_pages;
+    bool live;  // positions of the step lie in it
+    __device__ __forceinline__ bool stored() const { return (uint32_t)page < n_pages; }  // its page is in the pool
 };
 __device__ __forceinline__ block_place place_block(const wm_paged_kv &kv, const wm_paged_batch &b, uint32_t touch,
                                                    uint32_t id) {
@@ -123,7 +125,7 @@ __device__ __forceinline__ block_place place_block(const wm_paged_kv &kv, const 
     p.lp = max(p.q.start, 0) / (int)kv.page_size + (int)(sm % touch);
     p.live = p.q.ok && p.q.n > 0 && (int64_t)p.lp * kv.page_size < p.q.len;
     p.page = p.live ? b.page_table[(uint64_t)s * b.table_stride + p.lp] : -1;
-    p.stored = p.page >= 0 && (uint32_t)p.page < kv.n_pages;
+    p.n_pages = kv.n_pages;
     return p;
 }
 
@@ -191,31 +193,39 @@ struct block_scale {
 // Keys: a thread's units are 8 dims of one position.
 template <typename T, int PS, int D>
 __device__ __forceinline__ void append_keys(const append_args &a, const block_place &p, int base, int first, int hi,
-                                            int64_t tok, uint64_t blk, float *red) {
+                                            int64_t tok, float *red) {
     constexpr int N = (PS * D / 8 + NT - 1) / NT;
     const int tid = threadIdx.x, n_rot = (int)a.rope.n_rot;
     const bool half = a.rope.layout == WM_ROPE_HALF;
-    int8_t *codes = a.kv.k_codes + blk * (PS * D);
-    const float old = first > 0 ? a.kv.k_scales[blk] : 0.0f;
     const T *k = (const T *)a.k + (uint64_t)p.h * D;
     wm_f4 x[N], y[N], c[N], s[N];
     uint32_t ox[N], oy[N];
+    // the new keys' loads go out before the page's id is here
 #pragma unroll
     for (int i = 0; i < N; i++) {
         const int unit = tid + i * NT, slot = unit / (D / 8), u = unit % (D / 8);
         const unit_dims d = dims_of(u, n_rot, half);
         x[i] = y[i] = wm_f4{0, 0, 0, 0};
         c[i] = s[i] = wm_f4{0, 0, 0, 0};
-        ox[i] = oy[i] = 0;
-        if (slot >= hi) continue;
-        if (slot >= first) {
+        if (slot >= first && slot < hi) {
             const T *row = k + (uint64_t)(tok + slot) * a.ks;
             x[i] = wm_ld4(row + d.a), y[i] = wm_ld4(row + d.b);
             if (d.rot) {
                 const uint64_t at = (uint64_t)(base + slot) * (n_rot / 2) + 4 * u;
                 c[i] = *(const wm_f4 *)(a.rope.cos + at), s[i] = *(const wm_f4 *)(a.rope.sin + at);
             }
-        } else {
+        }
+    }
+    if (!p.stored()) return;
+    const uint64_t blk = (uint64_t)p.page * a.kv.n_kv_heads + p.h;
+    int8_t *codes = a.kv.k_codes + blk * (PS * D);
+    const float old = first > 0 ? a.kv.k_scales[blk] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int unit = tid + i * NT, slot = unit / (D / 8);
+        const unit_dims d = dims_of(unit % (D / 8), n_rot, half);
+        ox[i] = oy[i] = 0;
+        if (slot < first) {
             ox[i] = *(const uint32_t *)(codes + slot * D + d.a);
             oy[i] = *(const uint32_t *)(codes + slot * D + d.b);
         }
@@ -249,11 +259,9 @@ __device__ __forceinline__ void append_keys(const append_args &a, const block_pl
 // codes leave as whole dwords.
 template <typename T, int PS, int D>
 __device__ __forceinline__ void append_values(const append_args &a, const block_place &p, int first, int hi, int64_t tok,
-                                              uint64_t blk, float *red) {
+                                              float *red) {
     constexpr int N = (PS * D / 16 + NT - 1) / NT;
     const int tid = threadIdx.x;
-    int8_t *codes = a.kv.v_codes + blk * (PS * D);
-    const float old = first > 0 ? a.kv.v_scales[blk] : 0.0f;
     const T *v = (const T *)a.v + (uint64_t)p.h * D;
     wm_f4 x[N][4];
     uint32_t o[N][4];
@@ -262,15 +270,21 @@ __device__ __forceinline__ void append_values(const append_args &a, const block_
     for (int i = 0; i < N; i++) {
         const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[i][j] = wm_f4{0, 0, 0, 0}, o[i][j] = 0;
-        if (quad >= hi) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int j = 0; j < 4; j++) {
+            x[i][j] = wm_f4{0, 0, 0, 0};
             if (quad + j >= first && quad + j < hi) x[i][j] = wm_ld4(v + (uint64_t)(tok + quad + j) * a.vs + dim);
-        if (quad < first || quad + 4 > hi) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[i][j] = *(const uint32_t *)(codes + (dim + j) * PS + quad);
         }
+    }
+    if (!p.stored()) return;
+    const uint64_t blk = (uint64_t)p.page * a.kv.n_kv_heads + p.h;
+    int8_t *codes = a.kv.v_codes + blk * (PS * D);
+    const float old = first > 0 ? a.kv.v_scales[blk] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int unit = tid + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
+        const bool part = quad < hi && (quad < first || quad + 4 > hi);  // earlier positions, or none yet
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[i][j] = part ? *(const uint32_t *)(codes + (dim + j) * PS + quad) : 0;
     }
 #pragma unroll
     for (int i = 0; i < N; i++)
@@ -313,10 +327,8 @@ __global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
         append_queries<T, D>(a, p, base, max(first, s0), min(hi, s0 + 16), tok);
         return;
     }
-    if (!p.stored) return;
-    const uint64_t blk = (uint64_t)p.page * a.kv.n_kv_heads + p.h;
-    if (kind == 0) append_keys<T, PS, D>(a, p, base, first, hi, tok, blk, red);
-    else append_values<T, PS, D>(a, p, first, hi, tok, blk, red);
+    if (kind == 0) append_keys<T, PS, D>(a, p, base, first, hi, tok, red);
+    else append_values<T, PS, D>(a, p, first, hi, tok, red);
 }
 
 struct read_args {
@@ -339,10 +351,11 @@ __global__ __launch_bounds__(NT) void k_paged_read(read_args a) {
     if (!p.live) return;
     const int base = p.lp * PS, first = max(max(p.q.start, 0) - base, 0), hi = min(p.q.len - base, PS);
     const int64_t tok = (int64_t)p.q.tok0 + base - p.q.start;
-    const uint64_t blk = (uint64_t)(p.stored ? p.page : 0) * a.kv.n_kv_heads + p.h;
+    const bool stored = p.stored();
+    const uint64_t blk = (uint64_t)(stored ? p.page : 0) * a.kv.n_kv_heads + p.h;
     const int8_t *kc = a.kv.k_codes + blk * (PS * D), *vc = a.kv.v_codes + blk * (PS * D);
     const float nan = __uint_as_float(0x7FC00000u);
-    const float sk = p.stored ? a.kv.k_scales[blk] : nan, sv = p.stored ? a.kv.v_scales[blk] : nan;
+    const float sk = stored ? a.kv.k_scales[blk] : nan, sv = stored ? a.kv.v_scales[blk] : nan;
     for (int unit = threadIdx.x; unit < PS * D / 16; unit += NT) {
         const int quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
         if (quad + 4 <= first || quad >= hi) continue;
