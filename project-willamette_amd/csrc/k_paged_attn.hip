@@ -44,9 +44,10 @@ struct attn_args {
     int type;
     float scale_log2;  // scale * log2 e
     // Sequences of few rows: few_blocks workgroups share all their positions
-    // evenly (few_share).  Those of many: many_n workgroups of many_len
-    // positions each per row tile, many_tiles row tiles of MANY at most.
-    uint32_t few_blocks, many_tiles, many_len, many_n;
+    // evenly (few_share).  Those of many: up to many_n workgroups of many_len
+    // positions each per row tile, many_levels row tiles and contexts of as
+    // many tokens at most (many_order).
+    uint32_t few_blocks, many_levels, many_len, many_n;
     // partial rows: FEW of each few_share::slot, then [token][head][many_n]
     float *part_o, *part_lse;
     // of each (sequence of few rows, kv head): the first workgroup that has a part of it, and how many have
@@ -544,6 +545,68 @@ __global__ __launch_bounds__(NT, 2) void k_paged_attn_few(attn_args a) {
     attend_few<D, TERMS>(a, blockIdx.x, sh);
 }
 
+// The order of the row tiles of sequences of many rows: those with the most
+// positions first, so that the last workgroups to start are short, and only
+// tiles that exist, so that the compute dies take equal shares (workgroup i
+// runs on die i % 8; with every sequence's tiles up to the longest one's in
+// the grid, one die had nine times another's work).  A tile's level is its
+// number in the sequence plus the context's length in tiles; the tiles at
+// level l or above are counted by a scan over the sequences, and a bisection
+// finds the level of the y-th.
+struct many_order {
+    wm_seq q;  // the first 64 sequences, one to a lane
+    uint32_t low = 0, tiles = 0;
+    __device__ __forceinline__ void load(const attn_args &a, uint32_t s0) {
+        const uint32_t s = s0 + (threadIdx.x & 63);
+        q = wm_load_seq(a.b, min(s, a.b.n_seqs - 1));
+        const int64_t rows = (int64_t)q.n * a.group;
+        const bool many = s < a.b.n_seqs && q.ok && rows > FEW;
+        tiles = many ? (uint32_t)(rows + MANY - 1) / MANY : 0;
+        low = many ? (uint32_t)((int64_t)max(q.start, 0) * a.group / MANY) : 0;
+    }
+    __device__ __forceinline__ uint32_t from_level(uint32_t l) const {
+        return wm_wave_total_i32(min(low + tiles > l ? low + tiles - l : 0, tiles));
+    }
+    // Tile y: its sequence and row tile; false past the last.
+    __device__ __forceinline__ bool find(const attn_args &a, uint32_t y, wm_seq &seq, uint32_t &s, uint32_t &rt) {
+        const bool one = a.b.n_seqs <= 64;
+        auto count = [&](uint32_t l) {
+            uint32_t n = 0;
+            for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
+                if (!one) load(a, s0);
+                n += from_level(l);
+            }
+            return n;
+        };
+        if (one) load(a, 0);
+        if (y >= count(0)) return false;
+        uint32_t l = 0, above = a.many_levels;  // count(l) > y >= count(above)
+        while (above - l > 1) {
+            const uint32_t mid = (l + above) / 2;
+            if (count(mid) > y) l = mid;
+            else above = mid;
+        }
+        uint32_t left = y - count(l + 1);  // among the tiles of level l, one of a sequence at most
+        for (uint32_t s0 = 0;; s0 += 64) {
+            if (!one) load(a, s0);
+            const bool has = low <= l && l < low + tiles;
+            const uint64_t mask = __ballot(has);
+            const uint32_t n = __popcll(mask);
+            if (left < n) {
+                const uint64_t hit = __ballot(has && __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                                                              __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0)) == left);
+                const int lane = __builtin_ctzll(hit);
+                s = s0 + lane, rt = l - __builtin_amdgcn_readlane(low, lane);
+                seq.tok0 = __builtin_amdgcn_readlane(q.tok0, lane), seq.n = __builtin_amdgcn_readlane(q.n, lane);
+                seq.start = __builtin_amdgcn_readlane(q.start, lane), seq.len = __builtin_amdgcn_readlane(q.len, lane);
+                seq.ok = true;
+                return true;
+            }
+            left -= n;
+        }
+    }
+};
+
 // Many rows.  One workgroup: 128 rows of one sequence and kv head, 32 to a
 // wave, one split of the positions (all of them where there are workgroups
 // enough).  Its four waves share each tile of 64 positions: converted once to
@@ -561,12 +624,13 @@ struct alignas(16) many_shared {
 template <int D, int TERMS>
 __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, many_shared<D> &sh) {
     constexpr int KS = D / 16, DT = D / 32, U = D / 64;  // units of 16 codes per thread, of K and of V
-    // the longest row tiles first: theirs are the last rows of the sequences
-    const uint32_t split = id % a.many_n;
-    id /= a.many_n;
-    const uint32_t unit = id % (a.b.n_seqs * a.kv.n_kv_heads), rt = a.many_tiles - 1 - id / (a.b.n_seqs * a.kv.n_kv_heads);
-    const row_tile t = load_tile(a, unit / a.kv.n_kv_heads, unit % a.kv.n_kv_heads, rt, MANY);
-    if (!t.q.ok || t.rows <= FEW || t.r0 >= t.rows) return;
+    const uint32_t part_id = id % a.many_n, tile_id = id / a.many_n;
+    wm_seq seq;
+    uint32_t s, rt;
+    if (!many_order().find(a, tile_id / a.kv.n_kv_heads, seq, s, rt)) return;
+    const row_tile t = make_tile(a, seq, s, tile_id % a.kv.n_kv_heads, rt, MANY);
+    // (a short tile's missing splits fall on every die)
+    const uint32_t split = (part_id + tile_id) % a.many_n;
     const int p0 = (int)(split * a.many_len);
     if (split && p0 >= t.len) return;
     const int p1 = (int)min((int64_t)p0 + a.many_len, (int64_t)t.len);
@@ -856,7 +920,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
 // How a step is divided: from the host's bounds alone.
 struct attn_plan {
     bool many;         // a sequence may have more than FEW rows
-    uint32_t many_tiles, many_len, many_n;
+    uint32_t many_tiles, many_levels, many_len, many_n;
     uint64_t few_blocks, many_blocks;
     bool join;
     size_t parts;      // partial rows
@@ -871,7 +935,7 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
     p.parts = rounds > 1 ? (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW : 0;
     p.join = rounds > 1;
     p.rounds = units * rounds;
-    p.many_tiles = 0, p.many_blocks = 0, p.many_len = 0, p.many_n = 1;
+    p.many_tiles = 0, p.many_levels = 0, p.many_blocks = 0, p.many_len = 0, p.many_n = 1;
     if (p.many) {
         p.many_tiles = (uint32_t)((rows + MANY - 1) / MANY);
         // as many row tiles as the packed tokens can fill, not as many as the longest would in every sequence
@@ -881,7 +945,8 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
         const uint32_t per = want < rounds ? (uint32_t)(rounds / want) : 1;
         p.many_len = per * ROUND;
         p.many_n = (rounds + per - 1) / per;
-        p.many_blocks = units * p.many_tiles * p.many_n;
+        p.many_blocks = tiles * kv->n_kv_heads * p.many_n;
+        p.many_levels = p.many_tiles + (uint32_t)((uint64_t)b->max_kv_len * (n_heads / kv->n_kv_heads) / MANY) + 1;
         if (p.many_n > 1) {
             p.parts = (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW;
             p.parts += ((size_t)b->n_tokens * n_heads * p.many_n + 1) & ~(size_t)1;
@@ -920,8 +985,10 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
     if ((st = wm_paged_check_array(ctx, who, "out", d_out, out_stride, n_heads, kv->head_dim, elem))) return st;
     if ((uintptr_t)d_lse % 4) return wm_set_error(ctx, WM_E_ARG, "%s: misaligned lse", who);
-    if ((uint64_t)batch->max_new * (n_heads / kv->n_kv_heads) > 1u << 30)
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: %u tokens of %u heads in one sequence", who, batch->max_new, n_heads);
+    if ((uint64_t)(batch->max_new > batch->max_kv_len ? batch->max_new : batch->max_kv_len) * (n_heads / kv->n_kv_heads) >
+        1u << 30)
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: max_new %u or max_kv_len %u is too large for %u heads over %u", who,
+                            batch->max_new, batch->max_kv_len, n_heads, kv->n_kv_heads);
     const attn_plan p = make_plan(kv, batch, n_heads);
     if (p.few_blocks + p.many_blocks > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups in one step", who,
@@ -940,7 +1007,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.type = type;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.few_blocks = (uint32_t)p.few_blocks;
-    a.many_tiles = p.many_tiles, a.many_len = p.many_len, a.many_n = p.many_n;
+    a.many_levels = p.many_levels, a.many_len = p.many_len, a.many_n = p.many_n;
     a.part_o = (float *)d_work;
     if (p.join) {
         a.part_lse = a.part_o + p.parts * kv->head_dim;
