@@ -45,8 +45,8 @@ struct attn_args {
     float scale_log2;  // scale * log2 e
     // Sequences of few rows: few_blocks workgroups share all their positions
     // evenly (few_share).  Those of many: up to many_n workgroups of many_len
-    // positions each per row tile, many_levels row tiles and contexts of as
-    // many tokens at most (many_order).
+    // positions each per row tile, many_levels row tiles of MANY and
+    // contexts of as many tokens at most (many_order).
     uint32_t few_blocks, many_levels, many_len, many_n;
     // partial rows: FEW of each few_share::slot, then [token][head][many_n]
     float *part_o, *part_lse;
@@ -219,7 +219,7 @@ struct scale_ref {
 struct row_max {
     float m = -INFINITY, l = 0.0f, from = 0.0f;
     __device__ __forceinline__ void begin(const scale_ref &r) {
-        if (r.down != 0.0f) m -= r.down, l *= __builtin_amdgcn_exp2f(r.down);
+        m -= r.down, l *= __builtin_amdgcn_exp2f(r.down);
         from = m == -INFINITY ? 0.0f : m;
     }
     // Every lane's scores have then to be lowered by `by`, O scaled by `alpha`.
@@ -561,7 +561,7 @@ struct many_order {
         q = wm_load_seq(a.b, min(s, a.b.n_seqs - 1));
         const int64_t rows = (int64_t)q.n * a.group;
         const bool many = s < a.b.n_seqs && q.ok && rows > FEW;
-        tiles = many ? (uint32_t)(rows + MANY - 1) / MANY : 0;
+        tiles = many ? (uint32_t)((rows + MANY - 1) / MANY) : 0;
         low = many ? (uint32_t)((int64_t)max(q.start, 0) * a.group / MANY) : 0;
     }
     __device__ __forceinline__ uint32_t from_level(uint32_t l) const {
@@ -607,47 +607,32 @@ struct many_order {
     }
 };
 
-// Many rows.  One workgroup: 128 rows of one sequence and kv head, 32 to a
-// wave, one split of the positions (all of them where there are workgroups
-// enough).  Its four waves share each tile of 64 positions: converted once to
-// f16 in LDS, K [position][dim], V [dim][position] with each 16 positions in
-// the order that a lane's half of the second product's K = 16 step takes
-// them (0-3, 8-11 | 4-7, 12-15), so both operands are 16-byte reads.  Rows are
-// padded by 16 bytes: 16 lanes' reads then fall into all 64 banks.  Two
-// buffers, one barrier per tile: the next tile's codes are loaded a tile
-// ahead and converted while the matrix cores work on this one.
-template <int D>
-struct alignas(16) many_shared {
-    _Float16 k[2][TILE][D + 8];
-    _Float16 v[2][D][TILE + 8];
-};
+// What a wave of a workgroup for many rows holds: 32 rows, their sums, and a
+// tile's scores on the way to weights.
 template <int D, int TERMS>
-__device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, many_shared<D> &sh) {
-    constexpr int KS = D / 16, DT = D / 32, U = D / 64;  // units of 16 codes per thread, of K and of V
-    const uint32_t part_id = id % a.many_n, tile_id = id / a.many_n;
-    wm_seq seq;
-    uint32_t s, rt;
-    if (!many_order().find(a, tile_id / a.kv.n_kv_heads, seq, s, rt)) return;
-    const row_tile t = make_tile(a, seq, s, tile_id % a.kv.n_kv_heads, rt, MANY);
-    // (a short tile's missing splits fall on every die)
-    const uint32_t split = (part_id + tile_id) % a.many_n;
-    const int p0 = (int)(split * a.many_len);
-    if (split && p0 >= t.len) return;
-    const int p1 = (int)min((int64_t)p0 + a.many_len, (int64_t)t.len);
-    const bool whole = t.len <= (int)a.many_len;
-
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 31, hi = lane >> 5;
-    // this wave's rows; positions that all of them, and that any, attend to
-    const int w0 = t.r0 + 32 * wave, at_row = w0 + n;
-    // (rows past the last repeat it, and are not written)
-    const bool valid = at_row < t.rows;
-    const int row = min(at_row, t.rows - 1), j = row / (int)a.group, count = t.q.start + j + 1;
-    const int all = t.q.start + w0 / (int)a.group + 1;
-    const int any = w0 < t.rows ? t.q.start + (min(w0 + 32, t.rows) - 1) / (int)a.group + 1 : 0;
-    const uint64_t tok = (uint64_t)(t.q.tok0 + j), head = (uint64_t)t.h * a.group + row - j * (int)a.group;
+struct wave_rows {
+    static constexpr int KS = D / 16, DT = D / 32;
+    int n, hi;            // the lane's row of the 32, and half
+    bool valid;           // (rows past the last repeat it, and are not written)
+    int count, all, any;  // positions that the row, all rows, and any row of the wave attend to
+    uint64_t tok, head;
     wm_h8 q[KS][TERMS];
     float kfac;
-    {
+    wm_f16v o[DT];
+    row_max sums;
+    scale_ref ref;
+    // a tile's scales: of the lane's group of 16 positions (lane % 4)
+    float ks, part, back;
+
+    __device__ __forceinline__ void begin(const attn_args &a, const row_tile &t, int w0) {
+        const int lane = threadIdx.x & 63;
+        n = lane & 31, hi = lane >> 5;
+        valid = w0 + n < t.rows;
+        const int row = min(w0 + n, t.rows - 1), j = row / (int)a.group;
+        count = t.q.start + j + 1;
+        all = t.q.start + w0 / (int)a.group + 1;
+        any = w0 < t.rows ? t.q.start + (min(w0 + 32, t.rows) - 1) / (int)a.group + 1 : 0;
+        tok = (uint64_t)(t.q.tok0 + j), head = (uint64_t)t.h * a.group + row - j * (int)a.group;
         float x[KS][8], m = 0.0f;
         const uint64_t at = tok * a.qs + head * D;
 #pragma unroll
@@ -660,185 +645,286 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
             }
         const int e = __builtin_amdgcn_frexp_expf(half_max(m));
         kfac = ldexpf(a.scale_log2, e - 15);
+        const float scale = ldexpf(1.0f, 15 - e);
 #pragma unroll
         for (int j = 0; j < KS; j++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 _Float16 h, lo;
-                to_terms<TERMS>(ldexpf(x[j][i], 15 - e), &h, &lo);
+                to_terms<TERMS>(x[j][i] * scale, &h, &lo);
                 q[j][0][i] = h;
                 if (TERMS > 1) q[j][TERMS - 1][i] = lo;
             }
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int c = 0; c < 16; c++) o[i][c] = 0.0f;
     }
-    wm_f16v o[DT];
-#pragma unroll
-    for (int i = 0; i < DT; i++)
-#pragma unroll
-        for (int c = 0; c < 16; c++) o[i][c] = 0.0f;
-    row_max sums;
-    scale_ref ref;
-
-    const uint32_t ps = a.kv.page_size, ps_log = 31 - __builtin_clz(ps);
-    const int32_t *table = a.b.page_table + (uint64_t)t.s * a.b.table_stride;
-    const uint64_t block = (uint64_t)ps * D;
-    // This thread's units: K's 16 dims (tid % (D / 16)) of one position each,
-    // V's 16 positions (group tid % 4) of one dim each.
-    const int kdim = tid % (D / 16) * 16, kpos = tid / (D / 16), vgrp = tid & 3, vdim = tid >> 2;
-    constexpr int KSTEP = NT / (D / 16), VSTEP = NT / 4;
-    int pk[U], pv;
-    auto load_pages = [&](int p) {
-        const int last = t.len - 1;
-#pragma unroll
-        for (int u = 0; u < U; u++) pk[u] = table[min(p + kpos + u * KSTEP, last) >> ps_log];
-        pv = table[min(p + 16 * vgrp, last) >> ps_log];
-    };
-    wm_u4 kr[U], vr[U];
-    float ks, vs;
-    auto load_codes = [&](int p) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const uint64_t pg = (uint32_t)pk[u] < a.kv.n_pages ? (uint32_t)pk[u] : 0;
-            kr[u] = *(const wm_u4 *)(a.kv.k_codes + (pg * a.kv.n_kv_heads + t.h) * block +
-                                     ((p + kpos + u * KSTEP) & (int)(ps - 1)) * D + kdim);
-        }
-        const bool good = (uint32_t)pv < a.kv.n_pages;
-        const uint64_t at = (good ? (uint64_t)(uint32_t)pv : 0) * a.kv.n_kv_heads + t.h;
-        const int8_t *src = a.kv.v_codes + at * block + ((p + 16 * vgrp) & (int)(ps - 1));
-#pragma unroll
-        for (int u = 0; u < U; u++) vr[u] = *(const wm_u4 *)(src + (uint64_t)(vdim + u * VSTEP) * ps);
-        ks = good ? a.kv.k_scales[at] : __uint_as_float(0x7FC00000u);
-        vs = good ? a.kv.v_scales[at] : 0.0f;
-    };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            wm_h8 c0, c1;
-            codes_to_f16(kr[u], c0, c1);
-            *(wm_h8 *)&sh.k[buf][kpos + u * KSTEP][kdim] = c0;
-            *(wm_h8 *)&sh.k[buf][kpos + u * KSTEP][kdim + 8] = c1;
-            codes_to_f16(wm_u4{vr[u].x, vr[u].z, vr[u].y, vr[u].w}, c0, c1);
-            *(wm_h8 *)&sh.v[buf][vdim + u * VSTEP][16 * vgrp] = c0;
-            *(wm_h8 *)&sh.v[buf][vdim + u * VSTEP][16 * vgrp + 8] = c1;
-        }
-    };
-    if (p0 < p1) {
-        load_pages(p0);
-        load_codes(p0);
-        load_pages(p0 + TILE);
-        stage(0);
-    }
-    int buf = 0;
-    for (int p = p0; p < p1; p += TILE, buf ^= 1) {
-        // of this tile's scales, before the next tile's are loaded: as for few
-        // rows, the lane's group of 16 positions
-        const int eb = vs != 0.0f ? __builtin_amdgcn_frexp_expf(vs) : E_NONE;
+    // The next tile's scales.
+    __device__ __forceinline__ void take_scales(const float (*scale)[2]) {
+        const float k = scale[threadIdx.x & 3][0], v = scale[threadIdx.x & 3][1];
+        const int eb = v != 0.0f ? __builtin_amdgcn_frexp_expf(v) : E_NONE;
         int e = max(eb, __builtin_amdgcn_mov_dpp(eb, 0xB1, 0xF, 0xF, true));  // over lanes l ^ 1, l ^ 2
         e = max(e, __builtin_amdgcn_mov_dpp(e, 0x4E, 0xF, 0xF, true));
         ref.raise(e);
-        const float my_ks = ks, my_part = ref.part(vs, eb), my_back = __builtin_amdgcn_exp2f(-my_part);
-        const bool more = p + TILE < p1;
-        if (more) {
-            load_codes(p + TILE);
-            load_pages(p + 2 * TILE);
-        }
-        __syncthreads();
-        const bool live = p < any;
-        wm_h8 w[4][TERMS];
+        ks = k, part = ref.part(v, eb), back = __builtin_amdgcn_exp2f(-part);
         sums.begin(ref);
         if (ref.excess)
 #pragma unroll
             for (int i = 0; i < DT; i++) o[i] *= ldexpf(1.0f, -ref.excess);
-        if (live) {
-            // scores relative to the maximum so far, the values' scale included
-            float x[4][8];
-            {
-                wm_f16v s[2];
+    }
+    // S^T = K Q^T of a tile in LDS.
+    __device__ __forceinline__ void scores(const _Float16 (*k)[D + 8], wm_f16v (&s)[2]) const {
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    s[i] = wm_f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        for (int i = 0; i < 2; i++) {
+            s[i] = wm_f16v{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < KS; j++) {
-                        const wm_h8 k = *(const wm_h8 *)&sh.k[buf][32 * i + n][16 * j + 8 * hi];
+            for (int j = 0; j < KS; j++) {
+                const wm_h8 x = *(const wm_h8 *)&k[32 * i + n][16 * j + 8 * hi];
 #pragma unroll
-                        for (int y = 0; y < TERMS; y++)
-                            s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[j][y], s[i], 0, 0, 0);
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const float f = kfac * read_lane(my_ks, g), c = read_lane(my_part, g) - sums.from;
-#pragma unroll
-                    for (int y = 0; y < 8; y++) x[g][y] = __builtin_fmaf(s[g / 2][8 * (g % 2) + y], f, c);
-                }
+                for (int y = 0; y < TERMS; y++) s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[j][y], s[i], 0, 0, 0);
             }
-            if (p + TILE > all) {
-                const int left = count - p - 4 * hi;
+        }
+    }
+    // Scores of the tile at p to weights, relative to the maximum so far, the
+    // values' scale included.
+    __device__ __forceinline__ void weights(const wm_f16v (&s)[2], int p, wm_h8 (&w)[4][TERMS]) {
+        float x[4][8];
 #pragma unroll
-                for (int g = 0; g < 4; g++)
+        for (int g = 0; g < 4; g++) {
+            const float f = kfac * read_lane(ks, g), c = read_lane(part, g) - sums.from;
 #pragma unroll
-                    for (int y = 0; y < 8; y++) x[g][y] = 16 * g + 8 * (y / 4) + y % 4 < left ? x[g][y] : -INFINITY;
-            }
-            float top = -INFINITY;
+            for (int y = 0; y < 8; y++) x[g][y] = __builtin_fmaf(s[g / 2][8 * (g % 2) + y], f, c);
+        }
+        if (p + TILE > all) {
+            const int left = count - p - 4 * hi;
 #pragma unroll
             for (int g = 0; g < 4; g++)
 #pragma unroll
-                for (int y = 0; y < 8; y++) top = fmaxf(top, x[g][y]);
-            float by, alpha;
-            if (sums.grows(half_max(top), by, alpha)) {
+                for (int y = 0; y < 8; y++) x[g][y] = 16 * g + 8 * (y / 4) + y % 4 < left ? x[g][y] : -INFINITY;
+        }
+        float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < DT; i++) o[i] *= alpha;
+        for (int g = 0; g < 4; g++)
 #pragma unroll
-                for (int g = 0; g < 4; g++)
+            for (int y = 0; y < 8; y++) top = fmaxf(top, x[g][y]);
+        float by, alpha;
+        if (sums.grows(half_max(top), by, alpha)) {
 #pragma unroll
-                    for (int y = 0; y < 8; y++) x[g][y] -= by;
+            for (int i = 0; i < DT; i++) o[i] *= alpha;
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int y = 0; y < 8; y++) x[g][y] -= by;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                const float e = __builtin_amdgcn_exp2f(x[g][y]);
+                sum += e;
+                _Float16 h, lo;
+                to_terms<TERMS>(e, &h, &lo);
+                w[g][0][y] = h;
+                if (TERMS > 1) w[g][TERMS - 1][y] = lo;
             }
+            sums.l = __builtin_fmaf(sum, read_lane(back, g), sums.l);
+        }
+    }
+    // O^T += V^T P^T of a tile in LDS.
+    __device__ __forceinline__ void values(const _Float16 (*v)[TILE + 8], const wm_h8 (&w)[4][TERMS]) {
+#pragma unroll
+        for (int i = 0; i < DT; i++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const float back = read_lane(my_back, g);
-                float sum = 0.0f;
+                const wm_h8 x = *(const wm_h8 *)&v[32 * i + n][16 * g + 8 * hi];
 #pragma unroll
-                for (int y = 0; y < 8; y++) {
-                    const float e = __builtin_amdgcn_exp2f(x[g][y]);
-                    sum += e;
-                    _Float16 h, lo;
-                    to_terms<TERMS>(e, &h, &lo);
-                    w[g][0][y] = h;
-                    if (TERMS > 1) w[g][TERMS - 1][y] = lo;
-                }
-                sums.l = __builtin_fmaf(sum, back, sums.l);
+                for (int y = 0; y < TERMS; y++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w[g][y], o[i], 0, 0, 0);
             }
+    }
+    __device__ __forceinline__ void write(const attn_args &a, bool whole, uint32_t split) const {
+        if (!valid) return;
+        const float sum = half_sum(sums.l), inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
+        const float lse2 = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
+        const uint64_t part_at = whole ? 0 : many_part(a, tok, head) + split;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int c = 0; c < 16; c += 4) {
+                wm_f4 v;
+#pragma unroll
+                for (int x = 0; x < 4; x++) v[x] = o[i][c + x] * inv;
+                const int d = 32 * i + 2 * c + 4 * hi;
+                if (whole) store_out4(a, tok * a.os + head * D + d, v);
+                else *(wm_f4 *)(a.part_o + part_at * D + d) = v;
+            }
+        if (hi == 0) {
+            if (!whole) a.part_lse[part_at] = lse2;
+            else if (a.lse) a.lse[tok * a.n_heads + head] = lse2 * 0.6931471805599453f;
         }
-        if (more) stage(buf ^ 1);
+    }
+};
+
+// A workgroup's row tile and split, of those that exist.
+struct many_work {
+    row_tile t;
+    uint32_t split;
+    int p0, p1;
+    bool whole;
+    __device__ __forceinline__ bool find(const attn_args &a, uint32_t id) {
+        const uint32_t part_id = id % a.many_n, tile_id = id / a.many_n;
+        wm_seq seq;
+        uint32_t s, rt;
+        if (!many_order().find(a, tile_id / a.kv.n_kv_heads, seq, s, rt)) return false;
+        t = make_tile(a, seq, s, tile_id % a.kv.n_kv_heads, rt, MANY);
+        split = (part_id + tile_id) % a.many_n;  // (a short tile's missing splits fall on every die)
+        p0 = (int)(split * a.many_len), p1 = (int)min((int64_t)p0 + a.many_len, (int64_t)t.len);
+        whole = t.len <= (int)a.many_len;
+        return split == 0 || p0 < t.len;
+    }
+};
+
+// A tile of 64 positions, converted once to f16 for all waves: K [position]
+// [dim], V [dim][position] with each 16 positions in the order that a lane's
+// half of the second product's K = 16 step takes them (0-3, 8-11 | 4-7,
+// 12-15), so both operands are 16-byte reads.  Rows are padded by 16 bytes:
+// 16 lanes' reads then fall into all 64 banks.
+template <int D>
+struct alignas(16) shared_tile {
+    _Float16 k[TILE][D + 8];
+    _Float16 v[D][TILE + 8];
+    float scale[4][2];  // of each 16 positions, K's and V's
+};
+
+// One wave's share in making tiles, a quarter of K's codes or of V's: wave w
+// of four takes what lies in the page of the tile's positions 16 w .. + 15,
+// so that a page is one scalar and a lane's addresses are a scalar base and
+// offsets that stay.  K: those 16 positions.  V: of a page of 16 n positions
+// that n waves share, the D / n dims that are its turn's, all positions.
+template <int D>
+struct stager {
+    static constexpr int U = D / 64;  // 16-byte units per lane
+    const int8_t *codes;
+    uint64_t block;
+    uint32_t off[U], lds[U];
+    bool is_v;
+    wm_u4 raw[U];
+    __device__ __forceinline__ void begin(const attn_args &a, uint32_t h, int w, bool v) {
+        const int ps = (int)a.kv.page_size, ng = ps / 16, lane = threadIdx.x & 63, sub = w & (ng - 1);
+        block = (uint64_t)ps * D;
+        codes = (v ? a.kv.v_codes : a.kv.k_codes) + h * block;
+        block *= a.kv.n_kv_heads;
+        is_v = v;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int x = lane + 64 * u;
+            const int pos = x / (D / 16), kdim = x % (D / 16) * 16;
+            const int grp = x & (ng - 1), dim = (sub * D + x) / ng;
+            off[u] = v ? dim * ps + 16 * grp : (16 * sub + pos) * D + kdim;
+            lds[u] = v ? (uint32_t)offsetof(shared_tile<D>, v) + (dim * (TILE + 8) + 16 * (w - sub + grp)) * 2
+                       : ((16 * w + pos) * (D + 8) + kdim) * 2;
+        }
+    }
+    __device__ __forceinline__ void load(uint32_t page) {
+        const int8_t *base = codes + page * block;
+#pragma unroll
+        for (int u = 0; u < U; u++) raw[u] = *(const wm_u4 *)(base + off[u]);
+    }
+    __device__ __forceinline__ void put(shared_tile<D> *tile) const {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            wm_h8 c0, c1;
+            // (V's 16 positions in a half's order)
+            codes_to_f16(wm_u4{raw[u].x, is_v ? raw[u].z : raw[u].y, is_v ? raw[u].y : raw[u].z, raw[u].w}, c0, c1);
+            char *to = (char *)tile + lds[u];
+            *(wm_h8 *)to = c0;
+            *(wm_h8 *)(to + 16) = c1;
+        }
+    }
+};
+// The page of a wave's 16 positions, tile after tile, loaded a turn ahead of
+// its use, and the block's two scales (lane 0 K's, lane 1 V's).
+struct page_walk {
+    const int32_t *table;
+    const float *scales;
+    uint32_t n_pages, n_kv, ps_log;
+    int last, ahead;
+    uint32_t page;  // of the tile last turned to: within the pool
+    bool good;      // as the table has it
+    float scale;
+    __device__ __forceinline__ void begin(const attn_args &a, const row_tile &t, int w) {
+        table = a.b.page_table + (uint64_t)t.s * a.b.table_stride;
+        scales = ((threadIdx.x & 1) ? a.kv.v_scales : a.kv.k_scales) + t.h;
+        n_pages = a.kv.n_pages, n_kv = a.kv.n_kv_heads, ps_log = 31 - __builtin_clz(a.kv.page_size);
+        last = t.len - 1;
+    }
+    // (past the last position: its page)
+    __device__ __forceinline__ void look(int position) { ahead = table[min(position, last) >> ps_log]; }
+    __device__ __forceinline__ void turn() {
+        const uint32_t id = (uint32_t)uniform(ahead);
+        good = id < n_pages;
+        page = good ? id : 0;
+    }
+    __device__ __forceinline__ void load_scale() { scale = scales[(uint64_t)page * n_kv]; }
+    __device__ __forceinline__ void put_scale(float (*to)[2], int w, bool good) const {
+        const int lane = threadIdx.x & 63;
+        if (lane < 2) to[w][lane] = good ? scale : lane ? 0.0f : __uint_as_float(0x7FC00000u);
+    }
+};
+
+// Many rows.  One workgroup: 128 rows of one sequence and kv head, 32 to a
+// wave, one split of the positions (all of them where there are workgroups
+// enough).  Two buffers, one barrier per tile: the next tile's codes are
+// loaded a tile ahead and converted while the matrix cores work on this one.
+template <int D>
+struct alignas(16) many_shared {
+    shared_tile<D> tile[2];
+};
+template <int D, int TERMS>
+__device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, many_shared<D> &sh) {
+    many_work work;
+    if (!work.find(a, id)) return;
+    const row_tile &t = work.t;
+    wave_rows<D, TERMS> rows;
+    stager<D> k, v;
+    page_walk pages;
+    const int wave = uniform((int)threadIdx.x >> 6);
+    pages.begin(a, t, wave);
+    pages.look(work.p0 + 16 * wave);
+    rows.begin(a, t, t.r0 + 32 * wave);
+    k.begin(a, t.h, wave, false), v.begin(a, t.h, wave, true);
+    auto load = [&](int next) {  // the tile turned to, and the page of the one behind it
+        pages.turn();
+        pages.look(next + 16 * wave);
+        pages.load_scale();
+        k.load(pages.page), v.load(pages.page);
+    };
+    auto put = [&](int buf) {
+        k.put(&sh.tile[buf]), v.put(&sh.tile[buf]);
+        pages.put_scale(sh.tile[buf].scale, wave, pages.good);
+    };
+    if (work.p0 < work.p1) {
+        load(work.p0 + TILE);
+        put(0);
+    }
+    int buf = 0;
+    for (int p = work.p0; p < work.p1; p += TILE, buf ^= 1) {
+        const bool more = p + TILE < work.p1;
+        if (more) load(p + 2 * TILE);
+        __syncthreads();
+        rows.take_scales(sh.tile[buf].scale);
+        const bool live = p < rows.any;
+        wm_h8 w[4][TERMS];
         if (live) {
-#pragma unroll
-            for (int i = 0; i < DT; i++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const wm_h8 v = *(const wm_h8 *)&sh.v[buf][32 * i + n][16 * g + 8 * hi];
-#pragma unroll
-                    for (int x = 0; x < TERMS; x++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[g][x], o[i], 0, 0, 0);
-                }
+            wm_f16v s[2];
+            rows.scores(sh.tile[buf].k, s);
+            rows.weights(s, p, w);
         }
+        if (more) put(buf ^ 1);
+        if (live) rows.values(sh.tile[buf].v, w);
     }
-    if (!valid) return;
-    const float sum = half_sum(sums.l), inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
-    const float lse2 = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
-    const uint64_t part = whole ? 0 : many_part(a, tok, head) + split;
-#pragma unroll
-    for (int i = 0; i < DT; i++)
-#pragma unroll
-        for (int c = 0; c < 16; c += 4) {
-            wm_f4 v;
-#pragma unroll
-            for (int x = 0; x < 4; x++) v[x] = o[i][c + x] * inv;
-            const int d = 32 * i + 2 * c + 4 * hi;
-            if (whole) store_out4(a, tok * a.os + head * D + d, v);
-            else *(wm_f4 *)(a.part_o + part * D + d) = v;
-        }
-    if (hi == 0) {
-        if (!whole) a.part_lse[part] = lse2;
-        else if (a.lse) a.lse[tok * a.n_heads + head] = lse2 * 0.6931471805599453f;
-    }
+    rows.write(a, work.whole, work.split);
 }
 
 // A step with sequences of many rows; those with few are the first
@@ -941,6 +1027,7 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
         // as many row tiles as the packed tokens can fill, not as many as the longest would in every sequence
         const uint64_t full = (uint64_t)b->n_tokens * (n_heads / kv->n_kv_heads) / MANY + b->n_seqs;
         const uint64_t tiles = full < (uint64_t)p.many_tiles * b->n_seqs ? full : (uint64_t)p.many_tiles * b->n_seqs;
+        // 512 workgroups fit the device
         const uint64_t want = (512 + tiles * kv->n_kv_heads - 1) / (tiles * kv->n_kv_heads);
         const uint32_t per = want < rounds ? (uint32_t)(rounds / want) : 1;
         p.many_len = per * ROUND;
