@@ -1,11 +1,24 @@
 // Log probabilities of given tokens, the entropy of their distribution, the
 // token's rank and the top alternatives, per row of logits.
 //
-// A row's logits are read once, which is the bound: a workgroup takes a part
-// of a row into registers (64 VGPRs a lane, all its loads in flight at once),
-// and maximum, sums, rank and top tokens come from there.  The top tokens of a
-// part: about the k-th largest of the lanes' maxima is a value that at least k
-// logits reach, and few more do, so those are listed and ranked by counting.  The parts of a row are joined by a second launch.
+// With m any number near the largest logit, l = sum e^(x - m) and
+// s = sum (x - m) e^(x - m):
+//   logprob = x[token] - m - log l,   entropy = log l - s / l,
+// and sums of two parts of a row join under the larger m.
+//
+// The bound is one read of the logits: a workgroup takes a part of a row into
+// registers (at most 64 VGPRs a lane, all loads in flight at once), and
+// maximum, sums, rank and top tokens come from there.  Lanes read whole
+// 16-byte vectors wherever the row begins.  The top tokens of a part: about
+// the k-th largest of the lanes' maxima is a value that at least k logits
+// reach, and few more do, so those are listed and ranked by counting.  A
+// second launch joins the parts of a row.
+//
+// Measured (f32, 512 rows of 128256, top 5): 51 us, of which 46 are the parts
+// (263 MB, 5.7 TB/s; the chip's last cache holds some of it).  16-bit logits
+// are bound by the vector unit, about 7 operations and one exponential per
+// logit: 2047 rows of 50257 in bfloat16 (206 MB) take 57 us.  One row of
+// 128256, in 32 short parts, takes 12.5 us, the length of two launches' chains.
 #include <cstdio>
 #include <cstring>
 
@@ -46,11 +59,66 @@ __device__ __forceinline__ float key_value(uint64_t key) {
     const uint32_t o = (uint32_t)(key >> 32);
     return o <= 1 ? __uint_as_float(0x7FC00000u) : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-    return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o, 64) << 32 | (uint32_t)__shfl_xor((int)v, o, 64);
+// The value of lane l ^ D, by moves inside the vector unit (a few cycles; a
+// shuffle through LDS takes about a hundred).
+template <int D>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if (D == 1) return __builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);
+    if (D == 2) return __builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);
+    if (D == 4) {  // lanes 0-3 and 8-11 of each 16 from four above, the others from four below
+        const int up = __builtin_amdgcn_update_dpp(0, (int)v, 0x104, 0xF, 0x5, false);
+        return __builtin_amdgcn_update_dpp(up, (int)v, 0x114, 0xF, 0xA, false);
+    }
+    if (D == 8) return __builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, true);
+    if (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (threadIdx.x & 32) ? r[0] : r[1];
+}
+template <int D> __device__ __forceinline__ float lane_xor(float v) { return __uint_as_float(lane_xor<D>(__float_as_uint(v))); }
+template <int D> __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+    return (uint64_t)lane_xor<D>((uint32_t)(v >> 32)) << 32 | lane_xor<D>((uint32_t)v);
+}
+// f(value, value of lane l ^ D) over D = 32 .. 1.
+template <typename T, typename F>
+__device__ __forceinline__ T over_lanes(T v, F f) {
+    v = f(v, lane_xor<32>(v));
+    v = f(v, lane_xor<16>(v));
+    v = f(v, lane_xor<8>(v));
+    v = f(v, lane_xor<4>(v));
+    v = f(v, lane_xor<2>(v));
+    return f(v, lane_xor<1>(v));
+}
+__device__ __forceinline__ float lanes_sum(float v) {
+    return over_lanes(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float lanes_max(float v) {
+    return over_lanes(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ uint64_t lanes_max(uint64_t v) {
+    return over_lanes(v, [](uint64_t a, uint64_t b) { return max(a, b); });
+}
+// One exchange of a descending bitonic sort over the wave: runs of SIZE.
+template <int SIZE, int D>
+__device__ __forceinline__ void exchange(float &y) {
+    const float o = lane_xor<D>(y);
+    const bool lower = ((threadIdx.x & D) != 0) != ((threadIdx.x & SIZE) != 0 && SIZE < 64);
+    y = lower ? fminf(y, o) : fmaxf(y, o);
+    if constexpr (D > 1) exchange<SIZE, D / 2>(y);
+}
+__device__ __forceinline__ float sorted(float y) {
+    exchange<2, 1>(y);
+    exchange<4, 2>(y);
+    exchange<8, 4>(y);
+    exchange<16, 8>(y);
+    exchange<32, 16>(y);
+    exchange<64, 32>(y);
+    return y;
 }
 
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // e^(x - m) sums of two parts under their common maximum.
 __device__ __forceinline__ lp_part join_parts(lp_part a, lp_part b) {
@@ -59,6 +127,14 @@ __device__ __forceinline__ lp_part join_parts(lp_part a, lp_part b) {
     const float ea = __builtin_amdgcn_exp2f(da * LOG2E), eb = __builtin_amdgcn_exp2f(db * LOG2E);
     return {m, a.l * ea + b.l * eb,
             ea * (a.s + a.l * fmaxf(da, -200.0f)) + eb * (b.s + b.l * fmaxf(db, -200.0f)), a.before + b.before};
+}
+
+// The same over lanes that differ in bits D and below.
+template <int D>
+__device__ __forceinline__ lp_part join_lanes(lp_part p) {
+    p = join_parts(p, {lane_xor<D>(p.m), lane_xor<D>(p.l), lane_xor<D>(p.s), (int)lane_xor<D>((uint32_t)p.before)});
+    if constexpr (D > 1) p = join_lanes<D / 2>(p);
+    return p;
 }
 
 // What a finished row says.
@@ -71,12 +147,14 @@ __device__ __forceinline__ row_end end_row(const lp_part &p) {
     return {p.m, none ? 0.0f : logf(p.l), none};
 }
 __device__ __forceinline__ float end_logprob(const row_end &e, float x) {
-    return e.none ? x : (x - e.m) - e.log_l;
+    const float p = e.none ? x : (x - e.m) - e.log_l;
+    return p > 0.0f ? 0.0f : p;  // (by the sum's rounding)
 }
 __device__ __forceinline__ void write_row(const lp_args &a, uint32_t row, const lp_part &p, const row_end &e, bool known,
                                           float xt) {
     if (a.logprob) a.logprob[row] = known ? end_logprob(e, xt) : __uint_as_float(0x7FC00000u);
-    if (a.entropy) a.entropy[row] = e.none ? 0.0f : e.log_l - p.s / p.l;
+    const float entropy = e.none ? 0.0f : e.log_l - p.s / p.l;
+    if (a.entropy) a.entropy[row] = entropy < 0.0f ? 0.0f : entropy;
     if (a.rank) a.rank[row] = known ? p.before : -1;
 }
 __device__ __forceinline__ void write_top(const lp_args &a, uint32_t row, uint32_t i, const row_end &e, uint64_t key) {
@@ -113,9 +191,9 @@ template <> struct vec<__bf16> {
     static __device__ __forceinline__ uint32_t bits(const __bf16 *p) { return *(const uint16_t *)p; }
 };
 
-// In front of each use of a vector in a pass over the registers: without it
-// values unpacked in one pass stay alive for the next, or all of a pass are
-// unpacked at its beginning, and the registers overflow.
+// In front of each use of a vector of 16-bit values in a pass over the
+// registers: without it values unpacked in one pass stay alive for the next,
+// or all of a pass are unpacked at its beginning, and the registers overflow.
 __device__ __forceinline__ void repack(wm_u4 &v) { asm volatile("" : "+v"(v)); }
 
 template <typename T, int NV>
@@ -167,44 +245,51 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
             }
         }
     }
-    // the part's maximum
     const int rounds = (v_end - v0 + NT - 1) / NT;  // of the NV, those that hold logits
+    auto maximum = [&](int n) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (N > 4) repack(v[i]);
+            if (i >= n) continue;
+#pragma unroll
+            for (int e = 0; e < N; e++) top = fmaxf(top, V::at(v[i], e));
+        }
+        return top;
+    };
+    auto of_all_waves = [&](float m) {
+        m = lanes_max(m);
+        __syncthreads();
+        if (lane == 0) sh_part[wave].m = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NT / 64; w++) m = fmaxf(m, sh_part[w].m);
+        return m;
+    };
+    // The sums are relative to the maximum of the part's first round, which
+    // saves a pass where no top tokens are asked for; sums that come out
+    // large, whose logarithm would take the differences' digits, are formed
+    // again under the part's maximum.
+    const float first = maximum(1);
     float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-        if (i >= rounds) continue;
-        repack(v[i]);
-#pragma unroll
-        for (int e = 0; e < N; e++) top = fmaxf(top, V::at(v[i], e));
-    }
-    float m = top;
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if (a.top_k) {
+        top = maximum(rounds);
         // The lanes' maxima in order, and two values that k of them reach: the
         // smallest of the waves' k/4-th, and the largest of their k-th (where
         // a wave holds few logits).
-        float y = top;
-#pragma unroll
-        for (int size = 2; size <= 64; size *= 2)
-#pragma unroll
-            for (int d = size / 2; d; d >>= 1) {
-                const float o = __shfl_xor(y, d, 64);
-                y = ((lane & d) != 0) == ((lane & size) != 0 && size < 64) ? fmaxf(y, o) : fminf(y, o);
-            }
+        const float y = sorted(top);
         const float quarter = __shfl(y, ((int)a.top_k + 3) / 4 - 1, 64), all = __shfl(y, (int)a.top_k - 1, 64);
         if (lane == 0) sh_thr[0][wave] = quarter, sh_thr[1][wave] = all;
+        if (tid == 0) sh_n = 0;
     }
-    if (lane == 0) sh_part[wave].m = m;
-    if (tid == 0) sh_n = 0;
-    __syncthreads();
-    float thr = -INFINITY, least = INFINITY;
+    float m = of_all_waves(first), thr = -INFINITY;
+    if (m == -INFINITY) m = of_all_waves(a.top_k ? top : maximum(rounds));
+    if (a.top_k) {
+        float least = INFINITY;
 #pragma unroll
-    for (int w = 0; w < NT / 64; w++) {
-        m = fmaxf(m, sh_part[w].m);
-        if (a.top_k) thr = fmaxf(thr, sh_thr[1][w]), least = fminf(least, sh_thr[0][w]);
+        for (int w = 0; w < NT / 64; w++) thr = fmaxf(thr, sh_thr[1][w]), least = fminf(least, sh_thr[0][w]);
+        thr = fmaxf(thr, least);
     }
-    if (a.top_k) thr = fmaxf(thr, least);
-    const float base = m == -INFINITY ? 0.0f : m;
 
     // Sums, and the logits before the token: x > xt, or x >= xt below its id,
     // which is x > the number before xt.  (A token at -inf or NaN: by keys.)
@@ -212,45 +297,50 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
     const float below = xt == 0.0f ? -1.401298464e-45f : __uint_as_float(__float_as_uint(xt) + (xt > 0.0f ? -1 : 1));
     float l = 0.0f, s = 0.0f;
     int before = 0;  // of the wave
+    // The exponentials' arguments in one fma, x log2 e - m log2 e; the
+    // rounding of the latter is known and put back into the sums.
+    auto fast = [&]() {
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float shift = base * LOG2E, off = -__builtin_fmaf(base, LOG2E, -shift);
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        if (i >= rounds) continue;
-        repack(v[i]);
-        const int id = (v0 + tid + i * NT) * N - skew;
-        const float limit = id + N <= token ? below : xt;
+        for (int i = 0; i < NV; i++) {
+            if (N > 4) repack(v[i]);
+            if (i >= rounds) continue;
+            const int id = (v0 + tid + i * NT) * N - skew;
+            const float limit = id + N <= token ? below : xt;
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            const float y = V::at(v[i], e), d = y - base, w = __builtin_amdgcn_exp2f(d * LOG2E);
-            l += w;
-            s = __builtin_fmaf(w, fmaxf(d, -200.0f), s);
-            before += __popcll(__ballot(y > limit));
+            for (int e = 0; e < N; e++) {
+                const float y = V::at(v[i], e), d = __builtin_fmaf(y, LOG2E, -shift), w = __builtin_amdgcn_exp2f(d);
+                l += w;
+                s = __builtin_fmaf(w, fmaxf(d, -300.0f), s);
+                before += __popcll(__ballot(y > limit));
+            }
+            if (__ballot(id <= token && id + N > token)) {
+                int same = 0;
+#pragma unroll
+                for (int e = 0; e < N; e++) same += id <= token && id + e < token && id + N > token && V::at(v[i], e) == xt;
+                before += over_lanes((uint32_t)same, [](uint32_t a, uint32_t b) { return a + b; });
+            }
         }
-        if (__ballot(id <= token && id + N > token)) {
-            int same = 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) same += id <= token && id + e < token && id + N > token && V::at(v[i], e) == xt;
-            for (int o = 32; o; o >>= 1) same += __shfl_xor(same, o, 64);
-            before += same;
-        }
-    }
+        s = LN2 * __builtin_fmaf(off, l, s);
+        s = __builtin_fmaf(s, off * LN2, s);
+        l = __builtin_fmaf(l, off * LN2, l);
+    };
+    fast();
     // the part's ids, for what reads them again
     const int id0 = max(v0 * N - skew, 0), id1 = min(v_end * N - skew, vocab);
     if (known && !plain) {
         const uint64_t mine = key_of(xt, token);
         before = 0;
         for (int id = id0 + tid; id < id1; id += NT) before += key_of(V::one(x + id), (uint32_t)id) > mine;
-        for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o, 64);
-    }
-    for (int o = 32; o; o >>= 1) {
-        l += __shfl_xor(l, o, 64);
-        s += __shfl_xor(s, o, 64);
+        before = over_lanes((uint32_t)before, [](uint32_t a, uint32_t b) { return a + b; });
     }
     // the logits that reach the threshold
     if (a.top_k && thr > -INFINITY && top >= thr) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
+            if (N > 4) repack(v[i]);
             if (i >= rounds) continue;
-            repack(v[i]);
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 const float y = V::at(v[i], e);
@@ -261,12 +351,32 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
             }
         }
     }
-    __syncthreads();  // sh_part's maxima are read
-    if (lane == 0) sh_part[wave] = {m, l, s, before};
-    __syncthreads();
-    lp_part p = sh_part[0];
+    auto join_waves = [&]() {
+        l = lanes_sum(l), s = lanes_sum(s);
+        __syncthreads();  // sh_part's maxima are read
+        if (lane == 0) sh_part[wave] = {m, l, s, before};
+        __syncthreads();
+        lp_part p = sh_part[0];
 #pragma unroll
-    for (int w = 1; w < NT / 64; w++) p.l += sh_part[w].l, p.s += sh_part[w].s, p.before += sh_part[w].before;
+        for (int w = 1; w < NT / 64; w++) p.l += sh_part[w].l, p.s += sh_part[w].s, p.before += sh_part[w].before;
+        return p;
+    };
+    lp_part p = join_waves();
+    if (!(p.l <= 1e12f && fabsf(m) <= 1024.0f) && m != -INFINITY) {
+        // The sums are large, or NaN, or the rounding put back is over 2^-13:
+        // the same from memory, by differences to the part's maximum.
+        m = -INFINITY;
+        for (int id = id0 + tid; id < id1; id += NT) m = fmaxf(m, V::one(x + id));
+        m = of_all_waves(m);
+        const float base = m == -INFINITY ? 0.0f : m;
+        l = s = 0.0f;
+        for (int id = id0 + tid; id < id1; id += NT) {
+            const float d = V::one(x + id) - base, w = __builtin_amdgcn_exp2f(d * LOG2E);
+            l += w;
+            s = __builtin_fmaf(w, fmaxf(d, -200.0f), s);
+        }
+        p = join_waves();
+    }
     const bool whole = a.parts == 1;
     const row_end end = end_row(p);
     if (tid == 0) {
@@ -283,6 +393,7 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
         for (int c = tid; c < n; c += NT) {
             const uint64_t mine = sh_list[c];
             uint32_t rank = 0;
+#pragma unroll 8
             for (int i = 0; i < n; i++) rank += sh_list[i] > mine;
             if (rank < a.top_k) put(rank, mine);
         }
@@ -297,7 +408,7 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
             const uint64_t key = key_of(V::one(x + id), (uint32_t)id);
             if (key < last && key > best) best = key;
         }
-        for (int o = 32; o; o >>= 1) best = max(best, shfl_xor64(best, o));
+        best = lanes_max(best);
         __syncthreads();
         if (lane == 0) sh_key[wave] = best;
         __syncthreads();
@@ -317,12 +428,15 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
 // and of another such list: the larger of a[i] and b[63 - i] are they, in an
 // order that six exchanges sort.
 __device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b_reversed, int lane) {
-    uint64_t v = max(a, b_reversed);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const uint64_t o = shfl_xor64(v, d);
-        v = (lane & d) ? min(v, o) : max(v, o);
-    }
+    uint64_t v = max(a, b_reversed), o;
+#define WM_MERGE(D) o = lane_xor<D>(v), v = (lane & D) ? min(v, o) : max(v, o)
+    WM_MERGE(32);
+    WM_MERGE(16);
+    WM_MERGE(8);
+    WM_MERGE(4);
+    WM_MERGE(2);
+    WM_MERGE(1);
+#undef WM_MERGE
     return v;
 }
 
@@ -339,8 +453,7 @@ __global__ __launch_bounds__(NT) void k_logprobs_join(lp_args a) {
     const lp_part *part = a.part + (uint64_t)row * a.parts;
     lp_part p = {-INFINITY, 0.0f, 0.0f, 0};
     for (uint32_t i = tid; i < a.parts; i += NT) p = join_parts(p, part[i]);
-    for (int o = 32; o; o >>= 1)
-        p = join_parts(p, {__shfl_xor(p.m, o, 64), __shfl_xor(p.l, o, 64), __shfl_xor(p.s, o, 64), __shfl_xor(p.before, o, 64)});
+    p = join_lanes<32>(p);
     if (lane == 0) sh_part[wave] = p;
     uint64_t list = 0;
     if (a.top_k) {
@@ -373,6 +486,21 @@ __global__ __launch_bounds__(NT) void k_logprobs_join(lp_args a) {
     }
 }
 
+// The same without top tokens, of at most 16 parts: 16 lanes per row.  (Sums
+// in the order of the kernel above, where the other lanes add nothing: what a
+// row gives does not depend on which outputs are asked for.)
+template <typename T>
+__global__ __launch_bounds__(64) void k_logprobs_join_rows(lp_args a) {
+    const uint32_t at = blockIdx.x * 4 + threadIdx.x / 16, i = threadIdx.x % 16, row = min(at, a.n_rows - 1);
+    const int32_t token = a.tokens ? a.tokens[row] : -1;
+    const bool known = token >= 0 && (uint32_t)token < a.vocab;
+    lp_part p = {-INFINITY, 0.0f, 0.0f, 0};
+    if (i < a.parts) p = a.part[(uint64_t)row * a.parts + i];
+    const float xt = known ? vec<T>::one((const T *)a.x + row * a.stride + token) : 0.0f;
+    p = join_lanes<8>(p);
+    if (i == 0 && at < a.n_rows) write_row(a, row, p, end_row(p), known, xt);
+}
+
 // How a row is divided: as few parts as its lanes' registers allow, and of
 // few rows parts a quarter as long.
 constexpr uint32_t LONG_PART = 64 * NT, SHORT_PART = 16 * NT;  // elements, at most
@@ -386,7 +514,8 @@ lp_plan make_plan(uint32_t n_rows, uint32_t vocab, size_t elem) {
     p.small = (uint64_t)n_rows * ((vocab + LONG_PART - 1) / LONG_PART) <= 128;
     const uint32_t most = (p.small ? SHORT_PART : LONG_PART) / per;
     p.parts = (vecs + most - 1) / most;
-    p.part_vecs = (vecs + p.parts - 1) / p.parts;
+    p.part_vecs = ((vecs + p.parts - 1) / p.parts + NT - 1) / NT * NT;  // of whole rounds, but for the last
+    p.parts = (vecs + p.part_vecs - 1) / p.part_vecs;
     return p;
 }
 size_t plan_bytes(uint32_t n_rows, const lp_plan &p, uint32_t top_k) {
@@ -398,7 +527,9 @@ void launch(const lp_args &a, const lp_plan &p, hipStream_t s) {
     const uint32_t grid = a.n_rows * a.parts;
     if (p.small) k_logprobs_part<T, SHORT_PART / NT / vec<T>::N><<<grid, NT, 0, s>>>(a);
     else k_logprobs_part<T, LONG_PART / NT / vec<T>::N><<<grid, NT, 0, s>>>(a);
-    if (a.parts > 1) k_logprobs_join<T><<<a.n_rows, NT, 0, s>>>(a);
+    if (a.parts <= 1) return;
+    if (!a.top_k && a.parts <= 16) k_logprobs_join_rows<T><<<(a.n_rows + 3) / 4, 64, 0, s>>>(a);
+    else k_logprobs_join<T><<<a.n_rows, NT, 0, s>>>(a);
 }
 
 }  // namespace
