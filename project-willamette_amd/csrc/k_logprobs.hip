@@ -28,7 +28,8 @@ namespace {
 
 constexpr int NT = 256;
 constexpr uint32_t MAX_TOP = 64;
-constexpr int LIST = 512;  // logits that may reach the threshold before the slow way is taken
+constexpr int LIST = 512;   // logits that may reach the threshold before a slower way is taken
+constexpr int FIRST = 128;  // a part's first ids, listed on that way
 
 struct lp_part {  // of one part of a row; with `keys` what the join reads
     float m, l, s;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
     __shared__ uint64_t sh_list[LIST];
     __shared__ lp_part sh_part[NT / 64];
     __shared__ uint64_t sh_key[NT / 64];
-    __shared__ int sh_n;
+    __shared__ int sh_n, sh_reach;
     __shared__ float sh_thr[2][NT / 64];
     const uint32_t row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     const T *x = (const T *)a.x + row * a.stride;
@@ -388,8 +389,29 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
         if (whole) write_top(a, row, i, end, key);
         else a.keys[(uint64_t)blockIdx.x * a.top_k + i] = key;
     };
-    const int n = sh_n;
-    if (thr > -INFINITY && n <= LIST) {
+    int n = sh_n;
+    bool listed = thr > -INFINITY && n <= LIST;
+    if (!listed) {
+        // Fewer than k lanes hold a number above -inf, or very many logits
+        // are equal, as a mask leaves them: what is above the threshold, and
+        // the part's first ids.  Logits at the threshold that are not listed
+        // come behind those that are; if k of the listed reach it, they are it.
+        __syncthreads();
+        if (tid == 0) sh_n = sh_reach = 0;
+        __syncthreads();
+        for (int id = id0 + tid; id < id1; id += NT) {
+            const float y = V::one(x + id);
+            if (y > thr || id < id0 + FIRST) {
+                const int at = atomicAdd(&sh_n, 1);
+                if (at < LIST) sh_list[at] = key_of(y, (uint32_t)id);
+                if (y >= thr) atomicAdd(&sh_reach, 1);
+            }
+        }
+        __syncthreads();
+        n = sh_n;
+        listed = n <= LIST && (sh_reach >= (int)a.top_k || id1 - id0 <= FIRST);
+    }
+    if (listed) {
         for (int c = tid; c < n; c += NT) {
             const uint64_t mine = sh_list[c];
             uint32_t rank = 0;
@@ -397,10 +419,11 @@ __global__ __launch_bounds__(NT, 4) void k_logprobs_part(lp_args a) {
             for (int i = 0; i < n; i++) rank += sh_list[i] > mine;
             if (rank < a.top_k) put(rank, mine);
         }
+        for (uint32_t i = n + tid; i < a.top_k; i += NT) put(i, 0);  // the part has no more
         return;
     }
-    // Fewer than k lanes hold a number above -inf, or very many logits are
-    // equal: one more pass over the part per token.
+    // Many equal or not numbers, and not at the beginning: one more pass over
+    // the part per token.
     uint64_t last = ~0ull;
     for (uint32_t k = 0; k < a.top_k; k++) {
         uint64_t best = 0;

@@ -194,3 +194,61 @@ def test_logprobs_captured(ctx):
         call()
         assert all(np.array_equal(a, o.host()) for a, o in zip(first, out))
     g.close()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("low", ["-inf", "lowest"])
+def test_logprobs_of_masked_vocabularies(ctx, kind, low):
+    """A grammar's mask leaves few tokens of a long row: none in most of its parts, all in one, some at the end."""
+    rng = np.random.default_rng(7)
+    vocab = 70001
+    low = -np.inf if low == "-inf" else float(np.finfo(np.float32).min) if kind == "f32" else -3.3895314e38
+    x = np.full((6, vocab), low, np.float32)
+    x[0, [5, 40000, 70000]] = [1.0, 2.0, 3.0]
+    x[1, 20000:20040] = rng.standard_normal(40)
+    x[2, -700:] = rng.standard_normal(700)        # behind the mask
+    x[3, 200:900] = 0.0                           # equal, and not at the beginning
+    x[4, :64] = rng.standard_normal(64)
+    x[5, ::300] = np.nan                          # no numbers, in each part
+    x = to_kind(x, kind)
+    tok = np.array([40000, 20001, 69000, 555, 65, 1], np.int32)
+    for k in (64, 3):
+        check(run(ctx, x, tok, k, kind), from_kind(x, kind), tok, k)
+
+
+@pytest.mark.parametrize("kind,vocab", [("f32", 16 * 1024 + 5), ("f32", 65536 + 1), ("bf16", 16385), ("f16", 16384 + 600)])
+def test_logprobs_with_a_short_last_part(ctx, kind, vocab):
+    rng = np.random.default_rng(8)
+    x = to_kind(rng.standard_normal((2, vocab)) * 3, kind)
+    x[1, -1] = to_kind(20.0, kind)
+    tok = np.array([vocab - 1, 3], np.int32)
+    for k in (0, 64):
+        check(run(ctx, x, tok, k, kind), from_kind(x, kind), tok, k)
+        check(run(ctx, x.repeat(80, 0), tok.repeat(80), k, kind), from_kind(x, kind).repeat(80, 0), tok.repeat(80), k)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [0, 4])
+def test_logprobs_of_rows_that_rise_late_or_lie_far_out(ctx, kind, k):
+    """Sums relative to a part's first values, where later ones are far above, below, or all are large."""
+    rng = np.random.default_rng(9)
+    x = (rng.standard_normal((6, 30000)) * 3).astype(np.float32)
+    x[0, 25000:] += 60.0
+    x[1, 9000] = 900.0
+    x[2, 4000:] -= 500.0
+    x[3] += 1e4
+    x[4] = x[4] * 300 - 2e4
+    x[5, :3000] = -np.inf
+    x = to_kind(x, kind)
+    tok = np.array([25001, 9000, 1, 77, 5, 2], np.int32)
+    check(run(ctx, x, tok, k, kind), from_kind(x, kind), tok, k)
+
+
+def test_logprobs_do_not_depend_on_what_else_is_asked(ctx):
+    rng = np.random.default_rng(10)
+    x = (rng.standard_normal((150, 70000)) * 3).astype(np.float32)
+    x[3, 60000:] += 80.0
+    tok = rng.integers(0, 70000, 150).astype(np.int32)
+    a, b, one = run(ctx, x, tok, 0), run(ctx, x, tok, 9), run(ctx, x[3:4], tok[3:4], 0)
+    assert all(np.array_equal(p, q) for p, q in zip(a[:3], b[:3]))
+    assert one[2][0] == a[2][3]
