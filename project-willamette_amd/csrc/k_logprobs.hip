@@ -27,7 +27,7 @@
 namespace {
 
 constexpr int NT = 256;
-constexpr uint32_t MAX_TOP = 64;
+constexpr uint32_t MAX_TOP = 64, MAX_VOCAB = 1u << 30;
 constexpr int LIST = 512;   // logits that may reach the threshold before a slower way is taken
 constexpr int FIRST = 128;  // a part's first ids, listed on that way
 
@@ -560,7 +560,7 @@ void launch(const lp_args &a, const lp_plan &p, hipStream_t s) {
 extern "C" {
 
 size_t wm_token_logprobs_workspace(uint32_t n_rows, uint32_t vocab, uint32_t top_k) {
-    if (vocab == 0 || top_k > MAX_TOP) return 0;
+    if (n_rows == 0 || vocab == 0 || vocab > MAX_VOCAB || top_k > MAX_TOP) return 0;
     // of any type: f32 has the most parts
     const size_t a = plan_bytes(n_rows, make_plan(n_rows, vocab, 4), top_k);
     const size_t b = plan_bytes(n_rows, make_plan(n_rows, vocab, 2), top_k);
@@ -575,7 +575,7 @@ wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uin
     if (!ctx) return WM_E_ARG;
     const size_t elem = wm_dtype_size(type);
     if (!elem) return wm_set_error(ctx, WM_E_UNSUPPORTED_TYPE, "%s: type %d is not F32, F16 or BF16", who, type);
-    if (vocab == 0 || vocab > 1u << 30) return wm_set_error(ctx, WM_E_SHAPE, "%s: vocabulary of %u", who, vocab);
+    if (vocab == 0 || vocab > MAX_VOCAB) return wm_set_error(ctx, WM_E_SHAPE, "%s: vocabulary of %u", who, vocab);
     if ((uint64_t)n_rows * make_plan(n_rows, vocab, elem).parts > 0x7FFFFFFFu / NT)  // the launch counts threads in 32 bits
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %u rows of %u", who, n_rows, vocab);
     if (top_k > MAX_TOP || top_k > vocab)

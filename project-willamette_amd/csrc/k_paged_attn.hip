@@ -200,11 +200,9 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // m) has no e_ref in it.
 struct scale_ref {
     int e = E_NONE;
-    float down = 0.0f;   // what m falls by in this tile, and l grows by 2^down
-    int excess = 0;      // what O falls by beyond that (scales more than 2^60 apart), almost never
+    int rise = 0;  // what e has risen by for this tile
     __device__ __forceinline__ void raise(int to) {
-        const int d = e == E_NONE ? 0 : max(to - e, 0);  // before the first scale, O is 0
-        down = (float)min(d, 60), excess = d - min(d, 60);
+        rise = e == E_NONE ? 0 : max(to - e, 0);  // before the first scale, O is 0
         e = max(e, to);
     }
     // log2 of a block's scale (of exponent eb) relative to e.  One 2^60 below
@@ -218,9 +216,16 @@ struct scale_ref {
 // any row of the wave needs it.
 struct row_max {
     float m = -INFINITY, l = 0.0f, from = 0.0f;
-    __device__ __forceinline__ void begin(const scale_ref &r) {
-        m -= r.down, l *= __builtin_amdgcn_exp2f(r.down);
+    // A risen reference lowers m, and l grows; where l would leave its range
+    // (scales more than 2^60 apart), O falls instead, by 2^-fall.  True where
+    // any row of the wave needs that.
+    __device__ __forceinline__ bool begin(const scale_ref &r, int &fall) {
         from = m == -INFINITY ? 0.0f : m;
+        if (uniform(r.rise) == 0) return false;
+        const int down = l > 0x1p60f ? 0 : min(r.rise, 60);
+        m -= (float)down, l = ldexpf(l, down), fall = r.rise - down;
+        from = m == -INFINITY ? 0.0f : m;
+        return __ballot(fall > 0);
     }
     // Every lane's scores have then to be lowered by `by`, O scaled by `alpha`.
     __device__ __forceinline__ bool grows(float top, float &by, float &alpha) {
@@ -233,6 +238,20 @@ struct row_max {
         return true;
     }
 };
+
+// O 2^e / sum: the exponents together, so that no factor leaves its range.
+struct row_scale {
+    float inv;
+    int e;
+    __device__ __forceinline__ row_scale(float sum, int ref_e) {
+        const int k = __builtin_amdgcn_frexp_expf(sum);
+        inv = sum == 0.0f ? 0.0f : 1.0f / ldexpf(sum, -k), e = ref_e - k;
+    }
+    __device__ __forceinline__ float operator()(float o) const { return ldexpf(o * inv, e); }
+};
+// The exponent that a query row is scaled by (rows below 2^-100 are taken as
+// if they reached it: the factor stays finite).
+__device__ __forceinline__ int query_exponent(float most) { return max(__builtin_amdgcn_frexp_expf(most), -100); }
 
 // f32 inputs take two terms, the half types one.
 template <int TERMS>
@@ -391,7 +410,7 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
         for (int i = 0; i < 8; i++) q_max = fmaxf(q_max, fabsf(x_q[j][i]));
     // queries
     wm_h8 q[KS][TERMS];
-    const int e = __builtin_amdgcn_frexp_expf(group_max(q_max));
+    const int e = query_exponent(group_max(q_max));
     const float kfac = ldexpf(a.scale_log2, e - 15), q_scale = ldexpf(1.0f, 15 - e);
 #pragma unroll
     for (int j = 0; j < KS; j++)
@@ -430,12 +449,14 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
         const int eb = sc.v != 0.0f ? __builtin_amdgcn_frexp_expf(sc.v) : E_NONE;
         ref.raise(group_max(eb));
         const float part = ref.part(sc.v, eb), back = __builtin_amdgcn_exp2f(-part);
-        if (ref.excess)
-#pragma unroll
-            for (int i = 0; i < DT; i++) o[i] *= ldexpf(1.0f, -ref.excess);
         const bool masked = p + TILE > all;
         wm_h8 w[2][TERMS];
-        sums.begin(ref);
+        int fall;
+        if (sums.begin(ref, fall))
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[i][c] = ldexpf(o[i][c], -fall);
         const float f = kfac * sc.k, c = part - sums.from;
         float x[16], top = -INFINITY;
 #pragma unroll
@@ -482,9 +503,15 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
 
     // rows of this wave, normalised, with the log2 of their sums
     {
-        const float sum = group_sum(sums.l), inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
+        const float sum = group_sum(sums.l);
+        const row_scale by(sum, ref.e);
 #pragma unroll
-        for (int i = 0; i < DT; i++) *(wm_f4 *)&sh.o[wave][n][16 * i + 4 * g] = o[i] * inv;
+        for (int i = 0; i < DT; i++) {
+            wm_f4 v;
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[c] = by(o[i][c]);
+            *(wm_f4 *)&sh.o[wave][n][16 * i + 4 * g] = v;
+        }
         // a sum of 0 is that of a row without positions, or without a tile
         if (g == 0) sh.lse[wave][n] = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
     }
@@ -643,7 +670,7 @@ struct wave_rows {
 #pragma unroll
                 for (int c = 0; c < 4; c++) x[j][i + c] = v[c], m = fmaxf(m, fabsf(v[c]));
             }
-        const int e = __builtin_amdgcn_frexp_expf(half_max(m));
+        const int e = query_exponent(half_max(m));
         kfac = ldexpf(a.scale_log2, e - 15);
         const float scale = ldexpf(1.0f, 15 - e);
 #pragma unroll
@@ -668,10 +695,12 @@ struct wave_rows {
         e = max(e, __builtin_amdgcn_mov_dpp(e, 0x4E, 0xF, 0xF, true));
         ref.raise(e);
         ks = k, part = ref.part(v, eb), back = __builtin_amdgcn_exp2f(-part);
-        sums.begin(ref);
-        if (ref.excess)
+        int fall;
+        if (sums.begin(ref, fall))
 #pragma unroll
-            for (int i = 0; i < DT; i++) o[i] *= ldexpf(1.0f, -ref.excess);
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int c = 0; c < 16; c++) o[i][c] = ldexpf(o[i][c], -fall);
     }
     // S^T = K Q^T of a tile in LDS.
     __device__ __forceinline__ void scores(const _Float16 (*k)[D + 8], wm_f16v (&s)[2]) const {
@@ -745,7 +774,8 @@ struct wave_rows {
     }
     __device__ __forceinline__ void write(const attn_args &a, bool whole, uint32_t split) const {
         if (!valid) return;
-        const float sum = half_sum(sums.l), inv = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ref.e);
+        const float sum = half_sum(sums.l);
+        const row_scale by(sum, ref.e);
         const float lse2 = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
         const uint64_t part_at = whole ? 0 : many_part(a, tok, head) + split;
 #pragma unroll
@@ -754,7 +784,7 @@ struct wave_rows {
             for (int c = 0; c < 16; c += 4) {
                 wm_f4 v;
 #pragma unroll
-                for (int x = 0; x < 4; x++) v[x] = o[i][c + x] * inv;
+                for (int x = 0; x < 4; x++) v[x] = by(o[i][c + x]);
                 const int d = 32 * i + 2 * c + 4 * hi;
                 if (whole) store_out4(a, tok * a.os + head * D + d, v);
                 else *(wm_f4 *)(a.part_o + part_at * D + d) = v;
@@ -891,7 +921,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
     page_walk pages;
     const int wave = uniform((int)threadIdx.x >> 6);
     pages.begin(a, t, wave);
-    pages.look(work.p0 + 16 * wave);
+    if (work.p0 < work.p1) pages.look(work.p0 + 16 * wave);  // (rows without positions have no page)
     rows.begin(a, t, t.r0 + 32 * wave);
     k.begin(a, t.h, wave, false), v.begin(a, t.h, wave, true);
     auto load = [&](int next) {  // the tile turned to, and the page of the one behind it
@@ -1003,11 +1033,13 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
     }
 }
 
-// How a step is divided: from the host's bounds alone.
+// How a step is divided: from the host's bounds alone, of a step that has
+// tokens and whose max_new times the group fits 32 bits.
 struct attn_plan {
     bool many;         // a sequence may have more than FEW rows
-    uint32_t many_tiles, many_levels, many_len, many_n;
-    uint64_t few_blocks, many_blocks;
+    uint32_t many_levels, many_len, many_n;
+    uint64_t few_blocks, many_blocks, join_blocks;
+    uint32_t join_chunks;  // of a sequence and kv head
     bool join;
     size_t parts;      // partial rows
     uint64_t rounds;   // of all sequences and kv heads, at most
@@ -1021,27 +1053,32 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
     p.parts = rounds > 1 ? (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW : 0;
     p.join = rounds > 1;
     p.rounds = units * rounds;
-    p.many_tiles = 0, p.many_levels = 0, p.many_blocks = 0, p.many_len = 0, p.many_n = 1;
+    p.many_levels = 0, p.many_blocks = 0, p.many_len = 0, p.many_n = 1, p.join_chunks = 1;
     if (p.many) {
-        p.many_tiles = (uint32_t)((rows + MANY - 1) / MANY);
+        const uint64_t most = (rows + MANY - 1) / MANY;  // of one sequence and kv head
         // as many row tiles as the packed tokens can fill, not as many as the longest would in every sequence
         const uint64_t full = (uint64_t)b->n_tokens * (n_heads / kv->n_kv_heads) / MANY + b->n_seqs;
-        const uint64_t tiles = full < (uint64_t)p.many_tiles * b->n_seqs ? full : (uint64_t)p.many_tiles * b->n_seqs;
+        const uint64_t tiles = full < most * b->n_seqs ? full : most * b->n_seqs;
         // 512 workgroups fit the device
         const uint64_t want = (512 + tiles * kv->n_kv_heads - 1) / (tiles * kv->n_kv_heads);
         const uint32_t per = want < rounds ? (uint32_t)(rounds / want) : 1;
         p.many_len = per * ROUND;
         p.many_n = (rounds + per - 1) / per;
         p.many_blocks = tiles * kv->n_kv_heads * p.many_n;
-        p.many_levels = p.many_tiles + (uint32_t)((uint64_t)b->max_kv_len * (n_heads / kv->n_kv_heads) / MANY) + 1;
+        p.many_levels = (uint32_t)most + (uint32_t)((uint64_t)b->max_kv_len * (n_heads / kv->n_kv_heads) / MANY) + 1;
         if (p.many_n > 1) {
             p.parts = (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW;
             p.parts += ((size_t)b->n_tokens * n_heads * p.many_n + 1) & ~(size_t)1;
+            p.join_chunks = (uint32_t)most * (MANY / FEW);
         }
     }
+    p.join_blocks = p.join ? units * p.join_chunks : 0;
     return p;
 }
 
+bool sizes_fit(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
+    return (uint64_t)(b->max_new > b->max_kv_len ? b->max_new : b->max_kv_len) * (n_heads / kv->n_kv_heads) <= 1u << 30;
+}
 // Partial rows, the log2 of their sums, and each unit's parts.
 size_t plan_bytes(const attn_plan &p, const wm_paged_kv *kv, const wm_paged_batch *b) {
     return p.join ? p.parts * (kv->head_dim + 1) * sizeof(float) + (size_t)b->n_seqs * kv->n_kv_heads * sizeof(wm_u2) : 0;
@@ -1052,7 +1089,8 @@ size_t plan_bytes(const attn_plan &p, const wm_paged_kv *kv, const wm_paged_batc
 extern "C" {
 
 size_t wm_paged_attention_workspace(const wm_paged_kv *kv, const wm_paged_batch *batch, uint32_t n_heads) {
-    if (!kv || !batch || !kv->n_kv_heads || n_heads % kv->n_kv_heads) return 0;
+    if (!kv || !batch || !kv->n_kv_heads || n_heads % kv->n_kv_heads || !sizes_fit(kv, batch, n_heads)) return 0;
+    if (batch->n_tokens == 0 || batch->n_seqs == 0 || batch->max_new == 0) return 0;
     return plan_bytes(make_plan(kv, batch, n_heads), kv, batch);
 }
 
@@ -1072,14 +1110,14 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
     if ((st = wm_paged_check_array(ctx, who, "out", d_out, out_stride, n_heads, kv->head_dim, elem))) return st;
     if ((uintptr_t)d_lse % 4) return wm_set_error(ctx, WM_E_ARG, "%s: misaligned lse", who);
-    if ((uint64_t)(batch->max_new > batch->max_kv_len ? batch->max_new : batch->max_kv_len) * (n_heads / kv->n_kv_heads) >
-        1u << 30)
+    if (!sizes_fit(kv, batch, n_heads))
         return wm_set_error(ctx, WM_E_SHAPE, "%s: max_new %u or max_kv_len %u is too large for %u heads over %u", who,
                             batch->max_new, batch->max_kv_len, n_heads, kv->n_kv_heads);
     const attn_plan p = make_plan(kv, batch, n_heads);
-    if (p.few_blocks + p.many_blocks > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups in one step", who,
-                            (unsigned long long)(p.few_blocks + p.many_blocks));
+    const uint64_t most = p.few_blocks + p.many_blocks > p.join_blocks ? p.few_blocks + p.many_blocks : p.join_blocks;
+    if (most > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups, %llu rounds of %d positions in one step", who,
+                            (unsigned long long)most, (unsigned long long)p.rounds, ROUND);
     const size_t need = plan_bytes(p, kv, batch);
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
@@ -1117,10 +1155,9 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
 #undef WM_ATTEND
     WM_HIP(ctx, hipGetLastError());
     if (p.join) {
-        const uint32_t chunks = p.many_n > 1 ? p.many_tiles * (MANY / FEW) : 1;
-        const uint64_t g = (uint64_t)batch->n_seqs * kv->n_kv_heads * chunks;
-        if (kv->head_dim == 64) k_paged_attn_join<64><<<(uint32_t)g, NT, 0, s>>>(a, chunks);
-        else k_paged_attn_join<128><<<(uint32_t)g, NT, 0, s>>>(a, chunks);
+        const uint32_t g = (uint32_t)p.join_blocks;
+        if (kv->head_dim == 64) k_paged_attn_join<64><<<g, NT, 0, s>>>(a, p.join_chunks);
+        else k_paged_attn_join<128><<<g, NT, 0, s>>>(a, p.join_chunks);
         WM_HIP(ctx, hipGetLastError());
     }
     return WM_OK;

@@ -549,3 +549,119 @@ def test_two_contexts(ctx):
     _, _, qx, out, lse, scale = attention_case(other, "f32", st, pool, rng, 4)
     assert_attention(st, pool, "f32", qx, out, lse, scale)
     other.close()
+
+
+# ---------------------------------------------------------------------------
+# many sequences, splits, and values at the ends of their ranges
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind,n_seqs,new,group", [
+    ("f32", 70, [1], 4), ("bf16", 150, [1, 0, 2], 2), ("f32", 130, [1, 0, 17, 9], 2), ("f16", 66, [20, 33], 1)])
+def test_attention_of_many_sequences(ctx, kind, n_seqs, new, group):
+    """More than the 64 that a wave scans at a time, with and without long ones among them."""
+    rng = np.random.default_rng(n_seqs)
+    steps = [(int(rng.integers(0, 40)), new[i % len(new)]) for i in range(n_seqs)]
+    steps[3], steps[n_seqs - 2] = (700, 1), (300, 1)
+    st = Step(rng, steps, 16, 2, 64, pad=1)
+    pool = st.pool(rng)
+    _, _, qx, out, lse, scale = attention_case(ctx, kind, st, pool, rng, 2 * group)
+    assert_attention(st, pool, kind, qx, out, lse, scale)
+
+
+@pytest.mark.parametrize("kind,page,kh,group,dim,steps", [
+    ("f32", 16, 1, 4, 64, [(1500, 40), (0, 20), (700, 1), (900, 0)]),
+    ("bf16", 64, 2, 1, 128, [(2000, 17), (3, 130)]),
+    ("f16", 32, 1, 6, 64, [(1023, 22), (1024, 21), (255, 1), (256, 3)]),
+    ("f32", 64, 1, 33, 128, [(600, 1), (10, 4)])])
+def test_attention_of_many_rows_in_splits(ctx, kind, page, kh, group, dim, steps):
+    """Few row tiles over long contexts: splits that short sequences do not have."""
+    rng = np.random.default_rng(page + group)
+    st = Step(rng, steps, page, kh, dim, pad=2)
+    pool = st.pool(rng)
+    d, _, qx, out, lse, scale = attention_case(ctx, kind, st, pool, rng, kh * group)
+    assert_attention(st, pool, kind, qx, out, lse, scale)
+    # a larger bound divides the step otherwise, and takes more workspace
+    st.max_kv, st.max_new = 64 * st.stride if page == 64 else page * st.stride, st.n_tokens
+    _, _, qx, out, lse, scale = attention_case(ctx, kind, st, pool, rng, kh * group)
+    assert_attention(st, pool, kind, qx, out, lse, scale)
+
+
+def test_more_tokens_than_the_bound_is_nan(ctx):
+    rng = np.random.default_rng(18)
+    st = Step(rng, [(40, 3), (20, 9), (70, 2)], 16, 2, 64)
+    pool = st.pool(rng)
+    st.max_new = 8  # the second sequence has 9
+    d, q, qx, out, lse, scale = attention_case(ctx, "f32", st, pool, rng, 4)
+    got, z = out.host(), lse.host()
+    assert np.isnan(got[3:12]).all() and np.isnan(z[3:12]).all()
+    keep = np.r_[0:3, 12:14]
+    o, want_z, tol, tol_z = ref.attention(st, pool, qx, scale, "f32")
+    assert np.all(np.abs(got[keep] - o[keep]) <= tol[keep]) and np.all(np.abs(z[keep] - want_z[keep]) <= tol_z[keep])
+    # its tokens are not appended, nor read
+    k, _ = typed(ctx, rng, (st.n_tokens, 2, 64), "f32")
+    before = d.host_pool()
+    d.append("f32", None, k, k, None)
+    after = d.host_pool()
+    pages = st.table[1, :2]
+    assert all(same_bits(a[pages], b[pages]) for a, b in zip(before, after))
+    ko = Array.full(ctx, (st.n_tokens, 2, 64), 7.0, "f32")
+    d.read("f32", ko, None)
+    assert np.all(ko.host()[3:12] == 7.0)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attention_of_queries_that_are_not_numbers_stays_in_its_rows(ctx, kind):
+    rng = np.random.default_rng(19)
+    st = Step(rng, [(100, 2), (40, 30)], 16, 1, 64)
+    pool = st.pool(rng)
+    qx = rng.standard_normal((st.n_tokens, 4, 64)).astype(np.float32)
+    bad = np.zeros((st.n_tokens, 4), bool)
+    for at, value in (((0, 1), np.nan), ((5, 2), np.nan), ((9, 0), np.inf), ((20, 3), -np.inf)):
+        qx[at][7] = value
+        bad[at] = True
+    q = Array(ctx, to_kind(qx, kind), kind)
+    out = Array.full(ctx, q.shape, 7.0, kind)
+    lse = Array.full(ctx, (st.n_tokens, 4), 7.0, "f32")
+    d = Device(ctx, st, pool)
+    d.attend(kind, q, out, lse, 0.125)
+    clean = np.where(bad[..., None], 0, q.values())
+    o, z, tol, tol_z = ref.attention(st, pool, clean, 0.125, kind)
+    got, got_z = out.values(), lse.values()
+    assert np.isnan(got[bad]).all()
+    assert np.all(np.abs(got - o)[~bad] <= tol[~bad]) and np.all(np.abs(got_z - z)[~bad] <= tol_z[~bad])
+
+
+@pytest.mark.parametrize("size", [1e-33, 1e-41, 0.0])
+def test_attention_of_tiny_queries(ctx, size):
+    rng = np.random.default_rng(20)
+    st = Step(rng, [(100, 2), (40, 30)], 16, 1, 64)
+    pool = st.pool(rng)
+    _, _, qx, out, lse, scale = attention_case(ctx, "f32", st, pool, rng, 4, size)
+    assert_attention(st, pool, "f32", qx, out, lse, scale)
+
+
+@pytest.mark.parametrize("first,step", [(-100, 40), (-120, 59), (-60, 25), (100, -50), (-100, 100)])
+@pytest.mark.parametrize("steps", [[(90, 1)], [(70, 21)]], ids=["few", "many"])
+def test_attention_under_scales_that_rise_past_f32(ctx, steps, first, step):
+    """Each page's values are 2^step times the last one's, and only the first page's weights count.
+
+    A block's scale that is below 2^-60 of the power of two 2^e at or above the largest of the row's tiles is taken as
+    2^(e - 60): its codes, 127 at most, under weights that sum to one then give up to 127 * 2^(e - 60), with 2^e at most
+    twice the largest scale.  That is the second tolerance; the sums themselves stay within their range."""
+    rng = np.random.default_rng(21)
+    st = Step(rng, steps, 16, 1, 128)
+    pool = st.pool(rng)
+    pages = st.table[0, :6]
+    for i, page in enumerate(pages):
+        pool[0][page] = 127 if i == 0 else -127
+        pool[2][page] = 1 / 64
+        pool[3][page] = 2.0 ** min(first + step * i, 118)
+    n = st.n_tokens
+    qx = (rng.random((n, 4, 128)) + 0.5).astype(np.float32)
+    q = Array(ctx, qx, "f32")
+    out, lse = Array.full(ctx, q.shape, 7.0, "f32"), Array.full(ctx, (n, 4), 7.0, "f32")
+    d = Device(ctx, st, pool)
+    d.attend("f32", q, out, lse, 1.0)
+    o, z, tol, tol_z = ref.attention(st, pool, qx.astype(np.float64), 1.0, "f32")
+    tol += 127 * 2.0 ** -59 * float(pool[3][pages].max())
+    assert np.all(np.abs(out.host() - o) <= tol) and np.all(np.abs(lse.host() - z) <= tol_z)

@@ -212,3 +212,20 @@ def test_logprobs_null_context_and_no_rows(hctx):
     assert f(hctx, None, 0, 5, None, 0, None, None, None, None, None) == 0
     x = np.zeros(5, np.float32)
     assert f(hctx, x.ctypes.data_as(C.POINTER(C.c_float)), 1, 5, None, 65, None, None, None, None, None) == SHAPE
+
+
+def test_workspaces_of_sizes_that_no_call_takes():
+    """Sizes whose plan would divide by nothing or leave 32 bits: no workspace, and no fault."""
+    for over in (dict(n_seqs=0), dict(n_tokens=0), dict(max_new=0), dict(max_new=0xFFFFFFFF, n_tokens=0xFFFFFFFF),
+                 dict(max_kv_len=0xFFFFFFFF), dict(max_new=1 << 31, n_tokens=1 << 31, n_seqs=1 << 31)):
+        kv, b = descriptors(**over)
+        assert wh.paged_attention_workspace(kv, b, 64) == 0
+    for rows, vocab in ((1, 0xFFFFFFFF), (1, 0xFFFFFFFA), (1, 0xFFFFFFF2), (0, 5000), (3, (1 << 30) + 1)):
+        assert wh.token_logprobs_workspace(rows, vocab, 5) == 0
+
+
+def test_attention_refuses_more_workgroups_than_a_launch_has(hctx):
+    kv, b = descriptors(n_kv_heads=4096, n_seqs=4096, max_kv_len=1024, table_stride=64, n_tokens=4096, max_new=1)
+    assert attend(hctx, kv, b, heads=4096, qs=4096 * 128, os=4096 * 128) == SHAPE
+    kv, b = descriptors(n_seqs=1 << 20, n_kv_heads=16, n_tokens=1 << 20, max_new=64)
+    assert attend(hctx, kv, b, heads=64, qs=64 * 128, os=64 * 128) == SHAPE
