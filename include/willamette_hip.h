@@ -427,8 +427,8 @@ typedef enum wm_dtype {
 
 /* One layer's page pool.  A page holds page_size positions (16, 32 or 64) of
  * every kv head; the block of one head in one page is int8 codes and one f32
- * scale for K and one for V: value = code * scale.  head_dim is 64 or 128.
- * The code arrays are 16-byte aligned. */
+ * scale, finite and not negative, for K and one for V: value = code * scale.
+ * head_dim is 64 or 128.  The code arrays are 16-byte aligned. */
 typedef struct wm_paged_kv {
     int8_t *k_codes;  /* [n_pages][n_kv_heads][page_size][head_dim] */
     int8_t *v_codes;  /* [n_pages][n_kv_heads][head_dim][page_size]: positions innermost */
@@ -501,7 +501,7 @@ wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batc
  *   and, where the scale grew, its earlier codes c * old scale / scale
  *   rounded the same way.
  * The quotients are rounded exactly.  Positions behind the last are left as
- * they were.  q_out is the rotated query rounded once to its type.
+ * they were.  q_out is the rotated query, rounded to f32 and then to its type.
  * A sequence whose lengths break their bounds is skipped; tokens of a page
  * outside the pool are not stored.  Two sequences must not append into one
  * page. */
@@ -524,9 +524,14 @@ wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_page
  * h / (n_heads / n_kv_heads).  For a token at position p:
  *   s_j = scale * q . k_j (j <= p),  out = sum_j softmax(s)_j v_j,
  *   lse = ln sum_j exp(s_j)  (d_lse [n_tokens][n_heads] f32, nullable).
+ * Queries count with 22 bits and more of their row's largest (f32) or
+ * exactly (f16, bf16: to 2^-28 of it), softmax weights with 22 bits (f32) or
+ * 11, sums in f32; a block whose value scale is less than 2^-60 of the
+ * largest that its row meets counts as if it were that.
  * A row without positions gives 0 and lse -inf.  A row that reads a page
  * outside the pool, or a sequence whose lengths break their bounds, gives NaN.
- * q and out are of `type`, as in the append; out may be q.
+ * q and out are of `type`, as in the append; out may be q, with q's stride.
+ * Up to 2^30 query rows (max_new * group) and positions * group.
  * work: wm_paged_attention_workspace bytes, 16-byte aligned, overwritten;
  * calls that may run at the same time (graphs replayed on two streams) need
  * one each.  The workspace grows with the batch's host bounds only. */
@@ -548,7 +553,10 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
  * log probabilities and entropy (NaN sorts below every number).  A token
  * outside the vocabulary gives logprob NaN and rank -1; with tokens null,
  * logprob and rank must be null.
- * work: wm_token_logprobs_workspace bytes, 16-byte aligned, as above. */
+ * What an output holds does not depend on which others are asked for.
+ * vocab is at most 2^30.
+ * work: wm_token_logprobs_workspace bytes (0 for one part per row: may be
+ * null), 16-byte aligned, as above. */
 size_t wm_token_logprobs_workspace(uint32_t n_rows, uint32_t vocab, uint32_t top_k);
 wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uint64_t row_stride, uint32_t n_rows,
                                 uint32_t vocab, const int32_t *d_tokens, uint32_t top_k, float *d_logprob,
