@@ -106,6 +106,8 @@ struct append_args {
     uint64_t qs, ks, vs, qos;  // elements between tokens
     uint32_t group;            // query heads per kv head (0: no queries)
     uint32_t touch;            // pages a sequence can touch, at most
+    uint32_t blocks;           // of all sequences, at most
+    bool by_kind;              // order of the workgroups (k_paged_append)
 };
 
 // One block's place in the step: sequence s, its page lp, kv head h.
@@ -321,8 +323,15 @@ template <typename T, int PS, int D>
 __global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
     static_assert(PS * D % (16 * NT) == 0 || PS * D < 16 * NT, "whole units per thread");
     __shared__ float red[NT / 64];
-    const uint32_t kinds = a.group ? 2 + PS / 16 : 2, kind = blockIdx.x % kinds;
-    const block_place p = place_block(a.kv, a.b, a.touch, blockIdx.x / kinds);
+    // Values, keys, queries: the longest chains first where all workgroups
+    // start at about the same time (24 ragged sequences 16.8 us, against 19.2
+    // with a block's kinds side by side), else a block's side by side, which
+    // read neighbouring rows (8 prompts 77 us against 92).
+    uint32_t kind, id;
+    if (a.by_kind) kind = blockIdx.x / a.blocks, id = blockIdx.x % a.blocks;
+    else if (a.group) kind = blockIdx.x % (2 + PS / 16), id = blockIdx.x / (2 + PS / 16);
+    else kind = blockIdx.x % 2, id = blockIdx.x / 2;
+    const block_place p = place_block(a.kv, a.b, a.touch, id);
     if (!p.live) return;
     const int base = p.lp * PS;  // first position of the page
     const int first = max(max(p.q.start, 0) - base, 0), hi = min(p.q.len - base, PS);  // its new slots
@@ -332,8 +341,8 @@ __global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
         append_queries<T, D>(a, p, base, max(first, s0), min(hi, s0 + 16), tok);
         return;
     }
-    if (kind == 0) append_keys<T, PS, D>(a, p, base, first, hi, tok, red);
-    else append_values<T, PS, D>(a, p, first, hi, tok, red);
+    if ((kind == 0) == a.by_kind) append_values<T, PS, D>(a, p, first, hi, tok, red);
+    else append_keys<T, PS, D>(a, p, base, first, hi, tok, red);
 }
 
 struct read_args {
@@ -361,22 +370,29 @@ __global__ __launch_bounds__(NT) void k_paged_read(read_args a) {
     const int8_t *kc = a.kv.k_codes + blk * (PS * D), *vc = a.kv.v_codes + blk * (PS * D);
     const float nan = __uint_as_float(0x7FC00000u);
     const float sk = stored ? a.kv.k_scales[blk] : nan, sv = stored ? a.kv.v_scales[blk] : nan;
-    for (int unit = threadIdx.x; unit < PS * D / 16; unit += NT) {
-        const int quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
-        if (quad + 4 <= first || quad >= hi) continue;
-        uint32_t wk[4], wv[4];
+    constexpr int N = (PS * D / 16 + NT - 1) / NT;
+    uint32_t wk[N][4], wv[N][4];
+#pragma unroll
+    for (int i = 0; i < N; i++) {  // all loads together
+        const int unit = threadIdx.x + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
+        const bool live = quad + 4 > first && quad < hi;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            wk[j] = *(const uint32_t *)(kc + (quad + j) * D + dim);
-            wv[j] = *(const uint32_t *)(vc + (dim + j) * PS + quad);
+            wk[i][j] = live ? *(const uint32_t *)(kc + (quad + j) * D + dim) : 0;
+            wv[i][j] = live ? *(const uint32_t *)(vc + (dim + j) * PS + quad) : 0;
         }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int unit = threadIdx.x + i * NT, quad = unit / (D / 4) * 4, dim = unit % (D / 4) * 4;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             const int slot = quad + t;
             if (slot < first || slot >= hi) continue;
             const uint64_t row = (uint64_t)(tok + slot);
-            if (a.k) wm_st4((T *)a.k + row * a.ks + (uint64_t)p.h * D + dim, values4(wk[t], sk));
-            const uint32_t col = pack_codes(byte_of(wv[0], t), byte_of(wv[1], t), byte_of(wv[2], t), byte_of(wv[3], t));
+            if (a.k) wm_st4((T *)a.k + row * a.ks + (uint64_t)p.h * D + dim, values4(wk[i][t], sk));
+            const uint32_t col = pack_codes(byte_of(wv[i][0], t), byte_of(wv[i][1], t), byte_of(wv[i][2], t),
+                                            byte_of(wv[i][3], t));
             if (a.v) wm_st4((T *)a.v + row * a.vs + (uint64_t)p.h * D + dim, values4(col, sv));
         }
     }
@@ -397,8 +413,10 @@ wm_status block_grid(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const 
 }
 
 template <typename T, int PS, int D> struct launch_append {
-    static void go(const append_args &a, uint32_t grid, hipStream_t s) {
-        k_paged_append<T, PS, D><<<grid * (a.group ? 2 + PS / 16 : 2), NT, 0, s>>>(a);
+    static void go(append_args a, uint32_t blocks, hipStream_t s) {
+        const uint32_t grid = blocks * (a.group ? 2 + PS / 16 : 2);
+        a.blocks = blocks, a.by_kind = grid <= 4096;
+        k_paged_append<T, PS, D><<<grid, NT, 0, s>>>(a);
     }
 };
 template <typename T, int PS, int D> struct launch_read {
