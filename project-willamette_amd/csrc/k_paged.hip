@@ -140,7 +140,7 @@ __device__ __forceinline__ block_place place_block(const wm_paged_kv &kv, const 
 // positions, 33.5 us against 19.2.
 //
 // Measured (20 query heads over 5, f32, pages of 16): 16 sequences of one
-// token 5.1 us, a launch's length; 8 prompts of 100 to 2000 tokens 61 us, and
+// token 4.9 us, a launch's length; 8 prompts of 100 to 2000 tokens 61 us, and
 // 14 to read them back, the time that the 360 MB of both take at the rate of
 // a large copy (4.7 TB/s).
 

@@ -665,3 +665,63 @@ def test_attention_under_scales_that_rise_past_f32(ctx, steps, first, step):
     o, z, tol, tol_z = ref.attention(st, pool, qx.astype(np.float64), 1.0, "f32")
     tol += 127 * 2.0 ** -59 * float(pool[3][pages].max())
     assert np.all(np.abs(out.host() - o) <= tol) and np.all(np.abs(lse.host() - z) <= tol_z)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_captured_ragged_step_follows_its_tokens(ctx, kind):
+    """One graph whose sequences take turns being long, short, empty and padded."""
+    rng = np.random.default_rng(22)
+    kh, group, dim, page, n_tokens, bound = 1, 4, 128, 32, 90, 700
+    whole = Step(rng, [(0, 700)] * 4, page, kh, dim)
+    pool = whole.pool(rng)
+    first = Step(rng, [(0, 1)] * 4, page, kh, dim)
+    first.table, first.stride, first.n_pages = whole.table, whole.stride, whole.n_pages
+    first.n_tokens, first.max_new, first.max_kv = n_tokens, 80, bound
+    d = Device(ctx, first, pool)
+    q, k, v = (Array.full(ctx, (n_tokens, h, dim), 0.0, kind) for h in (kh * group, kh, kh))
+    q_rot, out = (Array.full(ctx, q.shape, 7.0, kind) for _ in range(2))
+    lse = Array.full(ctx, (n_tokens, kh * group), 7.0, "f32")
+    ws = Array(ctx, np.zeros(max(1, wh.paged_attention_workspace(d.kv, d.b, kh * group)), np.uint8))
+
+    def call():
+        d.append(kind, q, k, v, q_rot)
+        d.attend(kind, q_rot, out, lse, 0.09, ws)
+    graph = Graph(ctx, call)
+    expect = [a.copy() for a in pool]
+    for steps in ([(0, 1), (620, 80), (5, 0), (33, 3)], [(699, 1)] * 4, [(0, 0), (0, 0), (690, 10), (0, 79)],
+                  [(400, 5), (0, 70), (31, 1), (0, 14)]):
+        st = Step(rng, steps, page, kh, dim)
+        st.table, st.stride, st.n_pages, st.n_tokens = whole.table, whole.stride, whole.n_pages, n_tokens
+        d.cu.put(st.cu)
+        d.len.put(st.kv_len)
+        x = []
+        for a in (q, k, v):
+            a.put(to_kind(rng.standard_normal(a.shape), kind))
+            x.append(a.values())
+        for a in (q_rot, out, lse):
+            a.put(np.full(a.shape, to_kind(7.0, a.kind)))
+        graph.replay()
+        first_out = out.host()
+        ref.append(st, expect, *x, None, None, 0)
+        assert all(same_bits(a, b) for a, b in zip(d.host_pool(), expect))
+        assert_attention(st, expect, kind, q_rot.values(), out, lse, 0.09)
+        call()
+        assert np.array_equal(out.host(), first_out)
+    graph.close()
+
+
+def test_sequences_share_the_pages_of_a_prefix(ctx):
+    """Three sequences read the same first pages, and append into pages of their own."""
+    rng = np.random.default_rng(23)
+    st = Step(rng, [(70, 1), (66, 20), (64, 2)], 32, 2, 64)
+    pool = st.pool(rng)
+    st.table[1:, :2] = st.table[0, :2]
+    k, kx = typed(ctx, rng, (st.n_tokens, 2, 64), "f32")
+    d, q, qx, out, lse, scale = attention_case(ctx, "f32", st, pool, rng, 4)
+    assert_attention(st, pool, "f32", qx, out, lse, scale)
+    wh.paged_batch_check(d.kv, d.b, st.cu, st.kv_len, st.table)
+    d.append("f32", q, k, k, q)
+    ref.append(st, pool, qx, kx, kx, None, None, 0)
+    assert all(same_bits(a, b) for a, b in zip(d.host_pool(), pool))
+    d.attend("f32", q, out, lse, scale)
+    assert_attention(st, pool, "f32", qx, out, lse, scale)
