@@ -478,8 +478,8 @@ typedef struct wm_rope {
  * cu_tokens non-decreasing from 0 and within n_tokens and max_new, kv_len
  * within 0 and max_kv_len, every page the step reads or writes within the
  * pool, and, with `appends` != 0, every page the append writes written by
- * one sequence only and read by no other.  WM_E_ARG (null pointer, a bound
- * of the structs themselves), WM_E_SHAPE (lengths), WM_E_BOUNDS (pages); the
+ * one sequence only and read by no other.  WM_E_ARG (null pointer),
+ * WM_E_SHAPE (a field of the structs, lengths), WM_E_BOUNDS (pages); the
  * device pointers in `kv` and `batch` are not looked at. */
 wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batch,
                                const int32_t *cu_tokens, const int32_t *kv_len,
