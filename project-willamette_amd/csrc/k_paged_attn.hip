@@ -229,11 +229,14 @@ struct row_max {
     float m = -INFINITY, l = 0.0f, from = 0.0f;
     // A risen reference lowers m, and l grows; where l would leave its range
     // (scales more than 2^60 apart), O falls instead, by 2^-fall.  True where
-    // any row of the wave needs that.
-    __device__ __forceinline__ bool begin(const scale_ref &r, int &fall) {
+    // any row of the wave needs that.  A row's lanes hold parts of its l, but
+    // one m: `row_max` takes the largest of the parts, so that all lanes of a
+    // row do the same.
+    template <typename F>
+    __device__ __forceinline__ bool begin(const scale_ref &r, F row_max, int &fall) {
         from = m == -INFINITY ? 0.0f : m;
         if (uniform(r.rise) == 0) return false;
-        const int down = l > 0x1p60f ? 0 : min(r.rise, 60);
+        const int down = row_max(l) > 0x1p60f ? 0 : min(r.rise, 60);
         m -= (float)down, l = ldexpf(l, down), fall = r.rise - down;
         from = m == -INFINITY ? 0.0f : m;
         return __ballot(fall > 0);
@@ -465,7 +468,7 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
         const bool masked = p + TILE > all;
         wm_h8 w[2][TERMS];
         int fall;
-        if (sums.begin(ref, fall))
+        if (sums.begin(ref, [](float l) { return group_max(l); }, fall))
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -709,7 +712,7 @@ struct wave_rows {
         ref.raise(e);
         ks = k, part = ref.part(v, eb), back = __builtin_amdgcn_exp2f(-part);
         int fall;
-        if (sums.begin(ref, fall))
+        if (sums.begin(ref, half_max, fall))
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll

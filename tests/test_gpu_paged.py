@@ -725,3 +725,46 @@ def test_sequences_share_the_pages_of_a_prefix(ctx):
     assert all(same_bits(a, b) for a, b in zip(d.host_pool(), pool))
     d.attend("f32", q, out, lse, scale)
     assert_attention(st, pool, "f32", qx, out, lse, scale)
+
+
+# ---------------------------------------------------------------------------
+# a row's sums: one decision for all of its lanes
+# ---------------------------------------------------------------------------
+
+def under_a_dominating_key(st, rng, tile, later):
+    """Zeros of a scale of 0 in the first page, whose fifth key alone scores 100 bits; then tiles of `tile` positions
+    with rising value scales: the first one's other keys score 0, `later` (bits, value scale) are those of the next
+    tiles, and all behind them score 0 under the first tile's value scale."""
+    kc, vc, ks, vs = pool = st.pool(rng)
+    ln2 = np.log(2.0)
+    kc[:] = 0
+    for s in range(len(st.steps)):
+        for lp in range(-(-int(st.kv_len[s]) // st.page)):
+            page, i = st.table[s, lp], lp * st.page // tile
+            ks[page], vs[page] = 1.0, 2.0 ** -3
+            if 0 < i <= len(later):
+                bits, vs[page] = later[i - 1]
+                ks[page] = bits * ln2 / 120
+                kc[page, :, :, 0] = rng.integers(112, 125, (st.kh, st.page))
+        first = st.table[s, 0]
+        kc[first, :, 4, 0], ks[first], vs[first] = 120, 100 * ln2 / 120, 0.0
+    return pool
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("kernel", ["few", "many"])
+def test_attention_of_a_dominating_key_without_values(ctx, kernel, kind):
+    """The fifth key's lane holds a sum that the row's other lanes do not when the value scales rise."""
+    rng = np.random.default_rng(24)
+    if kernel == "few":
+        # 17 rounds of 256 positions of 64 heads: more than 1024 rounds, so that a wave has several tiles
+        st, tile, group = Step(rng, [(4200, 1)], 16, 64, 64), 256, 1
+    else:
+        st, tile, group = Step(rng, [(200, 20)], 16, 2, 64), 64, 4
+    pool = under_a_dominating_key(st, rng, tile, [(103, 0.5), (102, 2.0)])
+    q = np.zeros((st.n_tokens, st.kh * group, 64), np.float32)
+    q[..., 0] = 1.0
+    q = Array(ctx, to_kind(q, kind), kind)
+    out, lse = Array.full(ctx, q.shape, 7.0, kind), Array.full(ctx, q.shape[:2], 7.0, "f32")
+    Device(ctx, st, pool).attend(kind, q, out, lse, 1.0)
+    assert_attention(st, pool, kind, q.values(), out, lse, 1.0)
