@@ -527,7 +527,8 @@ wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_page
  * Queries count with 22 bits and more of their row's largest (f32) or
  * exactly (f16, bf16: to 2^-28 of it), softmax weights with 22 bits (f32) or
  * 11, sums in f32; a block whose value scale is less than 2^-60 of the
- * largest that its row meets counts as if it were that.
+ * largest of the blocks that its row attends to counts as if it were that.
+ * What a row gives does not depend on what the positions behind it hold.
  * A row without positions gives 0 and lse -inf.  A row that reads a page
  * outside the pool, or a sequence whose lengths break their bounds, gives NaN.
  * q and out are of `type`, as in the append; out may be q, with q's stride.

@@ -39,7 +39,7 @@ constexpr int NT = 256;    // threads per workgroup, four waves
 constexpr int TILE = 64;   // positions per tile of one wave
 constexpr float W_EXP = 7.0f;   // the largest weight is 2^W_EXP when the sums are scaled,
 constexpr float W_MOST = 15.0f; // and may grow to this before they are scaled anew (f16 ends at 2^16)
-constexpr int E_NONE = -200;    // the exponent of a zero scale
+constexpr int E_NONE = -1000;   // the exponent of a zero scale
 constexpr int FEW = 16;    // rows (tokens x group) of a sequence and kv head up to which a wave takes them all
 constexpr int MANY = 128;  // rows of a workgroup beyond
 
@@ -204,11 +204,19 @@ __device__ __forceinline__ float read_lane(float v, int lane) {
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// The value scales' reference exponent over the tiles so far: what is held
-// is O 2^-e_ref, and the running maximum m is that of score + log2(scale) -
-// e_ref, so that the f16 weights hold their 11 bits relative to the largest
-// product of weight and scale, however the scales differ.  l = sum 2^(score -
-// m) has no e_ref in it.
+// A value scale's exponent, and the log2 of what the exponent leaves.
+__device__ __forceinline__ int scale_exponent(float v) { return v != 0.0f ? __builtin_amdgcn_frexp_expf(v) : E_NONE; }
+__device__ __forceinline__ float scale_rest(float v, int e) {
+    return v != 0.0f ? __builtin_amdgcn_logf(ldexpf(v, -e)) : -60.0f;
+}
+
+// A row's reference exponent, the largest of the value scales of the blocks
+// that it attends to in the tiles so far (a tile's other blocks do not count:
+// what a row gives must not depend on them).  What is held is O 2^-e, and the
+// running maximum m is that of score + log2(scale) - e, so that the f16
+// weights hold their 11 bits relative to the largest product of weight and
+// scale, however the scales differ.  l = sum 2^(score - m) has no e in it.
+// Until a tile is masked all rows of a wave have the same e.
 struct scale_ref {
     int e = E_NONE;
     int rise = 0;  // what e has risen by for this tile
@@ -216,10 +224,10 @@ struct scale_ref {
         rise = e == E_NONE ? 0 : max(to - e, 0);  // before the first scale, O is 0
         e = max(e, to);
     }
-    // log2 of a block's scale (of exponent eb) relative to e.  One 2^60 below
-    // it, or 0, counts as 2^-60: such a weight is 0 in f16.
-    __device__ __forceinline__ float part(float v, int eb) const {
-        return v == 0.0f || eb < e - 60 ? -60.0f : (float)(eb - e) + __builtin_amdgcn_logf(ldexpf(v, -eb));
+    // log2 of a block's scale (scale_exponent, scale_rest) relative to e.  One
+    // 2^60 below it, or 0, counts as 2^-60: such a weight is 0 in f16.
+    __device__ __forceinline__ float part(int eb, float rest) const {
+        return eb < e - 60 ? -60.0f : (float)(eb - e) + rest;
     }
 };
 // Under a new tile's largest relative score `top` (of the row): m, l and what
@@ -235,16 +243,18 @@ struct row_max {
     template <typename F>
     __device__ __forceinline__ bool begin(const scale_ref &r, F row_max, int &fall) {
         from = m == -INFINITY ? 0.0f : m;
-        if (uniform(r.rise) == 0) return false;
+        if (!__ballot(r.rise != 0)) return false;
         const int down = row_max(l) > 0x1p60f ? 0 : min(r.rise, 60);
         m -= (float)down, l = ldexpf(l, down), fall = r.rise - down;
         from = m == -INFINITY ? 0.0f : m;
         return __ballot(fall > 0);
     }
-    // Every lane's scores have then to be lowered by `by`, O scaled by `alpha`.
+    // Every lane's scores have then to be lowered by `by`, O scaled by `alpha`
+    // (by 0 and 1 in rows that do not need it).
     __device__ __forceinline__ bool grows(float top, float &by, float &alpha) {
-        if (!__ballot(top > (m == -INFINITY ? -INFINITY : W_MOST))) return false;
-        const float to = fmaxf(m, from + top - W_EXP), base = to == -INFINITY ? 0.0f : to;
+        const bool over = top > (m == -INFINITY ? -INFINITY : W_MOST);
+        if (!__ballot(over)) return false;
+        const float to = over ? fmaxf(m, from + top - W_EXP) : m, base = to == -INFINITY ? 0.0f : to;
         alpha = __builtin_amdgcn_exp2f(m - base);
         l *= alpha;
         m = to;
@@ -462,10 +472,11 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
             sc_next = load_scales(pg_next.v);
             if (p + 8 * TILE < p1) pg_after = load_pages(p + 8 * TILE);
         }
-        const int eb = sc.v != 0.0f ? __builtin_amdgcn_frexp_expf(sc.v) : E_NONE;
-        ref.raise(group_max(eb));
-        const float part = ref.part(sc.v, eb), back = __builtin_amdgcn_exp2f(-part);
         const bool masked = p + TILE > all;
+        const int left = masked ? count - (p + g * 16) : 16;  // of the lane's positions, those that its row attends to
+        const int eb = scale_exponent(sc.v);
+        ref.raise(group_max(left > 0 ? eb : E_NONE));
+        const float part = ref.part(eb, scale_rest(sc.v, eb)), back = __builtin_amdgcn_exp2f(-part);
         wm_h8 w[2][TERMS];
         int fall;
         if (sums.begin(ref, [](float l) { return group_max(l); }, fall))
@@ -478,7 +489,6 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
 #pragma unroll
         for (int i = 0; i < 16; i++) x[i] = __builtin_fmaf(s[i / 4][i % 4], f, c);
         if (masked) {
-            const int left = count - (p + g * 16);
 #pragma unroll
             for (int i = 0; i < 16; i++) x[i] = i < left ? x[i] : -INFINITY;
         }
@@ -664,8 +674,9 @@ struct wave_rows {
     wm_f16v o[DT];
     row_max sums;
     scale_ref ref;
-    // a tile's scales: of the lane's group of 16 positions (lane % 4)
-    float ks, part, back;
+    // a tile's scales, K's and V's: of the lane's group of 16 positions (lane % 4)
+    float ks, v_rest, part, back;
+    int v_exp;
 
     __device__ __forceinline__ void begin(const attn_args &a, const row_tile &t, int w0) {
         const int lane = threadIdx.x & 63;
@@ -703,14 +714,21 @@ struct wave_rows {
 #pragma unroll
             for (int c = 0; c < 16; c++) o[i][c] = 0.0f;
     }
-    // The next tile's scales.
-    __device__ __forceinline__ void take_scales(const float (*scale)[2]) {
-        const float k = scale[threadIdx.x & 3][0], v = scale[threadIdx.x & 3][1];
-        const int eb = v != 0.0f ? __builtin_amdgcn_frexp_expf(v) : E_NONE;
-        int e = max(eb, __builtin_amdgcn_mov_dpp(eb, 0xB1, 0xF, 0xF, true));  // over lanes l ^ 1, l ^ 2
+    // The scales of the tile at p, and the rows' reference with them: the
+    // scales relative to it as logarithms, and their inverses, where all rows
+    // have the same (in masked tiles `weights` does that row by row).
+    __device__ __forceinline__ void take_scales(const float (*scale)[2], int p) {
+        const float v = scale[threadIdx.x & 3][1];
+        ks = scale[threadIdx.x & 3][0], v_exp = scale_exponent(v), v_rest = scale_rest(v, v_exp);
+        int e = max(v_exp, __builtin_amdgcn_mov_dpp(v_exp, 0xB1, 0xF, 0xF, true));  // over lanes l ^ 1, l ^ 2
         e = max(e, __builtin_amdgcn_mov_dpp(e, 0x4E, 0xF, 0xF, true));
+        if (p + TILE > all) {
+            e = E_NONE;
+#pragma unroll
+            for (int g = 0; g < 4; g++) e = max(e, 16 * g < count - p ? __builtin_amdgcn_readlane(v_exp, g) : E_NONE);
+        }
         ref.raise(e);
-        ks = k, part = ref.part(v, eb), back = __builtin_amdgcn_exp2f(-part);
+        part = ref.part(v_exp, v_rest), back = __builtin_amdgcn_exp2f(-part);
         int fall;
         if (sums.begin(ref, half_max, fall))
 #pragma unroll
@@ -734,14 +752,25 @@ struct wave_rows {
     // Scores of the tile at p to weights, relative to the maximum so far, the
     // values' scale included.
     __device__ __forceinline__ void weights(const wm_f16v (&s)[2], int p, wm_h8 (&w)[4][TERMS]) {
+        const bool masked = p + TILE > all;
+        float c[4], inverse[4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) c[g] = read_lane(part, g) - sums.from, inverse[g] = read_lane(back, g);
+        if (masked) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float of_row = ref.part(__builtin_amdgcn_readlane(v_exp, g), read_lane(v_rest, g));
+                c[g] = of_row - sums.from, inverse[g] = __builtin_amdgcn_exp2f(-of_row);
+            }
+        }
         float x[4][8];
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-            const float f = kfac * read_lane(ks, g), c = read_lane(part, g) - sums.from;
+            const float f = kfac * read_lane(ks, g);
 #pragma unroll
-            for (int y = 0; y < 8; y++) x[g][y] = __builtin_fmaf(s[g / 2][8 * (g % 2) + y], f, c);
+            for (int y = 0; y < 8; y++) x[g][y] = __builtin_fmaf(s[g / 2][8 * (g % 2) + y], f, c[g]);
         }
-        if (p + TILE > all) {
+        if (masked) {
             const int left = count - p - 4 * hi;
 #pragma unroll
             for (int g = 0; g < 4; g++)
@@ -774,7 +803,7 @@ struct wave_rows {
                 w[g][0][y] = h;
                 if (TERMS > 1) w[g][TERMS - 1][y] = lo;
             }
-            sums.l = __builtin_fmaf(sum, read_lane(back, g), sums.l);
+            sums.l = __builtin_fmaf(sum, inverse[g], sums.l);
         }
     }
     // O^T += V^T P^T of a tile in LDS.
@@ -962,7 +991,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         const bool more = p + TILE < work.p1;
         if (more) load(p + 2 * TILE);
         __syncthreads();
-        rows.take_scales(sh.tile[buf].scale);
+        rows.take_scales(sh.tile[buf].scale, p);
         const bool live = p < rows.any;
         wm_h8 w[4][TERMS];
         if (live) {

@@ -768,3 +768,29 @@ def test_attention_of_a_dominating_key_without_values(ctx, kernel, kind):
     out, lse = Array.full(ctx, q.shape, 7.0, kind), Array.full(ctx, q.shape[:2], 7.0, "f32")
     Device(ctx, st, pool).attend(kind, q, out, lse, 1.0)
     assert_attention(st, pool, kind, q.values(), out, lse, 1.0)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_attention_does_not_depend_on_scales_behind_its_rows(ctx, kind, group):
+    """Value scales of a tile's later pages, far above those that a row attends to (rows of the kernel for few and for
+    many): within the tolerance of the row's own values, and bit for bit what other scales there leave."""
+    rng = np.random.default_rng(25)
+    st = Step(rng, [(8, 16), (40, 60)] if group > 1 else [(8, 16), (5, 9)], 16, 1, 64)
+    pool = st.pool(rng)
+    q, qx = typed(ctx, rng, (st.n_tokens, group, 64), kind, 2.0)
+    first = {}
+    for step in (100, 70, 1, 0, -30):
+        for s in range(2):
+            for i, page in enumerate(st.table[s, :-(-int(st.kv_len[s]) // 16)]):
+                pool[3][page] = np.float32(1.3) * np.float32(2.0) ** (-100 if i == 0 else min(-100 + step * i, 100))
+        out, lse = Array.full(ctx, q.shape, 7.0, kind), Array.full(ctx, q.shape[:2], 7.0, "f32")
+        Device(ctx, st, pool).attend(kind, q, out, lse, 0.125)
+        o, z, tol, tol_z = ref.attention(st, pool, qx, 0.125, kind)
+        # rows that attend to the first page only
+        for t in [t for s in range(2) for t in range(st.cu[s], st.cu[s + 1]) if t - st.cu[s] + st.steps[s][0] < 16]:
+            assert np.all(np.abs(out.values()[t] - o[t]) <= tol[t]), (step, t)
+            # (1e-37 of the tolerance is no more than 2^-22 of these values)
+            assert np.abs(o[t]).max() > 2.0 ** -100
+            assert np.all(np.abs(lse.values()[t] - z[t]) <= tol_z[t])
+            assert same_bits(out.host()[t], first.setdefault(t, out.host()[t])), (step, t)
