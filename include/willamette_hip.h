@@ -446,7 +446,12 @@ typedef struct wm_paged_kv {
  * page page_table[i * table_stride + position / page_size].  Tokens from
  * cu_tokens[n_seqs] to n_tokens are padding: no output of theirs is written.
  * A token whose position is negative (kv_len[i] < n) has no place in the
- * cache: it is not appended, and its attention row is empty. */
+ * cache: it is not appended, and its attention row is empty.
+ * A sequence breaks its bounds where its two cu_tokens fall or lie outside 0
+ * to n_tokens (or the first is not 0), where n > max_new, or where kv_len is
+ * outside 0 to max_kv_len.  Not defined, but within the buffers: the rows of
+ * sequences whose tokens overlap, as offsets that fall can leave them, and
+ * pages that two sequences append to. */
 typedef struct wm_paged_batch {
     const int32_t *cu_tokens;  /* n_seqs + 1, non-decreasing from 0 */
     const int32_t *kv_len;     /* n_seqs */

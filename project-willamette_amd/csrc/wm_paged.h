@@ -39,8 +39,9 @@ __device__ __forceinline__ void wm_st4(__bf16 *p, wm_f4 v) { *(wm_b4 *)p = __bui
 // ---------------------------------------------------------------------------
 
 // The arrays are device contents that no host check has seen: tok0 and n
-// always lie within the packed arrays, and a sequence with `ok` has its
-// positions within the bounds the grid and the page table were sized for.
+// always lie within the packed arrays, and a sequence with `ok` has all its
+// tokens there and its positions within the bounds the grid and the page table
+// were sized for.
 struct wm_seq {
     int tok0, n;  // first packed token, tokens
     int start;    // position of the first (negative: that many tokens have none)
@@ -54,7 +55,8 @@ __device__ __forceinline__ wm_seq wm_load_seq(const wm_paged_batch &b, uint32_t 
     q.tok0 = min(max(c0, 0), most);
     q.n = min(max(c1, q.tok0), most) - q.tok0;
     q.len = len;
-    q.ok = len >= 0 && len <= (int)b.max_kv_len && q.n <= (int)b.max_new;
+    q.ok = c0 >= 0 && c1 >= c0 && c1 <= most && (s != 0 || c0 == 0) && len >= 0 && len <= (int)b.max_kv_len &&
+           q.n <= (int)b.max_new;
     q.start = q.ok ? len - q.n : 0;
     return q;
 }

@@ -794,3 +794,47 @@ def test_attention_does_not_depend_on_scales_behind_its_rows(ctx, kind, group):
             assert np.abs(o[t]).max() > 2.0 ** -100
             assert np.all(np.abs(lse.values()[t] - z[t]) <= tol_z[t])
             assert same_bits(out.host()[t], first.setdefault(t, out.host()[t])), (step, t)
+
+
+@pytest.mark.parametrize("cu", [[0, 6, 14], [0, 6, 1 << 30], [3, 6, 10], [-2, 6, 10], [0, -1, 4], [0, 6, 5]],
+                         ids=["past", "far-past", "not-from-0", "before-0", "negative", "falls"])
+def test_sequences_whose_tokens_break_their_bounds(ctx, cu):
+    """Token offsets past the packed arrays, not from 0, negative, falling: such a sequence is not appended nor read, the
+    rows of the packed arrays that it has are NaN, and the others are as they are without it."""
+    rng = np.random.default_rng(26)
+    kh, dim, page = 2, 64, 16
+    st = Step(rng, [(0, 6), (16, 4)], page, kh, dim)
+    st.max_new = 8
+    pool = st.pool(rng)
+    st.cu = np.array(cu, np.int32)
+    bad = [s for s in range(2) if not 0 <= cu[s] <= cu[s + 1] <= st.n_tokens or (s == 0 and cu[0])]
+    good = [s for s in range(2) if s not in bad]
+    q, qx = typed(ctx, rng, (st.n_tokens, 4, dim), "f32")
+    k, kx = typed(ctx, rng, (st.n_tokens, kh, dim), "f32")
+    q_out, out = (Array.full(ctx, q.shape, 7.0, "f32") for _ in range(2))
+    ko, vo = (Array.full(ctx, k.shape, 7.0, "f32") for _ in range(2))
+    lse = Array.full(ctx, q.shape[:2], 7.0, "f32")
+    d = Device(ctx, st, pool)
+    with pytest.raises(wh.WillametteError):
+        wh.paged_batch_check(d.kv, d.b, st.cu, st.kv_len, st.table)
+    d.append("f32", q, k, k, q_out)
+    d.read("f32", ko, vo)
+    d.attend("f32", q, out, lse, 0.125)
+    for a, b in zip(d.host_pool(), pool):
+        for s in bad:
+            own = st.table[s][st.table[s] >= 0]
+            assert same_bits(a[own], b[own])
+    # every row: of a good sequence, of a bad one, or of none
+    owner = np.full(st.n_tokens, -1)
+    for s in range(2):
+        owner[max(cu[s], 0):max(cu[s + 1], 0)] = s
+    for t, s in enumerate(owner):
+        if s in good:
+            assert np.array_equal(q_out.host()[t], qx[t].astype(np.float32)) and np.isfinite(ko.host()[t]).all()
+            assert np.isfinite(out.host()[t]).all() and np.isfinite(lse.host()[t]).all()
+        else:
+            assert np.all(q_out.host()[t] == 7.0) and np.all(ko.host()[t] == 7.0) and np.all(vo.host()[t] == 7.0)
+            if s in bad:
+                assert np.isnan(out.host()[t]).all() and np.isnan(lse.host()[t]).all()
+            else:
+                assert np.all(out.host()[t] == 7.0) and np.all(lse.host()[t] == 7.0)
