@@ -540,7 +540,10 @@ wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_page
  * Up to 2^30 query rows (max_new * group) and positions * group.
  * work: wm_paged_attention_workspace bytes, 16-byte aligned, overwritten;
  * calls that may run at the same time (graphs replayed on two streams) need
- * one each.  The workspace grows with the batch's host bounds only. */
+ * one each.  The size goes by the batch's host bounds (n_seqs, n_tokens,
+ * max_new, max_kv_len) and is enough for every step whose bounds are no
+ * larger; with head_dim 128 it is at most 110 MB and 8.3 KB per sequence and
+ * kv head. */
 size_t wm_paged_attention_workspace(const wm_paged_kv *kv, const wm_paged_batch *batch, uint32_t n_heads);
 wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
                                  const void *d_q, uint64_t q_stride, uint32_t n_heads, float scale, void *d_out,

@@ -59,8 +59,10 @@ struct attn_args {
     // positions each per row tile, many_blocks in all; many_levels row tiles of MANY and
     // contexts of as many tokens at most (many_order).
     uint32_t few_blocks, many_blocks, many_levels, many_len, many_n;
-    // partial rows: FEW of each few_share::slot, then [token][head][many_n]
+    // partial rows: FEW of each few_share::slot, then [token][head][many_n] of
+    // the packed tokens or, where they are fewer, of max_new to a sequence
     float *part_o, *part_lse;
+    bool parts_by_seq;
     // of each (sequence of few rows, kv head): the first workgroup that has a part of it, and how many have
     uint32_t *few_parts;
 };
@@ -71,7 +73,8 @@ constexpr int ROUND = 4 * TILE;  // positions that a workgroup's four waves take
 // 1024 workgroups 144 us against 139 over 512.
 constexpr uint32_t FEW_RESIDENT = 512;
 __host__ __device__ inline uint64_t few_slots(uint32_t blocks, uint32_t units) { return (uint64_t)blocks + units; }
-__device__ __forceinline__ uint64_t many_part(const attn_args &a, uint64_t token, uint64_t head) {
+__device__ __forceinline__ uint64_t many_part(const attn_args &a, uint32_t s, const wm_seq &q, uint64_t token, uint64_t head) {
+    if (a.parts_by_seq) token = (uint64_t)s * a.b.max_new + (token - q.tok0);
     return (a.few_blocks ? few_slots(a.few_blocks, a.b.n_seqs * a.kv.n_kv_heads) * FEW : 0) +
            (token * a.n_heads + head) * a.many_n;
 }
@@ -817,12 +820,12 @@ struct wave_rows {
                 for (int y = 0; y < TERMS; y++) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w[g][y], o[i], 0, 0, 0);
             }
     }
-    __device__ __forceinline__ void write(const attn_args &a, bool whole, uint32_t split) const {
+    __device__ __forceinline__ void write(const attn_args &a, const row_tile &t, bool whole, uint32_t split) const {
         if (!valid) return;
         const float sum = half_sum(sums.l);
         const row_scale by(sum, ref.e);
         const float lse2 = sum == 0.0f ? -INFINITY : sums.m + __builtin_amdgcn_logf(sum);
-        const uint64_t part_at = whole ? 0 : many_part(a, tok, head) + split;
+        const uint64_t part_at = whole ? 0 : many_part(a, t.s, t.q, tok, head) + split;
 #pragma unroll
         for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -1002,7 +1005,7 @@ __device__ __forceinline__ void attend_many(const attn_args &a, uint32_t id, man
         if (more) put(buf ^ 1);
         if (live) rows.values(sh.tile[buf].v, w);
     }
-    rows.write(a, work.whole, work.split);
+    rows.write(a, t, work.whole, work.split);
 }
 
 // A step with sequences of many rows, whose workgroups run longer and come
@@ -1045,7 +1048,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
     for (int i = threadIdx.x; i < rows * (D / 4); i += NT) {
         const int r = r0 + i / (D / 4), c = i % (D / 4) * 4;
         const uint64_t tok = row_token(a, t, r), head = row_head(a, t, r);
-        const uint64_t part = few ? first + r : many_part(a, tok, head);
+        const uint64_t part = few ? first + r : many_part(a, s, t.q, tok, head);
         const float *ls = a.part_lse + part, *os = a.part_o + part * D + c;
         // eight splits at a time, their loads together
         wm_f4 v = {0, 0, 0, 0};
@@ -1091,8 +1094,15 @@ struct attn_plan {
     uint32_t join_chunks;  // of a sequence and kv head
     bool join;
     size_t parts;      // partial rows
+    bool parts_by_seq;
     uint64_t rounds;   // of all sequences and kv heads, at most
 };
+// Tokens that rows of splits are kept of: the packed ones or max_new of each
+// sequence, whichever are fewer, so that padding costs none.
+uint64_t kept_tokens(const wm_paged_batch *b) {
+    const uint64_t by_seq = (uint64_t)b->n_seqs * b->max_new;
+    return by_seq < b->n_tokens ? by_seq : b->n_tokens;
+}
 attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
     attn_plan p;
     const uint64_t rows = (uint64_t)b->max_new * (n_heads / kv->n_kv_heads), units = (uint64_t)b->n_seqs * kv->n_kv_heads;
@@ -1101,6 +1111,7 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
     p.few_blocks = units * rounds < 2 * FEW_RESIDENT ? units * rounds : 2 * FEW_RESIDENT;
     p.parts = rounds > 1 ? (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW : 0;
     p.join = rounds > 1;
+    p.parts_by_seq = kept_tokens(b) < b->n_tokens;
     p.rounds = units * rounds;
     p.many_levels = 0, p.many_blocks = 0, p.many_len = 0, p.many_n = 1, p.join_chunks = 1;
     if (p.many) {
@@ -1117,7 +1128,7 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
         p.many_levels = (uint32_t)most + (uint32_t)((uint64_t)b->max_kv_len * (n_heads / kv->n_kv_heads) / MANY) + 1;
         if (p.many_n > 1) {
             p.parts = (size_t)few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW;
-            p.parts += ((size_t)b->n_tokens * n_heads * p.many_n + 1) & ~(size_t)1;
+            p.parts += (kept_tokens(b) * n_heads * p.many_n + 1) & ~(size_t)1;
             p.join_chunks = (uint32_t)most * (MANY / FEW);
         }
     }
@@ -1128,9 +1139,24 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
 bool sizes_fit(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
     return (uint64_t)(b->max_new > b->max_kv_len ? b->max_new : b->max_kv_len) * (n_heads / kv->n_kv_heads) <= 1u << 30;
 }
-// Partial rows, the log2 of their sums, and each unit's parts.
-size_t plan_bytes(const attn_plan &p, const wm_paged_kv *kv, const wm_paged_batch *b) {
-    return p.join ? p.parts * (kv->head_dim + 1) * sizeof(float) + (size_t)b->n_seqs * kv->n_kv_heads * sizeof(wm_u2) : 0;
+// Partial rows, the log2 of their sums, and each unit's parts: of this plan
+// and of those of all smaller bounds (a smaller step may have more splits).
+// Of T = tiles * kv heads a split step has T < 512 and up to 2 ceil(512 / T) -
+// 1 splits, so T * many_n <= 1022 + T <= 1533, and its kept tokens fill MANY
+// rows of each tile at most.
+constexpr uint64_t MOST_PARTS = (uint64_t)MANY * 1533;
+size_t plan_bytes(const attn_plan &p, const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_heads) {
+    if (!p.join) return 0;
+    const uint64_t units = (uint64_t)b->n_seqs * kv->n_kv_heads, rounds = (b->max_kv_len + ROUND - 1) / ROUND;
+    uint64_t many = 0;
+    if (p.many) {
+        const uint64_t tokens = kept_tokens(b);
+        many = tokens < MOST_PARTS ? tokens * n_heads : MOST_PARTS;
+        many = many < MOST_PARTS ? (many * rounds + 1) & ~(uint64_t)1 : MOST_PARTS;
+        many = many < MOST_PARTS ? many : MOST_PARTS;
+    }
+    return (few_slots((uint32_t)p.few_blocks, (uint32_t)units) * FEW + many) * (kv->head_dim + 1) * sizeof(float) +
+           units * sizeof(wm_u2);
 }
 
 }  // namespace
@@ -1140,7 +1166,7 @@ extern "C" {
 size_t wm_paged_attention_workspace(const wm_paged_kv *kv, const wm_paged_batch *batch, uint32_t n_heads) {
     if (!kv || !batch || !kv->n_kv_heads || n_heads % kv->n_kv_heads || !sizes_fit(kv, batch, n_heads)) return 0;
     if (batch->n_tokens == 0 || batch->n_seqs == 0 || batch->max_new == 0) return 0;
-    return plan_bytes(make_plan(kv, batch, n_heads), kv, batch);
+    return plan_bytes(make_plan(kv, batch, n_heads), kv, batch, n_heads);
 }
 
 wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch, int type,
@@ -1167,7 +1193,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if (most > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups, %llu rounds of %d positions in one step", who,
                             (unsigned long long)most, (unsigned long long)p.rounds, ROUND);
-    const size_t need = plan_bytes(p, kv, batch);
+    const size_t need = plan_bytes(p, kv, batch, n_heads);
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
                             d_work ? work_bytes : (size_t)0, need);
@@ -1182,7 +1208,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.scale_log2 = scale * 1.4426950408889634f;
     a.few_blocks = (uint32_t)p.few_blocks, a.many_blocks = (uint32_t)p.many_blocks;
     a.many_levels = p.many_levels, a.many_len = p.many_len, a.many_n = p.many_n;
-    a.part_o = (float *)d_work;
+    a.part_o = (float *)d_work, a.parts_by_seq = p.parts_by_seq;
     if (p.join) {
         a.part_lse = a.part_o + p.parts * kv->head_dim;
         a.few_parts = (uint32_t *)(a.part_lse + p.parts);  // FEW rows to a part: an even count

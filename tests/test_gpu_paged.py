@@ -838,3 +838,28 @@ def test_sequences_whose_tokens_break_their_bounds(ctx, cu):
                 assert np.isnan(out.host()[t]).all() and np.isnan(lse.host()[t]).all()
             else:
                 assert np.all(out.host()[t] == 7.0) and np.all(lse.host()[t] == 7.0)
+
+
+@pytest.mark.parametrize("kind,group,pad", [("f32", 4, 0), ("bf16", 20, 0), ("f32", 4, 700)])
+def test_attention_in_the_workspace_of_a_larger_step(ctx, kind, group, pad):
+    """One workspace, sized for the largest step, serves smaller ones: fewer tokens have more splits.  Padding tokens,
+    which no sequence has, take no part in that."""
+    rng = np.random.default_rng(27)
+    big = Step(rng, [(1500, 300), (900, 200), (100, 30)], 32, 1, 64, pad=pad)
+    pool = big.pool(rng)
+    kv = wh.PagedKV(0, 0, 0, 0, big.n_pages, 32, 1, 64)
+    b = wh.PagedBatch(0, 0, 0, 3, big.stride, big.n_tokens, big.max_new, big.max_kv)
+    size = wh.paged_attention_workspace(kv, b, group)
+    for steps in ([(1500, 40), (900, 2), (100, 9)], [(1790, 9)], [(1799, 1), (3, 5)], [(0, 300), (700, 12)]):
+        st = Step(rng, steps, 32, 1, 64, pad=pad)
+        st.table = np.ascontiguousarray(big.table[:len(steps)])
+        st.stride, st.n_pages = big.stride, big.n_pages
+        d = Device(ctx, st, pool)
+        q, qx = typed(ctx, rng, (st.n_tokens, group, 64), kind, 2.0)
+        out, lse = Array.full(ctx, q.shape, 7.0, kind), Array.full(ctx, q.shape[:2], 7.0, "f32")
+        # full of NaN, and some behind it that stays as it is
+        work = Array.full(ctx, (size // 4 + 1000,), np.nan, "f32")
+        ctx.check(wh.lib.wm_paged_attention_dev(ctx.h, d.kv, d.b, wh.DTYPES[kind], q.ptr, group * 64, group, 0.125, out.ptr,
+                                                group * 64, lse.ptr, work.ptr, size))
+        assert_attention(st, pool, kind, qx, out, lse, 0.125)
+        assert np.isnan(work.host()[size // 4:]).all()

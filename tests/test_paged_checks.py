@@ -229,3 +229,27 @@ def test_attention_refuses_more_workgroups_than_a_launch_has(hctx):
     assert attend(hctx, kv, b, heads=4096, qs=4096 * 128, os=4096 * 128) == SHAPE
     kv, b = descriptors(n_seqs=1 << 20, n_kv_heads=16, n_tokens=1 << 20, max_new=64)
     assert attend(hctx, kv, b, heads=64, qs=64 * 128, os=64 * 128) == SHAPE
+
+
+def test_attention_workspace_covers_smaller_steps():
+    """The size falls with no bound: what a server allocates for its largest step serves all others."""
+    rng = np.random.default_rng(0)
+    names = ("n_seqs", "n_tokens", "max_new", "max_kv_len")
+    for turn in range(3000):
+        most = [int(2 ** x) for x in rng.uniform(0, (8, 14, 12, 15))]
+        most[2] = min(most[2], most[1])
+        less = [max(1, int(m * rng.choice([1, 1, rng.random(), rng.random() ** 4]))) for m in most]
+        less[2] = min(less[2], less[1])
+        kvh, group = int(rng.choice([1, 2, 5, 8])), int(rng.choice([1, 4, 8, 33]))
+        sizes = []
+        for bounds in (most, less):
+            kv, b = descriptors(n_kv_heads=kvh, table_stride=1 << 12, **dict(zip(names, bounds)))
+            sizes.append(wh.paged_attention_workspace(kv, b, kvh * group))
+        assert sizes[1] <= sizes[0], (most, less, kvh, group, sizes)
+        assert sizes[0] <= 110_000_000 + 8300 * kvh * most[0]
+    # a long prompt, and the chunk of it that a smaller step has
+    kv, b = descriptors(n_kv_heads=5, n_seqs=1, n_tokens=8192, max_new=8192, max_kv_len=8192, table_stride=512)
+    whole = wh.paged_attention_workspace(kv, b, 20)
+    for n in (2048, 512, 100, 10, 1):
+        b.n_tokens = b.max_new = n
+        assert wh.paged_attention_workspace(kv, b, 20) <= whole
