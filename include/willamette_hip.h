@@ -564,8 +564,9 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
  * logprob and rank must be null.
  * What an output holds does not depend on which others are asked for.
  * vocab is at most 2^30.
- * work: wm_token_logprobs_workspace bytes (0 for one part per row: may be
- * null), 16-byte aligned, as above. */
+ * work: wm_token_logprobs_workspace bytes (0: may be null), 16-byte aligned,
+ * as above; enough for every call of no more rows, no larger a vocabulary and
+ * no more top tokens. */
 size_t wm_token_logprobs_workspace(uint32_t n_rows, uint32_t vocab, uint32_t top_k);
 wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uint64_t row_stride, uint32_t n_rows,
                                 uint32_t vocab, const int32_t *d_tokens, uint32_t top_k, float *d_logprob,

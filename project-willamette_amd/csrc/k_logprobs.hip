@@ -19,6 +19,7 @@
 // are bound by the vector unit, about 7 operations and one exponential per
 // logit: 2047 rows of 50257 in bfloat16 (206 MB) take 57 us.  One row of
 // 128256, in 32 short parts, takes 12.5 us, the length of two launches' chains.
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 
@@ -527,22 +528,36 @@ __global__ __launch_bounds__(64) void k_logprobs_join_rows(lp_args a) {
 // How a row is divided: as few parts as its lanes' registers allow, and of
 // few rows parts a quarter as long.
 constexpr uint32_t LONG_PART = 64 * NT, SHORT_PART = 16 * NT;  // elements, at most
+constexpr uint32_t SMALL = 128;  // long parts of a call up to which it takes short ones
 struct lp_plan {
     bool small;
     uint32_t parts, part_vecs;
 };
+uint32_t most_parts(uint32_t vocab, size_t elem, uint32_t len) {
+    const uint32_t per = (uint32_t)(16 / elem), vecs = (vocab + 2 * per - 2) / per;  // with any skew
+    return (vecs + len / per - 1) / (len / per);
+}
 lp_plan make_plan(uint32_t n_rows, uint32_t vocab, size_t elem) {
     const uint32_t per = (uint32_t)(16 / elem), vecs = (vocab + 2 * per - 2) / per;  // with any skew
     lp_plan p;
-    p.small = (uint64_t)n_rows * ((vocab + LONG_PART - 1) / LONG_PART) <= 128;
-    const uint32_t most = (p.small ? SHORT_PART : LONG_PART) / per;
-    p.parts = (vecs + most - 1) / most;
+    p.small = (uint64_t)n_rows * ((vocab + LONG_PART - 1) / LONG_PART) <= SMALL;
+    p.parts = most_parts(vocab, elem, p.small ? SHORT_PART : LONG_PART);
     p.part_vecs = ((vecs + p.parts - 1) / p.parts + NT - 1) / NT * NT;  // of whole rounds, but for the last
     p.parts = (vecs + p.part_vecs - 1) / p.part_vecs;
     return p;
 }
-size_t plan_bytes(uint32_t n_rows, const lp_plan &p, uint32_t top_k) {
-    return p.parts > 1 ? (size_t)n_rows * p.parts * (sizeof(lp_part) + 8 * (size_t)top_k) : 0;
+// Parts of a call, of any type, and of every one of fewer rows or a smaller
+// vocabulary, which may take short parts where this one does not.  With c long
+// parts of a row, c * n_rows <= SMALL, a row has 4 c + 1 short ones at most:
+// 5 SMALL of the call.
+size_t kept_parts(uint32_t n_rows, uint32_t vocab) {
+    size_t n = 0;
+    for (size_t elem = 2; elem <= 4; elem *= 2) {
+        const size_t few = most_parts(vocab, elem, SHORT_PART), many = most_parts(vocab, elem, LONG_PART);
+        if (few > 1) n = std::max(n, std::min<size_t>(n_rows * few, 5 * SMALL));
+        if (many > 1) n = std::max(n, n_rows * many);
+    }
+    return n;
 }
 
 template <typename T>
@@ -561,10 +576,7 @@ extern "C" {
 
 size_t wm_token_logprobs_workspace(uint32_t n_rows, uint32_t vocab, uint32_t top_k) {
     if (n_rows == 0 || vocab == 0 || vocab > MAX_VOCAB || top_k > MAX_TOP) return 0;
-    // of any type: f32 has the most parts
-    const size_t a = plan_bytes(n_rows, make_plan(n_rows, vocab, 4), top_k);
-    const size_t b = plan_bytes(n_rows, make_plan(n_rows, vocab, 2), top_k);
-    return a > b ? a : b;
+    return kept_parts(n_rows, vocab) * (sizeof(lp_part) + 8 * (size_t)top_k);
 }
 
 wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uint64_t row_stride, uint32_t n_rows,
@@ -593,11 +605,11 @@ wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uin
         ((uintptr_t)d_tokens | (uintptr_t)d_logprob | (uintptr_t)d_entropy | (uintptr_t)d_rank | (uintptr_t)d_top_ids |
          (uintptr_t)d_top_logprobs) % 4)
         return wm_set_error(ctx, WM_E_ARG, "%s: misaligned pointer", who);
-    const size_t need = wm_token_logprobs_workspace(n_rows, vocab, top_k);
+    const lp_plan p = make_plan(n_rows, vocab, elem);
+    const size_t need = p.parts > 1 ? wm_token_logprobs_workspace(n_rows, vocab, top_k) : 0;
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
                             d_work ? work_bytes : (size_t)0, need);
-    const lp_plan p = make_plan(n_rows, vocab, elem);
     lp_args a;
     memset(&a, 0, sizeof a);
     a.x = d_logits, a.stride = row_stride, a.n_rows = n_rows, a.vocab = vocab;

@@ -252,3 +252,22 @@ def test_logprobs_do_not_depend_on_what_else_is_asked(ctx):
     a, b, one = run(ctx, x, tok, 0), run(ctx, x, tok, 9), run(ctx, x[3:4], tok[3:4], 0)
     assert all(np.array_equal(p, q) for p, q in zip(a[:3], b[:3]))
     assert one[2][0] == a[2][3]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_logprobs_in_the_workspace_of_a_larger_call(ctx, kind):
+    """The workspace of many rows serves few, which are divided into more parts; nothing behind it is written."""
+    rng = np.random.default_rng(11)
+    rows, vocab, k = 60, 50001, 9
+    size = wh.token_logprobs_workspace(rows, vocab, k)
+    work = Array(ctx, np.full(size // 4 + 100, np.nan, np.float32))
+    for n, v in ((rows, vocab), (32, vocab), (31, vocab), (1, vocab), (rows, 16385), (rows, 4097), (rows, 100), (128, 16000)):
+        x = to_kind(rng.standard_normal((n, v)) * 3, kind)
+        tok = rng.integers(0, v, n).astype(np.int32)
+        out = outputs(ctx, n, k)
+        if n <= rows:
+            score(ctx, Array(ctx, x, kind), kind, 0, v, n, v, Array(ctx, tok), k, out, work, size)
+            check([o.host() for o in out], from_kind(x, kind), tok, k)
+            assert np.isnan(work.host()[size // 4:]).all()
+        # its own size is enough too
+        check(run(ctx, x, tok, k, kind), from_kind(x, kind), tok, k)

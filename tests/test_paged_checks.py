@@ -253,3 +253,14 @@ def test_attention_workspace_covers_smaller_steps():
     for n in (2048, 512, 100, 10, 1):
         b.n_tokens = b.max_new = n
         assert wh.paged_attention_workspace(kv, b, 20) <= whole
+
+
+def test_logprobs_workspace_covers_smaller_calls():
+    """Few rows are taken in short parts, many in long ones: what serves many serves few."""
+    rng = np.random.default_rng(1)
+    for turn in range(5000):
+        most = [int(2 ** x) for x in rng.uniform(0, (11, 18))] + [int(rng.integers(0, 65))]
+        less = [max(1, int(m * rng.choice([1, 1, rng.random()]))) for m in most[:2]] + [int(rng.integers(0, most[2] + 1))]
+        assert wh.token_logprobs_workspace(*less) <= wh.token_logprobs_workspace(*most), (most, less)
+    for rows in range(1, 700):
+        assert wh.token_logprobs_workspace(rows, 128256, 20) <= wh.token_logprobs_workspace(rows + 1, 128256, 20), rows
