@@ -329,11 +329,15 @@ _CTX = []
 
 
 def _lib():
-    """The library and the program's one context."""
+    """The library and the program's one context, whose stream torch then works on too, so that what either enqueues
+    is in order; what torch had enqueued before is waited for."""
     if not _CTX:
         sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "project-willamette_amd"))
         import willamette_hip as wh
-        _CTX.extend([wh, wh.Context(0)])
+        ctx = wh.Context(0)
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(torch.cuda.ExternalStream(ctx.stream))
+        _CTX.extend([wh, ctx])
     return _CTX
 
 
