@@ -863,3 +863,20 @@ def test_attention_in_the_workspace_of_a_larger_step(ctx, kind, group, pad):
                                                 group * 64, lse.ptr, work.ptr, size))
         assert_attention(st, pool, kind, qx, out, lse, 0.125)
         assert np.isnan(work.host()[size // 4:]).all()
+
+
+# ---------------------------------------------------------------------------
+# sequences of few rows in more rounds of 256 positions than workgroups: every
+# wave has several tiles, runs end inside a sequence's head and span several
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind,page,kh,group,steps", [
+    ("f32", 16, 8, 2, [(20000, 1), (9001, 3), (254, 1), (3000, 8), (0, 1), (255, 1), (256, 1)]),
+    ("bf16", 64, 16, 1, [(9000, 16), (0, 0), (255, 1), (8191, 1), (700, 2), (5, 1)])])
+def test_attention_of_more_rounds_than_workgroups(ctx, kind, page, kh, group, steps):
+    rng = np.random.default_rng(28)
+    st = Step(rng, steps, page, kh, 64, pad=1)
+    assert kh * sum(-(-(c + n) // 256) for c, n in steps if n) > 1024
+    pool = st.pool(rng)
+    _, _, qx, out, lse, scale = attention_case(ctx, kind, st, pool, rng, kh * group)
+    assert_attention(st, pool, kind, qx, out, lse, scale)
