@@ -276,6 +276,9 @@ struct row_scale {
     }
     __device__ __forceinline__ float operator()(float o) const { return ldexpf(o * inv, e); }
 };
+// Parts of a row are joined under weights 2^x, applied as two factors: a
+// part far below the others in its sum may be as far above them in its values.
+__device__ __forceinline__ float half_weight(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
 // The exponent that a query row is scaled by (rows below 2^-100 are taken as
 // if they reached it: the factor stays finite).
 __device__ __forceinline__ int query_exponent(float most) { return max(__builtin_amdgcn_frexp_expf(most), -100); }
@@ -556,9 +559,9 @@ __device__ __forceinline__ void attend_few_part(const attn_args &a, const wm_seq
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float e = __builtin_amdgcn_exp2f(ls[w] - base);
-            sum += e;
-            v += *(const wm_f4 *)&sh.o[w][row][c] * e;
+            const float e = half_weight(ls[w] - base);
+            sum += e * e;
+            v += *(const wm_f4 *)&sh.o[w][row][c] * e * e;
         }
         if (sum != 0.0f) v *= 1.0f / sum;
         const float lse2 = sum == 0.0f ? -INFINITY : base + __builtin_amdgcn_logf(sum);
@@ -1068,13 +1071,13 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
                 if (s0 + s >= n) z[s] = -INFINITY;
                 m = fmaxf(m, z[s]);
             }
-            const float to = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(top - to);
-            sum *= alpha, v *= alpha, top = m;
+            const float to = m == -INFINITY ? 0.0f : m, alpha = half_weight(top - to);
+            sum *= alpha * alpha, v *= alpha, v *= alpha, top = m;
 #pragma unroll
             for (int s = 0; s < 8; s++) {
-                const float e = __builtin_amdgcn_exp2f(z[s] - to);
-                sum += e;
-                v += x[s] * e;
+                const float e = half_weight(z[s] - to);
+                sum += e * e;
+                v += x[s] * e * e;
             }
         }
         const float base = top == -INFINITY ? 0.0f : top;

@@ -880,3 +880,26 @@ def test_attention_of_more_rounds_than_workgroups(ctx, kind, page, kh, group, st
     pool = st.pool(rng)
     _, _, qx, out, lse, scale = attention_case(ctx, kind, st, pool, rng, kh * group)
     assert_attention(st, pool, kind, qx, out, lse, scale)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("step", [12, -12, 40])
+def test_attention_of_rounds_under_rising_scales(ctx, kind, step):
+    """Round i of 256 positions has values of 2^(step i) under scores of -step i bits: each round that is kept counts as
+    much as the others, at the ordinary tolerance.  (Falling scales stay within 2^-60 of the largest for five rounds, and
+    the keys behind them are out of reach.)"""
+    rng = np.random.default_rng(29)
+    st = Step(rng, [(1279, 1)] * 5, 16, 48, 64)
+    kc, vc, ks, vs = pool = st.pool(rng)
+    kc[:], ks[:] = 0, 1.0
+    for s in range(5):
+        for lp in range(80):
+            page, i = st.table[s, lp], lp // 16
+            kc[page, :, :, 0] = rng.integers(112, 125, (48, 16)) * -np.sign(step)
+            ks[page], vs[page] = abs(step) * i * np.log(2.0) / 120, 2.0 ** (step * i - 60)
+    q = np.zeros((5, 48, 64), np.float32)
+    q[..., 0] = 1.0
+    q = Array(ctx, to_kind(q, kind), kind)
+    out, lse = Array.full(ctx, q.shape, 7.0, kind), Array.full(ctx, q.shape[:2], 7.0, "f32")
+    Device(ctx, st, pool).attend(kind, q, out, lse, 1.0)
+    assert_attention(st, pool, kind, q.values(), out, lse, 1.0)
