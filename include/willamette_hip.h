@@ -530,8 +530,9 @@ wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_page
  *   s_j = scale * q . k_j (j <= p),  out = sum_j softmax(s)_j v_j,
  *   lse = ln sum_j exp(s_j)  (d_lse [n_tokens][n_heads] f32, nullable).
  * Queries count with 22 bits and more of their row's largest (f32) or
- * exactly (f16, bf16: to 2^-28 of it), softmax weights with 22 bits (f32) or
- * 11, sums in f32; a block whose value scale is less than 2^-60 of the
+ * exactly (f16, bf16: to 2^-28 of it); products of a softmax weight and a
+ * block's value scale with 22 bits (f32) or 11, and to 2^-31 of the row's
+ * largest; sums in f32; a block whose value scale is less than 2^-60 of the
  * largest of the blocks that its row attends to counts as if it were that.
  * What a row gives does not depend on what the positions behind it hold.
  * A row without positions gives 0 and lse -inf.  A row that reads a page

@@ -4,6 +4,7 @@
 // one for V.  One workgroup serves one block of one sequence: it owns the
 // block for the launch (two sequences may not append into one page), so the
 // maximum, the codes and the scale need no exchange between workgroups.
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <new>
@@ -106,11 +107,13 @@ struct append_args {
     uint64_t qs, ks, vs, qos;  // elements between tokens
     uint32_t group;            // query heads per kv head (0: no queries)
     uint32_t touch;            // pages a sequence can touch, at most
-    uint32_t blocks;           // of all sequences, at most
+    uint32_t seq0;             // the launch's first sequence
+    uint32_t blocks;           // of the launch's sequences, at most
     bool by_kind;              // order of the workgroups (k_paged_append)
 };
 
-// One block's place in the step: sequence s, its page lp, kv head h.
+// One block's place in the step: sequence s, its page lp, kv head h, of a
+// launch's id-th from sequence seq0 on.
 struct block_place {
     wm_seq q;
     int lp, h, page;
@@ -119,10 +122,10 @@ struct block_place {
     __device__ __forceinline__ bool stored() const { return (uint32_t)page < n_pages; }  // its page is in the pool
 };
 __device__ __forceinline__ block_place place_block(const wm_paged_kv &kv, const wm_paged_batch &b, uint32_t touch,
-                                                   uint32_t id) {
+                                                   uint32_t seq0, uint32_t id) {
     block_place p;
     p.h = id % kv.n_kv_heads;
-    const uint32_t sm = id / kv.n_kv_heads, s = sm / touch;
+    const uint32_t sm = id / kv.n_kv_heads, s = seq0 + sm / touch;
     p.q = wm_load_seq(b, s);
     p.lp = max(p.q.start, 0) / (int)kv.page_size + (int)(sm % touch);
     p.live = p.q.ok && p.q.n > 0 && (int64_t)p.lp * kv.page_size < p.q.len;
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
     if (a.by_kind) kind = blockIdx.x / a.blocks, id = blockIdx.x % a.blocks;
     else if (a.group) kind = blockIdx.x % (2 + PS / 16), id = blockIdx.x / (2 + PS / 16);
     else kind = blockIdx.x % 2, id = blockIdx.x / 2;
-    const block_place p = place_block(a.kv, a.b, a.touch, id);
+    const block_place p = place_block(a.kv, a.b, a.touch, a.seq0, id);
     if (!p.live) return;
     const int base = p.lp * PS;  // first position of the page
     const int first = max(max(p.q.start, 0) - base, 0), hi = min(p.q.len - base, PS);  // its new slots
@@ -350,7 +353,7 @@ struct read_args {
     wm_paged_batch b;
     void *k, *v;
     uint64_t ks, vs;
-    uint32_t touch;
+    uint32_t touch, seq0;
 };
 
 __device__ __forceinline__ wm_f4 values4(uint32_t w, float s) {
@@ -361,7 +364,7 @@ __device__ __forceinline__ wm_f4 values4(uint32_t w, float s) {
 // rows are a dword each, V's transposed through the unit's 16 bytes.
 template <typename T, int PS, int D>
 __global__ __launch_bounds__(NT) void k_paged_read(read_args a) {
-    const block_place p = place_block(a.kv, a.b, a.touch, blockIdx.x);
+    const block_place p = place_block(a.kv, a.b, a.touch, a.seq0, blockIdx.x);
     if (!p.live) return;
     const int base = p.lp * PS, first = max(max(p.q.start, 0) - base, 0), hi = min(p.q.len - base, PS);
     const int64_t tok = (int64_t)p.q.tok0 + base - p.q.start;
@@ -404,11 +407,14 @@ uint32_t touched_pages(const wm_paged_kv *kv, const wm_paged_batch *b) {
     const uint64_t most = b->max_new < b->max_kv_len ? b->max_new : b->max_kv_len;
     return most ? (uint32_t)((most + 2 * kv->page_size - 2) / kv->page_size) : 0;
 }
-wm_status block_grid(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t *grid) {
-    const uint64_t n = (uint64_t)touched_pages(kv, b) * b->n_seqs * kv->n_kv_heads;
-    if (n > 0x7FFFFFFFull / NT / 6)  // the launch counts threads in 32 bits, and an append has up to six workgroups a block
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu blocks in one step", who, (unsigned long long)n);
-    *grid = (uint32_t)n;
+// Sequences of one launch, which counts threads in 32 bits; an append has up
+// to six workgroups a block.  Many sequences next to a long one take several
+// launches: the host knows no lengths, only their bound.
+wm_status launch_seqs(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t *seqs) {
+    const uint64_t one = (uint64_t)touched_pages(kv, b) * kv->n_kv_heads, most = 0x7FFFFFFFull / NT / 6;
+    if (one > most || b->n_seqs > most)
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %u sequences of up to %llu blocks", who, b->n_seqs, (unsigned long long)one);
+    *seqs = one ? (uint32_t)(most / one) : 0;
     return WM_OK;
 }
 
@@ -572,13 +578,16 @@ wm_status wm_paged_kv_append_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.qs = q_stride, a.ks = k_stride, a.vs = v_stride, a.qos = q_out_stride;
     a.group = n_heads / kv->n_kv_heads;
     a.touch = touched_pages(kv, batch);
-    uint32_t grid;
-    if ((st = block_grid(ctx, who, kv, batch, &grid))) return st;
-    if (!grid) return WM_OK;
+    uint32_t seqs;
+    if ((st = launch_seqs(ctx, who, kv, batch, &seqs))) return st;
+    if (!seqs) return WM_OK;
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
-    by_shape<launch_append>(type, kv->page_size, kv->head_dim, a, grid, ctx->stream);
-    WM_HIP(ctx, hipGetLastError());
+    for (uint32_t left; a.seq0 < batch->n_seqs; a.seq0 += left) {
+        left = std::min(seqs, batch->n_seqs - a.seq0);
+        by_shape<launch_append>(type, kv->page_size, kv->head_dim, a, left * a.touch * kv->n_kv_heads, ctx->stream);
+        WM_HIP(ctx, hipGetLastError());
+    }
     return WM_OK;
 }
 
@@ -595,14 +604,17 @@ wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_page
         return st;
     if (d_v_out && (st = wm_paged_check_array(ctx, who, "v_out", d_v_out, v_stride, kv->n_kv_heads, kv->head_dim, elem)))
         return st;
-    read_args a{*kv, *batch, d_k_out, d_v_out, k_stride, v_stride, touched_pages(kv, batch)};
-    uint32_t grid;
-    if ((st = block_grid(ctx, who, kv, batch, &grid))) return st;
-    if (!grid) return WM_OK;
+    read_args a{*kv, *batch, d_k_out, d_v_out, k_stride, v_stride, touched_pages(kv, batch), 0};
+    uint32_t seqs;
+    if ((st = launch_seqs(ctx, who, kv, batch, &seqs))) return st;
+    if (!seqs) return WM_OK;
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
-    by_shape<launch_read>(type, kv->page_size, kv->head_dim, a, grid, ctx->stream);
-    WM_HIP(ctx, hipGetLastError());
+    for (uint32_t left; a.seq0 < batch->n_seqs; a.seq0 += left) {
+        left = std::min(seqs, batch->n_seqs - a.seq0);
+        by_shape<launch_read>(type, kv->page_size, kv->head_dim, a, left * a.touch * kv->n_kv_heads, ctx->stream);
+        WM_HIP(ctx, hipGetLastError());
+    }
     return WM_OK;
 }
 

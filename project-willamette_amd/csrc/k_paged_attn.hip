@@ -28,6 +28,7 @@
 // to 421 us, 820 TFLOP/s of products: a wave's exponentials, conversions and
 // masks take about as long as its products, two waves on a SIMD overlap them
 // in part.  16 sequences of 1 to 32 rows over up to 4064 positions, f32, 46 us.
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 
@@ -1025,13 +1026,14 @@ __global__ __launch_bounds__(NT, 2) void k_paged_attn_many(attn_args a) {
 }
 
 // The rows' parts joined: weights 2^(lse - max), one thread per four dims;
-// one workgroup per FEW rows of a sequence and kv head.
+// one workgroup per FEW rows of a sequence (of the launch's, from seq0 on) and
+// kv head.
 template <int D>
-__global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t chunks) {
+__global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t chunks, uint32_t seq0) {
     uint32_t id = blockIdx.x;
     const uint32_t chunk = id % chunks;
     id /= chunks;
-    const uint32_t s = id / a.kv.n_kv_heads, h = id % a.kv.n_kv_heads;
+    const uint32_t s = seq0 + id / a.kv.n_kv_heads, h = id % a.kv.n_kv_heads;
     const uint32_t unit = s * a.kv.n_kv_heads + h;
     const wm_u2 parts = a.few_blocks ? *(const wm_u2 *)(a.few_parts + 2 * unit) : wm_u2{0, 0};  // where its rows are few
     const row_tile t = load_tile(a, s, h, chunk / (MANY / FEW), MANY);
@@ -1093,7 +1095,7 @@ __global__ __launch_bounds__(NT) void k_paged_attn_join(attn_args a, uint32_t ch
 struct attn_plan {
     bool many;         // a sequence may have more than FEW rows
     uint32_t many_levels, many_len, many_n;
-    uint64_t few_blocks, many_blocks, join_blocks;
+    uint64_t few_blocks, many_blocks;
     uint32_t join_chunks;  // of a sequence and kv head
     bool join;
     size_t parts;      // partial rows
@@ -1135,7 +1137,6 @@ attn_plan make_plan(const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t n_h
             p.join_chunks = (uint32_t)most * (MANY / FEW);
         }
     }
-    p.join_blocks = p.join ? units * p.join_chunks : 0;
     return p;
 }
 
@@ -1192,10 +1193,14 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
         return wm_set_error(ctx, WM_E_SHAPE, "%s: max_new %u or max_kv_len %u is too large for %u heads over %u", who,
                             batch->max_new, batch->max_kv_len, n_heads, kv->n_kv_heads);
     const attn_plan p = make_plan(kv, batch, n_heads);
-    const uint64_t most = p.few_blocks + p.many_blocks > p.join_blocks ? p.few_blocks + p.many_blocks : p.join_blocks;
-    if (most > 0x7FFFFFFFull / NT || p.rounds > 0x3FFFFFFF)  // the launch counts threads in 32 bits
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups, %llu rounds of %d positions in one step", who,
-                            (unsigned long long)most, (unsigned long long)p.rounds, ROUND);
+    // A launch counts threads in 32 bits.  The join, which has a workgroup for
+    // every FEW rows that any sequence may have, takes some sequences at a time.
+    const uint64_t most = 0x7FFFFFFFull / NT, blocks = p.few_blocks + p.many_blocks;
+    const uint64_t seq_blocks = (uint64_t)kv->n_kv_heads * p.join_chunks, units = (uint64_t)kv->n_kv_heads * batch->n_seqs;
+    if (blocks > most || p.rounds > 0x3FFFFFFF || (p.join && (seq_blocks > most || units > most)))
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %llu workgroups, %llu rounds of %d positions, %u sequences of up to %llu "
+                            "joins in one step", who, (unsigned long long)blocks, (unsigned long long)p.rounds, ROUND,
+                            batch->n_seqs, (unsigned long long)seq_blocks);
     const size_t need = plan_bytes(p, kv, batch, n_heads);
     if (need && (!d_work || work_bytes < need || (uintptr_t)d_work % 16))
         return wm_set_error(ctx, WM_E_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who,
@@ -1218,7 +1223,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     }
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
-    const uint32_t grid = (uint32_t)(p.few_blocks + p.many_blocks);
+    const uint32_t grid = (uint32_t)blocks;
     hipStream_t s = ctx->stream;
     const bool two = type == WM_DTYPE_F32;
 #define WM_ATTEND(D_)                                                                  \
@@ -1232,10 +1237,11 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     else WM_ATTEND(128);
 #undef WM_ATTEND
     WM_HIP(ctx, hipGetLastError());
-    if (p.join) {
-        const uint32_t g = (uint32_t)p.join_blocks;
-        if (kv->head_dim == 64) k_paged_attn_join<64><<<g, NT, 0, s>>>(a, p.join_chunks);
-        else k_paged_attn_join<128><<<g, NT, 0, s>>>(a, p.join_chunks);
+    for (uint32_t s0 = 0, n; p.join && s0 < batch->n_seqs; s0 += n) {
+        n = (uint32_t)std::min<uint64_t>(batch->n_seqs - s0, most / seq_blocks);
+        const uint32_t g = (uint32_t)(n * seq_blocks);
+        if (kv->head_dim == 64) k_paged_attn_join<64><<<g, NT, 0, s>>>(a, p.join_chunks, s0);
+        else k_paged_attn_join<128><<<g, NT, 0, s>>>(a, p.join_chunks, s0);
         WM_HIP(ctx, hipGetLastError());
     }
     return WM_OK;

@@ -903,3 +903,57 @@ def test_attention_of_rounds_under_rising_scales(ctx, kind, step):
     out, lse = Array.full(ctx, q.shape, 7.0, kind), Array.full(ctx, q.shape[:2], 7.0, "f32")
     Device(ctx, st, pool).attend(kind, q, out, lse, 1.0)
     assert_attention(st, pool, kind, q.values(), out, lse, 1.0)
+
+
+def weight_steps(st, pool, heads):
+    """What the steps of small weights can add to an output, beside the 22 bits that the tolerance counts.
+
+    A weight w, relative to a largest one of 2^7 or more, is two f16 terms: h, cut to 11 bits, and w - h.  Below 2^-14
+    f16 has steps of 2^-24, so rounding either is off by up to 2^-25, together 2^-24, or 2^-31 of the largest.  A weight
+    holds its block's value scale: the largest is at most the row's largest scale, as softmax weights are at most 1, and
+    the output's error at most 2^-31 of that times the sum of the codes' sizes."""
+    tol = np.zeros((st.n_tokens, heads, st.dim))
+    for s in range(len(st.steps)):
+        pages = st.table[s, :-(-int(st.kv_len[s]) // st.page)]
+        for h in range(heads):
+            hk = h // (heads // st.kh)
+            codes = np.abs(pool[1][pages, hk].astype(np.int64)).sum((0, 2)) if len(pages) else 0
+            tol[st.cu[s]:st.cu[s + 1], h] = 2.0 ** -31 * codes * (pool[3][pages, hk].max() if len(pages) else 0)
+    return tol
+
+
+def test_many_sequences_next_to_a_long_bound(ctx):
+    """520 sequences of few tokens in a step whose bound is 8192 each: more blocks and joined rows than one launch counts,
+    though hardly any exist."""
+    rng = np.random.default_rng(30)
+    kh, group, dim, bound = 8, 4, 64, 8192
+    steps = [(int(rng.integers(0, 40)), 1) for _ in range(520)]
+    steps[3], steps[517], steps[519] = (300, 150), (500, 30), (900, 1)
+    st = Step(rng, steps, 16, kh, dim, extra_stride=bound // 16)
+    st.n_tokens, st.max_new, st.max_kv = bound, bound, bound
+    pool = st.pool(rng)
+    expect = [a.copy() for a in pool]
+    used = int(st.cu[-1])
+    q, qx = typed(ctx, rng, (bound, kh * group, dim), "f32", 2.0)
+    k, kx = typed(ctx, rng, (bound, kh, dim), "f32")
+    q_out, out = (Array.full(ctx, q.shape, 7.0, "f32") for _ in range(2))
+    ko = Array.full(ctx, k.shape, 7.0, "f32")
+    lse = Array.full(ctx, q.shape[:2], 7.0, "f32")
+    d = Device(ctx, st, pool)
+    d.append("f32", q, k, k, q_out)
+    d.read("f32", ko, None)
+    d.attend("f32", q, out, lse, 0.125)
+    ref.append(st, expect, qx, kx, kx, None, None, 0)
+    assert all(same_bits(a, b) for a, b in zip(d.host_pool(), expect))
+    assert np.array_equal(q_out.host()[:used], q.host()[:used]) and np.all(q_out.host()[used:] == 7.0)
+    got = ko.host()
+    assert np.all(got[used:] == 7.0)
+    for s in (0, 3, 300, 517, 519):
+        for h in (0, 7):
+            want = ref.values(st, expect, s, int(st.kv_len[s]), h)[0][steps[s][0]:]
+            assert np.array_equal(got[st.cu[s]:st.cu[s + 1], h], want.astype(np.float32))
+    o, z, tol, tol_z = ref.attention(st, expect, qx, 0.125, "f32")
+    tol += weight_steps(st, expect, kh * group)
+    assert np.all(np.abs(out.host()[:used] - o[:used]) <= tol[:used])
+    assert np.all(np.abs(lse.host()[:used] - z[:used]) <= tol_z[:used])
+    assert np.all(out.host()[used:] == 7.0) and np.all(lse.host()[used:] == 7.0)
