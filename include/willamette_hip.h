@@ -494,7 +494,7 @@ wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batc
  * queries.  q [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads]
  * [head_dim] of `type` (wm_dtype), tokens q_stride, k_stride and v_stride
  * elements apart (parts of one fused row are fine); q_out like q (may be q
- * itself).  n_heads = 0: no queries (q and q_out may be null).  rope null: no
+ * itself, with q's stride).  n_heads = 0: no queries (q and q_out may be null).  rope null: no
  * rotation.  Pointers are 16-byte aligned and strides a multiple of 16 bytes.
  *
  * With r the rotated key (exact products and sum, rounded once to f32) or

@@ -500,6 +500,14 @@ wm_status wm_paged_check_array(wm_ctx *ctx, const char *who, const char *name, c
     return WM_OK;
 }
 
+wm_status wm_paged_check_over(wm_ctx *ctx, const char *who, const void *q, uint64_t q_stride, const void *out,
+                              uint64_t out_stride) {
+    if (q == out && q_stride != out_stride)
+        return wm_set_error(ctx, WM_E_ARG, "%s: the output over q has rows %llu apart, not %llu", who,
+                            (unsigned long long)out_stride, (unsigned long long)q_stride);
+    return WM_OK;
+}
+
 extern "C" {
 
 wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *b, const int32_t *cu_tokens,
@@ -572,6 +580,7 @@ wm_status wm_paged_kv_append_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if (n_heads) {
         if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
         if ((st = wm_paged_check_array(ctx, who, "q_out", d_q_out, q_out_stride, n_heads, kv->head_dim, elem))) return st;
+        if ((st = wm_paged_check_over(ctx, who, d_q, q_stride, d_q_out, q_out_stride))) return st;
     }
     a.kv = *kv, a.b = *batch;
     a.q = d_q, a.k = d_k, a.v = d_v, a.q_out = d_q_out;

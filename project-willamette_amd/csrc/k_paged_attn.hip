@@ -1188,6 +1188,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if (batch->n_tokens == 0 || batch->n_seqs == 0 || batch->max_new == 0) return WM_OK;
     if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
     if ((st = wm_paged_check_array(ctx, who, "out", d_out, out_stride, n_heads, kv->head_dim, elem))) return st;
+    if ((st = wm_paged_check_over(ctx, who, d_q, q_stride, d_out, out_stride))) return st;
     if ((uintptr_t)d_lse % 4) return wm_set_error(ctx, WM_E_ARG, "%s: misaligned lse", who);
     if (!sizes_fit(kv, batch, n_heads))
         return wm_set_error(ctx, WM_E_SHAPE, "%s: max_new %u or max_kv_len %u is too large for %u heads over %u", who,

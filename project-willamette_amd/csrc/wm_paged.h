@@ -70,6 +70,9 @@ wm_status wm_paged_check(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, co
 // One packed array: `heads` heads of head_dim values per token, tokens `stride` apart.
 wm_status wm_paged_check_array(wm_ctx *ctx, const char *who, const char *name, const void *p, uint64_t stride,
                                uint32_t heads, uint32_t head_dim, size_t elem);
+// An output over its own queries: only with their stride.
+wm_status wm_paged_check_over(wm_ctx *ctx, const char *who, const void *q, uint64_t q_stride, const void *out,
+                              uint64_t out_stride);
 // Makes the context's device current for the call and the caller's again at its end.
 struct wm_device_guard {
     int before = -1;

@@ -264,3 +264,11 @@ def test_logprobs_workspace_covers_smaller_calls():
         assert wh.token_logprobs_workspace(*less) <= wh.token_logprobs_workspace(*most), (most, less)
     for rows in range(1, 700):
         assert wh.token_logprobs_workspace(rows, 128256, 20) <= wh.token_logprobs_workspace(rows + 1, 128256, 20), rows
+
+
+def test_output_over_its_queries_has_their_stride(hctx):
+    """With another stride a row's output would fall on queries that are still to be read."""
+    kv, b = descriptors()
+    for call in (append, attend):
+        assert call(hctx, kv, b, qs=1024, os=1040) == ARG
+        assert call(hctx, kv, b, qs=1040, os=1024) == ARG
