@@ -538,7 +538,8 @@ wm_status wm_paged_kv_read_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_page
  * A row without positions gives 0 and lse -inf.  A row that reads a page
  * outside the pool, or a sequence whose lengths break their bounds, gives NaN.
  * q and out are of `type`, as in the append; out may be q, with q's stride.
- * Up to 2^30 query rows (max_new * group) and positions * group.
+ * Up to 2^30 query rows (max_new * group) and positions * group; |scale| up
+ * to 2.3e38.
  * work: wm_paged_attention_workspace bytes, 16-byte aligned, overwritten;
  * calls that may run at the same time (graphs replayed on two streams) need
  * one each.  The size goes by the batch's host bounds (n_seqs, n_tokens,

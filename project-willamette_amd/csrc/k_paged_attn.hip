@@ -1184,7 +1184,8 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     if (!elem) return wm_set_error(ctx, WM_E_UNSUPPORTED_TYPE, "%s: type %d is not F32, F16 or BF16", who, type);
     if (n_heads == 0 || n_heads % kv->n_kv_heads || n_heads > 1u << 20)
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %u query heads over %u kv heads", who, n_heads, kv->n_kv_heads);
-    if (!(scale - scale == 0.0f)) return wm_set_error(ctx, WM_E_NONFINITE, "%s: scale %g", who, (double)scale);
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!(scale_log2 - scale_log2 == 0.0f)) return wm_set_error(ctx, WM_E_NONFINITE, "%s: scale %g", who, (double)scale);
     if (batch->n_tokens == 0 || batch->n_seqs == 0 || batch->max_new == 0) return WM_OK;
     if ((st = wm_paged_check_array(ctx, who, "q", d_q, q_stride, n_heads, kv->head_dim, elem))) return st;
     if ((st = wm_paged_check_array(ctx, who, "out", d_out, out_stride, n_heads, kv->head_dim, elem))) return st;
@@ -1214,7 +1215,7 @@ wm_status wm_paged_attention_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_pa
     a.n_heads = n_heads, a.group = n_heads / kv->n_kv_heads;
     a.few_recip = (0x10000 + a.group - 1) / a.group;
     a.type = type;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     a.few_blocks = (uint32_t)p.few_blocks, a.many_blocks = (uint32_t)p.many_blocks;
     a.many_levels = p.many_levels, a.many_len = p.many_len, a.many_n = p.many_n;
     a.part_o = (float *)d_work, a.parts_by_seq = p.parts_by_seq;

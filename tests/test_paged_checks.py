@@ -272,3 +272,10 @@ def test_output_over_its_queries_has_their_stride(hctx):
     for call in (append, attend):
         assert call(hctx, kv, b, qs=1024, os=1040) == ARG
         assert call(hctx, kv, b, qs=1040, os=1024) == ARG
+
+
+def test_attention_refuses_a_scale_without_a_base_2_form(hctx):
+    """Scores are formed in base 2: scale * log2 e has to be finite too."""
+    kv, b = descriptors()
+    for s in (2.4e38, -3.4e38):
+        assert attend(hctx, kv, b, scale=s) == NONFINITE
