@@ -570,6 +570,24 @@ void launch(const lp_args &a, const lp_plan &p, hipStream_t s) {
     else k_logprobs_join<T><<<a.n_rows, NT, 0, s>>>(a);
 }
 
+constexpr char who[] = "token_logprobs";
+wm_status check_sizes(wm_ctx *ctx, size_t elem, uint32_t n_rows, uint32_t vocab, uint32_t top_k) {
+    if (vocab == 0 || vocab > MAX_VOCAB) return wm_set_error(ctx, WM_E_SHAPE, "%s: vocabulary of %u", who, vocab);
+    if ((uint64_t)n_rows * make_plan(n_rows, vocab, elem).parts > 0x7FFFFFFFu / NT)  // the launch counts threads in 32 bits
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: %u rows of %u", who, n_rows, vocab);
+    if (top_k > MAX_TOP || top_k > vocab)
+        return wm_set_error(ctx, WM_E_SHAPE, "%s: top_k %u of %u tokens, %u at most", who, top_k, vocab, MAX_TOP);
+    return WM_OK;
+}
+wm_status check_outputs(wm_ctx *ctx, uint32_t top_k, const void *tokens, const void *logprob, const void *rank,
+                        const void *top_ids, const void *top_logprobs) {
+    if (!top_k && (top_ids || top_logprobs))
+        return wm_set_error(ctx, WM_E_ARG, "%s: outputs for the top tokens with top_k 0", who);
+    if (!tokens && (logprob || rank))
+        return wm_set_error(ctx, WM_E_ARG, "%s: log probabilities or ranks of no tokens", who);
+    return WM_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -583,22 +601,14 @@ wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uin
                                 uint32_t vocab, const int32_t *d_tokens, uint32_t top_k, float *d_logprob,
                                 float *d_entropy, int32_t *d_rank, int32_t *d_top_ids, float *d_top_logprobs,
                                 void *d_work, size_t work_bytes) {
-    static const char who[] = "token_logprobs";
     if (!ctx) return WM_E_ARG;
     const size_t elem = wm_dtype_size(type);
     if (!elem) return wm_set_error(ctx, WM_E_UNSUPPORTED_TYPE, "%s: type %d is not F32, F16 or BF16", who, type);
-    if (vocab == 0 || vocab > MAX_VOCAB) return wm_set_error(ctx, WM_E_SHAPE, "%s: vocabulary of %u", who, vocab);
-    if ((uint64_t)n_rows * make_plan(n_rows, vocab, elem).parts > 0x7FFFFFFFu / NT)  // the launch counts threads in 32 bits
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: %u rows of %u", who, n_rows, vocab);
-    if (top_k > MAX_TOP || top_k > vocab)
-        return wm_set_error(ctx, WM_E_SHAPE, "%s: top_k %u of %u tokens, %u at most", who, top_k, vocab, MAX_TOP);
+    if (wm_status st = check_sizes(ctx, elem, n_rows, vocab, top_k)) return st;
     if (n_rows > 1 && (row_stride < vocab || row_stride > 1ull << 40))
         return wm_set_error(ctx, WM_E_SHAPE, "%s: rows of %u values are %llu apart", who, vocab,
                             (unsigned long long)row_stride);
-    if (!top_k && (d_top_ids || d_top_logprobs))
-        return wm_set_error(ctx, WM_E_ARG, "%s: outputs for the top tokens with top_k 0", who);
-    if (!d_tokens && (d_logprob || d_rank))
-        return wm_set_error(ctx, WM_E_ARG, "%s: log probabilities or ranks of no tokens", who);
+    if (wm_status st = check_outputs(ctx, top_k, d_tokens, d_logprob, d_rank, d_top_ids, d_top_logprobs)) return st;
     if (n_rows == 0) return WM_OK;
     if (!d_logits) return wm_set_error(ctx, WM_E_ARG, "%s: null logits", who);
     if ((uintptr_t)d_logits % elem ||
@@ -631,12 +641,13 @@ wm_status wm_token_logprobs_dev(wm_ctx *ctx, int type, const void *d_logits, uin
 wm_status wm_token_logprobs(wm_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t vocab, const int32_t *tokens,
                             uint32_t top_k, float *logprob, float *entropy, int32_t *rank, int32_t *top_ids,
                             float *top_logprobs) {
-    static const char who[] = "token_logprobs";
     if (!ctx) return WM_E_ARG;
-    if (n_rows == 0 || vocab == 0 || !logits)  // the device form's words for these
+    if (n_rows == 0 || !logits)  // the device form's words for these
         return wm_token_logprobs_dev(ctx, WM_DTYPE_F32, logits, vocab, n_rows, vocab, tokens, top_k, logprob, entropy,
                                      rank, top_ids, top_logprobs, nullptr, 0);
-    if (top_k > MAX_TOP) return wm_set_error(ctx, WM_E_SHAPE, "%s: top_k %u, %u at most", who, top_k, MAX_TOP);
+    // (before anything is allocated or copied)
+    if (wm_status st = check_sizes(ctx, sizeof(float), n_rows, vocab, top_k)) return st;
+    if (wm_status st = check_outputs(ctx, top_k, tokens, logprob, rank, top_ids, top_logprobs)) return st;
     wm_device_guard dev(ctx->device);
     WM_HIP(ctx, dev.err);
     // one block of the context's scratch: logits, tokens, outputs, workspace

@@ -279,3 +279,17 @@ def test_attention_refuses_a_scale_without_a_base_2_form(hctx):
     kv, b = descriptors()
     for s in (2.4e38, -3.4e38):
         assert attend(hctx, kv, b, scale=s) == NONFINITE
+
+
+def test_logprobs_host_form_refuses_before_it_copies(hctx):
+    """Sizes that the device form refuses are refused before anything is allocated or read."""
+    x = np.zeros(5, np.float32)
+    p = x.ctypes.data_as(C.POINTER(C.c_float))
+    f = wh.lib.wm_token_logprobs
+    assert f(hctx, p, 1, (1 << 30) + 1, None, 0, None, None, None, None, None) == SHAPE
+    assert f(hctx, p, 1 << 31, 5, None, 0, None, None, None, None, None) == SHAPE
+    assert f(hctx, p, 1, 5, None, 6, None, None, None, None, None) == SHAPE
+    ids = (C.c_int32 * 5)()
+    assert f(hctx, p, 1, 5, None, 0, None, None, None, ids, None) == ARG
+    lp = (C.c_float * 5)()
+    assert f(hctx, p, 1, 5, None, 0, lp, None, None, None, None) == ARG
