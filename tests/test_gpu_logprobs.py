@@ -271,3 +271,22 @@ def test_logprobs_in_the_workspace_of_a_larger_call(ctx, kind):
             assert np.isnan(work.host()[size // 4:]).all()
         # its own size is enough too
         check(run(ctx, x, tok, k, kind), from_kind(x, kind), tok, k)
+
+
+@pytest.mark.parametrize("kind,rows,vocab", [("f32", 3, 128256), ("f32", 200, 50257), ("f16", 200, 128256), ("bf16", 2, 9999)])
+def test_logprobs_count_as_32_bits(ctx, kind, rows, vocab):
+    """Log probabilities to what their own additions and exponentials may be off by.
+
+    A lane adds up to 64 exponentials, 6 exchanges a wave, 3 additions the waves, 14 at most the parts: 87 roundings of
+    2^-24.  An exponential is good to 2^-23, and its argument, up to r / ln 2 for logits r apart, to 2^-24 and the
+    constant's 2^-26 of it: 2 + 1.25 r steps.  The sum's relative error is the logarithm's absolute one; the logarithm
+    and two differences add two steps of at most twice the largest value."""
+    rng = np.random.default_rng(12)
+    x = to_kind(rng.standard_normal((rows, vocab)) * 3, kind)
+    h = from_kind(x, kind)
+    tok = rng.integers(0, vocab, rows).astype(np.int32)
+    got = run(ctx, x, tok, 5, kind)
+    want = reference(h, tok, 5)
+    r = float(np.ptp(h))
+    for i in (0, 4):
+        assert np.all(np.abs(got[i] - want[i]) <= 2.0 ** -24 * (87 + 2 + 1.25 * r + 4 * 2 * np.abs(want[i])))

@@ -957,3 +957,47 @@ def test_many_sequences_next_to_a_long_bound(ctx):
     assert np.all(np.abs(out.host()[:used] - o[:used]) <= tol[:used])
     assert np.all(np.abs(lse.host()[:used] - z[:used]) <= tol_z[:used])
     assert np.all(out.host()[used:] == 7.0) and np.all(lse.host()[used:] == 7.0)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_appended_in_parts_stays_near_its_values(ctx, page):
+    """The same keys and values appended whole, in chunks and one at a time: other codes, as a block's earlier codes are
+    rounded again whenever its scale grows, but the same scales, and near the values.
+
+    A code is rounded once when it is stored, by half a step, and once for each later growth of its block's scale, by half
+    a step of the scale then, which is no larger than the last: (1 + growths) / 2 steps of the last scale."""
+    rng = np.random.default_rng(31)
+    kh, dim, n = 2, 64, 150
+    whole = Step(rng, [(0, n)], page, kh, dim)
+    pool = whole.pool(rng)
+    k, kx = typed(ctx, rng, (n, kh, dim), "f32")
+    pages = whole.table[0, :-(-n // page)]
+    codes = {}
+    for name, cuts in (("whole", [n]), ("chunks", [7, 20, 21, 64, 90, n]), ("single", list(range(1, n + 1)))):
+        d = Device(ctx, whole, pool)
+        growths, before = np.zeros((n, kh, 2), int), None
+        at = 0
+        for cut in cuts:
+            st = Step(rng, [(at, cut - at)], page, kh, dim)
+            st.table, st.stride, st.n_pages = whole.table, whole.stride, whole.n_pages
+            e = Device(ctx, st, pool)
+            e.pool, e.kv = d.pool, d.kv
+            part = (k, kh * dim, at * kh * dim)
+            e.append("f32", None, part, part, None)
+            scales = [x[pages] for x in e.host_pool()[2:]]
+            if before is not None:
+                for i in range(2):
+                    for p in range(at):
+                        growths[p, :, i] += scales[i][p // page] > before[i][p // page]
+            before, at = scales, cut
+        got = d.host_pool()
+        codes[name] = got
+        for h in range(kh):
+            for i, x in enumerate(ref.values(whole, got, 0, n, h)):
+                step = np.array([got[2 + i][whole.table[0, p // page], h] for p in range(n)], np.float64)
+                tol = step * (1 + growths[:, h, i]) / 2 * (1 + 1e-12)
+                assert np.all(np.abs(x - kx[:, h]) <= tol[:, None]), name
+        assert growths.any() == (name != "whole")
+    for name in ("chunks", "single"):
+        assert all(same_bits(codes[name][i][pages], codes["whole"][i][pages]) for i in (2, 3))
+        assert not same_bits(codes[name][0][pages], codes["whole"][0][pages])
