@@ -408,8 +408,11 @@ wm_status wm_server_release(wm_server *s, uint64_t request_id);
 /* No counterpart in the reference (its KVCache is one buffer per sequence
  * with a scale per position, src/model/kv_cache.rs:41-54): a cache in pages
  * that any number of sequences share, for one layer, and the attention that
- * reads it.  All arithmetic is f32 or wider; the results are those of the
- * formulas below up to rounding, not tied to a summation order.
+ * reads it.  Sums, maxima and logarithms are f32 or wider, and what is held in
+ * fewer bits is said at each call; the results are those of the formulas below
+ * up to rounding, not tied to a summation order.  They repeat exactly, but a
+ * sequence's attention may differ in its last bits from step to step with the
+ * others' lengths, which divide the work.
  *
  * Every pointer in these structs is device memory of the caller, which the
  * library reads or writes only during the work it enqueues on the context's
@@ -497,19 +500,22 @@ wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batc
  * itself, with q's stride).  n_heads = 0: no queries (q and q_out may be null).  rope null: no
  * rotation.  Pointers are 16-byte aligned and strides a multiple of 16 bytes.
  *
- * With r the rotated key (exact products and sum, rounded once to f32) or
- * the value, a block (page, head) that receives tokens gets
+ * With r the rotated key (exact products, their sum rounded to f64 and then to
+ * f32) or the value, a block (page, head) that receives tokens gets
  *   scale = max(its scale before, if positions before this step's first lie
  *               in it, else 0;  f32(max |r| over the finite new r / 127)),
  *   new codes  r / scale rounded half away from zero, within +-127
  *              (NaN: 0; scale 0: 0),
  *   and, where the scale grew, its earlier codes c * old scale / scale
  *   rounded the same way.
- * The quotients are rounded exactly.  Positions behind the last are left as
- * they were.  q_out is the rotated query, rounded to f32 and then to its type.
+ * The quotients are rounded exactly.  Earlier codes are rounded again each time
+ * their block's scale grows, by up to half a step of the new scale: the scales
+ * of a cache do not depend on how its tokens were divided into steps, its codes
+ * do.  Positions behind the last are left as they were.  q_out is the rotated query, rounded to f32 and then to its type.
  * A sequence whose lengths break their bounds is skipped; tokens of a page
  * outside the pool are not stored.  Two sequences must not append into one
- * page. */
+ * page.  The host sizes the launch by max_new for every sequence: a step of
+ * hundreds of sequences should not be given a bound far above its lengths. */
 wm_status wm_paged_kv_append_dev(wm_ctx *ctx, const wm_paged_kv *kv, const wm_paged_batch *batch,
                                  const wm_rope *rope, int type, const void *d_q, uint64_t q_stride,
                                  uint32_t n_heads, const void *d_k, uint64_t k_stride, const void *d_v,

@@ -16,9 +16,10 @@
 //
 // Measured (f32, 512 rows of 128256, top 5): 51 us, of which 46 are the parts
 // (263 MB, 5.7 TB/s; the chip's last cache holds some of it).  16-bit logits
-// are bound by the vector unit, about 7 operations and one exponential per
-// logit: 2047 rows of 50257 in bfloat16 (206 MB) take 57 us.  One row of
-// 128256, in 32 short parts, takes 12.5 us, the length of two launches' chains.
+// are nearer to the vector unit's rate: 14 instructions per logit, among them
+// an exponential, take 65 % of a SIMD's time; 2047 rows of 50257 in bfloat16
+// (206 MB) take 57 us.  One row of 128256, in 32 short parts, takes 12.5 us,
+// the length of two launches' chains.
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
@@ -528,7 +529,10 @@ __global__ __launch_bounds__(64) void k_logprobs_join_rows(lp_args a) {
 // How a row is divided: as few parts as its lanes' registers allow, and of
 // few rows parts a quarter as long.
 constexpr uint32_t LONG_PART = 64 * NT, SHORT_PART = 16 * NT;  // elements, at most
-constexpr uint32_t SMALL = 128;  // long parts of a call up to which it takes short ones
+// Long parts of a call up to which it takes short ones.  Long and short, f32
+// rows of 128256, top 20: 8 of them 15.8 us and 12.6, 128 16.1 and 13.6, 256
+// 16.4 and 15.8, 512 18.6 and 19.5, 1024 23.5 and 27.8.
+constexpr uint32_t SMALL = 128;
 struct lp_plan {
     bool small;
     uint32_t parts, part_vecs;

@@ -69,8 +69,8 @@ __device__ __forceinline__ unit_dims dims_of(int u, int n_rot, bool half) {
     d.b = split ? n_rot / 2 + 4 * u : 8 * u + 4;
     return d;
 }
-// The rotation of one unit's four pairs, products and sums exact in f64
-// (48-bit products, one rounding of their sum), rounded to f32.
+// The rotation of one unit's four pairs: products exact in f64 (48 bits), one
+// rounding of their sum to f64 and one of that to f32.
 __device__ __forceinline__ float rot_lo(float x, float y, float c, float s) {
     return (float)__builtin_fma((double)x, (double)c, -((double)y * (double)s));
 }
@@ -327,9 +327,11 @@ __global__ __launch_bounds__(NT) void k_paged_append(append_args a) {
     static_assert(PS * D % (16 * NT) == 0 || PS * D < 16 * NT, "whole units per thread");
     __shared__ float red[NT / 64];
     // Values, keys, queries: the longest chains first where all workgroups
-    // start at about the same time (24 ragged sequences 16.8 us, against 19.2
-    // with a block's kinds side by side), else a block's side by side, which
-    // read neighbouring rows (8 prompts 77 us against 92).
+    // start at about the same time, else a block's kinds side by side, which
+    // read neighbouring rows.  Both ways, first and side by side, in bf16
+    // pages of 64: a grid of 1440 12.1 us and 13.8, 4320 13.7 and 17.4, 7440
+    // 28.8 and 31.7; in f32 pages of 16: 1920 13.2 and 12.1, 6720 34.5 and
+    // 29.9, 15120 95 and 83.
     uint32_t kind, id;
     if (a.by_kind) kind = blockIdx.x / a.blocks, id = blockIdx.x % a.blocks;
     else if (a.group) kind = blockIdx.x % (2 + PS / 16), id = blockIdx.x / (2 + PS / 16);

@@ -8,8 +8,11 @@
 // largest) or two (f32: 22 bits).  A weight 2^(s - max) * v_scale comes out of
 // one exponential, the scale's logarithm in its argument: the product of
 // the scores becomes the argument by one fma.  It is one f16 term for half
-// outputs (2^-11, no more than the output's own rounding), two for f32.
-// Maxima, sums and accumulators are f32.
+// outputs, two for f32, which takes the second product twice.  One term is
+// rounded by up to 2^-11: an eighth of a bf16 output's own rounding (64 long
+// sequences are 0.0017 off 64 bits, as their plain form in f32 is), as much as
+// an f16 output's (8 prompts 0.00026, their plain form 0.00021).  Maxima, sums
+// and accumulators are f32.
 //
 // A wave holds scores transposed, S^T = K Q^T: lane l has query row l % 16
 // and 16 positions in a row, (l / 16) * 16 .. + 15 of a 64-position tile,
@@ -23,11 +26,12 @@
 // Measured with 20 query heads over 5 of 128 dims.  Few rows: 64 sequences of
 // 2000 to 16000 positions, bf16, 138 us, 726 MB of codes at 5.2 TB/s (the
 // bound; a large copy moves 4.7).  16 of 128 to 4064, f32, 18.4 us, and one of
-// 1024, 9.8 us: the length of two launches' chains (lengths, page id, codes,
-// scores, exponentials, the join).  Many rows: one prompt of 8192, bf16, 408
-// to 421 us, 820 TFLOP/s of products: a wave's exponentials, conversions and
-// masks take about as long as its products, two waves on a SIMD overlap them
-// in part.  16 sequences of 1 to 32 rows over up to 4064 positions, f32, 46 us.
+// 1024, 9.9 us: the length of two launches' chains (lengths, page id, codes,
+// scores, exponentials, the join).  Many rows: one prompt of 8192, bf16, 416
+// to 426 us, 815 TFLOP/s of products: a SIMD runs vector instructions
+// (exponentials, conversions, masks) for 53 % of that time and its matrix core
+// for 35 %, which two waves overlap only in part.  16 sequences of 1 to 32
+// tokens over up to 4064 positions, f32, 46 us.
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
@@ -41,8 +45,12 @@ constexpr int TILE = 64;   // positions per tile of one wave
 constexpr float W_EXP = 7.0f;   // the largest weight is 2^W_EXP when the sums are scaled,
 constexpr float W_MOST = 15.0f; // and may grow to this before they are scaled anew (f16 ends at 2^16)
 constexpr int E_NONE = -1000;   // the exponent of a zero scale
-constexpr int FEW = 16;    // rows (tokens x group) of a sequence and kv head up to which a wave takes them all
-constexpr int MANY = 128;  // rows of a workgroup beyond
+// Rows (tokens x group) of a sequence and kv head up to which a wave takes
+// them all, one tile of the matrix instruction, and rows of a workgroup beyond.
+// 16 sequences over 128 to 4064 positions, f32: 16 rows each 23.1 us, 20 rows
+// 35.2, 64 rows 43.1, 128 rows 47.6.
+constexpr int FEW = 16;
+constexpr int MANY = 128;
 
 struct attn_args {
     wm_paged_kv kv;
