@@ -497,8 +497,9 @@ wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batc
  * queries.  q [n_tokens][n_heads][head_dim], k and v [n_tokens][n_kv_heads]
  * [head_dim] of `type` (wm_dtype), tokens q_stride, k_stride and v_stride
  * elements apart (parts of one fused row are fine); q_out like q (may be q
- * itself, with q's stride).  n_heads = 0: no queries (q and q_out may be null).  rope null: no
- * rotation.  Pointers are 16-byte aligned and strides a multiple of 16 bytes.
+ * itself, with q's stride).  n_heads = 0: no queries (q and q_out may be null).
+ * rope null: no rotation.  Pointers are 16-byte aligned and strides a multiple
+ * of 16 bytes.
  *
  * With r the rotated key (exact products, their sum rounded to f64 and then to
  * f32) or the value, a block (page, head) that receives tokens gets
@@ -511,7 +512,8 @@ wm_status wm_paged_batch_check(const wm_paged_kv *kv, const wm_paged_batch *batc
  * The quotients are rounded exactly.  Earlier codes are rounded again each time
  * their block's scale grows, by up to half a step of the new scale: the scales
  * of a cache do not depend on how its tokens were divided into steps, its codes
- * do.  Positions behind the last are left as they were.  q_out is the rotated query, rounded to f32 and then to its type.
+ * do.  Positions behind the last are left as they were.  q_out is the rotated
+ * query, rounded to f32 and then to its type.
  * A sequence whose lengths break their bounds is skipped; tokens of a page
  * outside the pool are not stored.  Two sequences must not append into one
  * page.  The host sizes the launch by max_new for every sequence: a step of

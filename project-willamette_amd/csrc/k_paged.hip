@@ -414,7 +414,7 @@ uint32_t touched_pages(const wm_paged_kv *kv, const wm_paged_batch *b) {
 // launches: the host knows no lengths, only their bound.
 wm_status launch_seqs(wm_ctx *ctx, const char *who, const wm_paged_kv *kv, const wm_paged_batch *b, uint32_t *seqs) {
     const uint64_t one = (uint64_t)touched_pages(kv, b) * kv->n_kv_heads, most = 0x7FFFFFFFull / NT / 6;
-    if (one > most || b->n_seqs > most)
+    if (one > most || (one && b->n_seqs > most))
         return wm_set_error(ctx, WM_E_SHAPE, "%s: %u sequences of up to %llu blocks", who, b->n_seqs, (unsigned long long)one);
     *seqs = one ? (uint32_t)(most / one) : 0;
     return WM_OK;
