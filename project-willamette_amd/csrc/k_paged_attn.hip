@@ -25,9 +25,9 @@
 //
 // Measured with 20 query heads over 5 of 128 dims.  Few rows: 64 sequences of
 // 2000 to 16000 positions, bf16, 138 us, 726 MB of codes at 5.2 TB/s (the
-// bound; a large copy moves 4.7).  16 of 128 to 4064, f32, 18.4 us, and one of
-// 1024, 9.9 us: the length of two launches' chains (lengths, page id, codes,
-// scores, exponentials, the join).  Many rows: one prompt of 8192, bf16, 416
+// bound; a large copy moves 4.7).  16 of 128 to 4064, f32, 18.8 us, and one of
+// 1024, 10.0 us: the length of two launches' chains (lengths, page id, codes,
+// scores, exponentials, the join).  Many rows: one prompt of 8192, bf16, 414
 // to 426 us, 815 TFLOP/s of products: a SIMD runs vector instructions
 // (exponentials, conversions, masks) for 53 % of that time and its matrix core
 // for 35 %, which two waves overlap only in part.  16 sequences of 1 to 32
@@ -122,15 +122,17 @@ struct few_share {
         total *= a.kv.n_kv_heads;
         per = total <= a.few_blocks ? 1 : (total + FEW_RESIDENT - 1) / FEW_RESIDENT;
     }
-    // The sequence that round x is of, its rounds and the first of them.
+    // The sequence that round x is of, its rounds and the first of them; no
+    // rounds where none has it, as lengths that change under the kernel leave
+    // it: the search ends whatever it reads.
     struct place {
         wm_seq q;
-        uint32_t s, rounds, first;
+        uint32_t s, rounds = 0, first;
     };
     __device__ __forceinline__ place find(const attn_args &a, uint32_t x) const {
         uint32_t base = 0, m = mine, u = upto;
         wm_seq at = q;
-        for (uint32_t s = 0;; s += 64) {
+        for (uint32_t s = 0; s < a.b.n_seqs; s += 64) {
             if (s) scan(a, s, at, m, u);
             const uint64_t hit = __ballot(base + u * a.kv.n_kv_heads > x);
             if (hit) {
@@ -145,6 +147,7 @@ struct few_share {
             }
             base += __builtin_amdgcn_readlane(u, 63) * a.kv.n_kv_heads;
         }
+        return place();
     }
     // Where workgroup w leaves its part of a unit (sequence, kv head): along
     // the runs either grows by one at a time.
@@ -593,6 +596,7 @@ __device__ __forceinline__ void attend_few(const attn_args &a, uint32_t w, few_s
     const uint32_t end = uniform(min((w + 1) * all.per, all.total));
     for (uint32_t x = uniform(w * all.per); x < end;) {
         const auto f = all.find(a, x);
+        if (f.rounds == 0) return;
         // its kv heads from round x on
         while (x < end && x < f.first + f.rounds * a.kv.n_kv_heads) {
             const uint32_t h = uniform((x - f.first) / f.rounds), k0 = x - f.first - h * f.rounds;
@@ -635,7 +639,8 @@ struct many_order {
     __device__ __forceinline__ uint32_t from_level(uint32_t l) const {
         return wm_wave_total_i32(min(low + tiles > l ? low + tiles - l : 0, tiles));
     }
-    // Tile y: its sequence and row tile; false past the last.
+    // Tile y: its sequence and row tile; false past the last (and where lengths
+    // change under the kernel).
     __device__ __forceinline__ bool find(const attn_args &a, uint32_t y, wm_seq &seq, uint32_t &s, uint32_t &rt) {
         const bool one = a.b.n_seqs <= 64;
         auto count = [&](uint32_t l) {
@@ -655,7 +660,7 @@ struct many_order {
             else above = mid;
         }
         uint32_t left = y - count(l + 1);  // among the tiles of level l, one of a sequence at most
-        for (uint32_t s0 = 0;; s0 += 64) {
+        for (uint32_t s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
             if (!one) load(a, s0);
             const bool has = low <= l && l < low + tiles;
             const uint64_t mask = __ballot(has);
@@ -672,6 +677,7 @@ struct many_order {
             }
             left -= n;
         }
+        return false;
     }
 };
 
